@@ -299,6 +299,81 @@ int mup_probe_load_latency(const void *zeros, int iters, uint64_t *out_ns, void 
 int mup_regroup_rows_synced(void *dst, const void *src, int up, int batch, int64_t seq,
                             int64_t row_elems, int to_batch_major, void *stream, mup_sync *sync);
 
+/* ---- sliding-window attention with sinks --------------------------------------- */
+
+/* The attention between a peer-write projection (whose result it takes) and a
+ * head-shard pull projection (which takes its result); the reference leaves it
+ * to the caller. Row i of a sequence with Lq queries and Lk keys stands at
+ * position at = i + Lk - Lq and sees key j < Lk when (not causal or j <= at) and
+ * (j < sinks or at - left <= j <= at + right):
+ *     out = softmax(scale * q k^T over the visible keys) v,
+ *     lse = log sum exp of the same (natural logarithm).
+ * A row that sees no key has out 0 and lse -inf. Query head h uses key/value
+ * head h / (heads_q / heads_kv). Strides are in elements, for {sequence of the
+ * batch, row, head}; the head dimension is contiguous; every base address and
+ * stride is a multiple of 16 bytes.
+ *
+ * Dense form: sequences == NULL, `batch` sequences of seq_q queries and seq_k
+ * keys; kv_lengths (device, optional) then holds the number of keys of each
+ * sequence that count, the first ones. Packed form: batch = 1, seq_q and seq_k are
+ * the total rows and `sequences` (device) holds, per sequence, {first query row,
+ * queries, first key row, keys}; the tile lists hold {sequence, first row} of the
+ * blocks of 256 and 128 query rows and of 128 key rows of every sequence. */
+typedef struct mup_window_attention {
+  int32_t device;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim; /* a multiple of 8, at most 128 */
+  int32_t seq_q;
+  int32_t seq_k;
+  int32_t causal;
+  int32_t left;  /* keys before the own position; negative: no limit */
+  int32_t right; /* keys behind it; negative: no limit; ignored when causal */
+  int32_t sinks;
+  float scale;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t out_strides[3];
+  int64_t dout_strides[3];
+  int64_t dq_strides[3];
+  int64_t dk_strides[3];
+  int64_t dv_strides[3];
+  const void *q;
+  const void *k;
+  const void *v;
+  void *out;
+  float *lse; /* [batch, heads_q, seq_q]; optional in the forward pass */
+  const void *dout;
+  void *dq;
+  void *dk;
+  void *dv;
+  const int32_t *kv_lengths;
+  const int32_t *sequences;
+  const int32_t *q_blocks_256;
+  const int32_t *q_blocks_128;
+  const int32_t *k_blocks_128;
+  int32_t n_sequences;
+  int32_t n_q_blocks_256;
+  int32_t n_q_blocks_128;
+  int32_t n_k_blocks_128;
+  int32_t longest_q; /* packed: the longest sequence's queries and keys */
+  int32_t longest_k;
+  void *workspace; /* device, 16-byte aligned, contents need not be set */
+  uint64_t workspace_bytes;
+  uint64_t timeout_ns; /* bound of the waits inside the kernels */
+} mup_window_attention;
+
+/* Bytes of workspace the two passes need for this problem (host arithmetic; the
+ * pointers need not be set). Either output pointer may be NULL. */
+int mup_window_attention_workspace(const mup_window_attention *args, uint64_t *forward_bytes,
+                                   uint64_t *backward_bytes);
+int mup_window_attention_forward(const mup_window_attention *args, void *stream);
+/* From q, k, v, out, lse and dout: dq, dk, dv, each written whole (rows that take
+ * no part become 0). Deterministic. kv_lengths must be NULL. */
+int mup_window_attention_backward(const mup_window_attention *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

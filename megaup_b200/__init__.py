@@ -14,6 +14,13 @@ The device code is hand-written sm_100a CUDA in ``libmegaup.so`` (C ABI in
 ``include/megaup.h``); this package is the host side.
 """
 
+from .attention import (
+    PackedSequences,
+    prepare_packed_sequences,
+    window_attention_bshd,
+    window_attention_sbhd,
+    window_attention_thd,
+)
 from .ops import (
     PreparedHeadShardPullGemm,
     PreparedHeadShardPullGemmSBHD,
@@ -54,6 +61,7 @@ __all__ = [
     "DEFAULT_MAX_ROWS",
     "SUPPORTED_UP_DEGREES",
     "MegaUPRuntime",
+    "PackedSequences",
     "PreparedHeadShardPullGemm",
     "PreparedHeadShardPullGemmSBHD",
     "PreparedHeadShardPullGemmTHD",
@@ -74,10 +82,14 @@ __all__ = [
     "prepare_headshard_pull_gemm_bshd",
     "prepare_headshard_pull_gemm_sbhd",
     "prepare_headshard_pull_gemm_thd",
+    "prepare_packed_sequences",
     "prepare_peer_write_gemm_bshd",
     "prepare_peer_write_gemm_sbhd",
     "prepare_peer_write_gemm_thd",
     "prepare_thd_layout",
     "supports_shape",
     "unsupported_shape_reason",
+    "window_attention_bshd",
+    "window_attention_sbhd",
+    "window_attention_thd",
 ]

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_int, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 # MEGAUP_LIBRARY names another build of the library (A/B comparisons of kernel variants).
@@ -47,6 +47,28 @@ class MupSync(ctypes.Structure):
         ("done_before", c_uint64),
         ("done_after", c_uint64),
         ("status_device_ptr", c_void_p),
+        ("timeout_ns", c_uint64),
+    ]
+
+
+class MupWindowAttention(ctypes.Structure):
+    """``mup_window_attention`` of include/megaup.h."""
+
+    _fields_ = [
+        *((name, c_int32) for name in (
+            "device", "batch", "heads_q", "heads_kv", "head_dim", "seq_q", "seq_k", "causal", "left", "right", "sinks",
+        )),
+        ("scale", ctypes.c_float),
+        *((name + "_strides", c_int64 * 3) for name in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")),
+        *((name, c_void_p) for name in (
+            "q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "kv_lengths", "sequences", "q_blocks_256",
+            "q_blocks_128", "k_blocks_128",
+        )),
+        *((name, c_int32) for name in (
+            "n_sequences", "n_q_blocks_256", "n_q_blocks_128", "n_k_blocks_128", "longest_q", "longest_k",
+        )),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_uint64),
         ("timeout_ns", c_uint64),
     ]
 
@@ -131,6 +153,12 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
         c_int,
         (c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_void_p),
     ),
+    "mup_window_attention_workspace": (
+        c_int,
+        (POINTER(MupWindowAttention), POINTER(c_uint64), POINTER(c_uint64)),
+    ),
+    "mup_window_attention_forward": (c_int, (POINTER(MupWindowAttention), c_void_p)),
+    "mup_window_attention_backward": (c_int, (POINTER(MupWindowAttention), c_void_p)),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -18,8 +18,8 @@ INCLUDE = PACKAGE_DIR.parent / "include"
 LIB_DIR = PACKAGE_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmegaup.so"
 
-SOURCES = (CSRC / "mup_api.cu",)
-HEADERS = (CSRC / "mup_ptx.cuh", CSRC / "mup_gemm.cuh", INCLUDE / "megaup.h")
+SOURCES = (CSRC / "mup_api.cu", CSRC / "mup_attention.cu")
+HEADERS = (*sorted(CSRC.glob("*.cuh")), INCLUDE / "megaup.h")
 
 NVCC_FLAGS = (
     "-gencode",
@@ -32,6 +32,8 @@ NVCC_FLAGS = (
     "-fPIC",
     "-cudart",
     "static",
+    "--threads",
+    "0",
 )
 
 

@@ -22,6 +22,7 @@
 
 #include "../../include/megaup.h"
 #include "mup_gemm.cuh"
+#include "mup_host.cuh"
 
 namespace {
 
@@ -134,6 +135,76 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t oute
   if (r != CUDA_SUCCESS) return driver_fail("cuTensorMapEncodeTiled", r);
   return MUP_OK;
 }
+
+}  // namespace
+
+namespace mup {
+
+int host_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const int64_t strides[3],
+                  const uint32_t box[4]) {
+  const DriverApi& d = driver();
+  if (!d.ok) return fail(MUP_ERR_DRIVER, "%s", d.error);
+  cuuint64_t sizes[4], bytes[3];
+  cuuint32_t boxes[4], steps[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    sizes[i] = dims[i];
+    boxes[i] = box[i];
+  }
+  for (int i = 0; i < 3; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  CUresult r = d.tensor_map_encode_tiled(
+      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), sizes, bytes, boxes, steps,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return driver_fail("cuTensorMapEncodeTiled", r);
+  return MUP_OK;
+}
+
+int device_status_word(int device, uint32_t** device_ptr) {
+  constexpr int kMaxDevices = 64;
+  static std::mutex mutex;
+  static uint32_t* host[kMaxDevices];
+  static uint32_t* mapped[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return fail(MUP_ERR_BAD_ARG, "device ordinal %d is out of range", device);
+  uint32_t* word = __atomic_load_n(&host[device], __ATOMIC_ACQUIRE);
+  if (word == nullptr) {
+    std::lock_guard<std::mutex> lock(mutex);
+    word = host[device];
+    if (word == nullptr) {
+      // a pinned allocation is no stream operation: allowed while a stream is being captured
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      MUP_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+      void *h = nullptr, *m = nullptr;
+      cudaError_t e = cudaHostAlloc(&h, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+      if (e == cudaSuccess) e = cudaHostGetDevicePointer(&m, h, 0);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e != cudaSuccess) return fail(MUP_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
+      memset(h, 0, 64);
+      mapped[device] = static_cast<uint32_t*>(m);
+      word = static_cast<uint32_t*>(h);
+      __atomic_store_n(&host[device], word, __ATOMIC_RELEASE);
+    }
+  }
+  *device_ptr = mapped[device];
+  const uint32_t seen = __atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL);
+  if (seen != 0)
+    return fail(MUP_ERR_DEVICE_STATUS,
+                "an earlier kernel of device %d gave up on a bounded wait (code %u, detail %u): the results of the "
+                "operations enqueued since are invalid",
+                device, seen >> 24, seen & 0xffffffu);
+  return MUP_OK;
+}
+
+}  // namespace mup
+
+namespace {
 
 // Rows per pull ticket: the largest power of two (at most 16) whose shard rows
 // fit one batch of 512 sixteen-byte peer loads per warp.

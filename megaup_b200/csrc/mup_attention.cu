@@ -1,0 +1,193 @@
+// C ABI of the sliding-window attention with sinks (include/megaup.h):
+// argument checks, tensor maps, the split of the work and the launches.
+#include <algorithm>
+
+#include "mup_attn_forward.cuh"
+#include "mup_host.cuh"
+
+namespace {
+
+using namespace mup;
+
+constexpr int kSms = 148;
+constexpr int kMaxLength = 1 << 29;  // positions plus a window side stay inside 32 bits
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+int padded_dim(const mup_window_attention& a) { return a.head_dim <= 64 ? 64 : 128; }
+
+int64_t total_rows(const mup_window_attention& a) { return static_cast<int64_t>(a.batch) * a.heads_q * a.seq_q; }
+
+int check_problem(const mup_window_attention* args) {
+  if (args == nullptr) return host_fail(MUP_ERR_BAD_ARG, "window attention: null argument");
+  const mup_window_attention& a = *args;
+  if (a.head_dim < 8 || a.head_dim > 128 || a.head_dim % 8 != 0)
+    return host_fail(MUP_ERR_UNSUPPORTED, "window attention: head_dim %d is not a multiple of 8 up to 128", a.head_dim);
+  if (a.batch < 1 || a.heads_q < 1 || a.heads_kv < 1 || a.heads_q % a.heads_kv != 0)
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: batch %d, heads %d / %d", a.batch, a.heads_q, a.heads_kv);
+  if (a.seq_q < 1 || a.seq_k < 1 || a.seq_q > kMaxLength || a.seq_k > kMaxLength)
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: %d queries and %d keys (1 .. %d)", a.seq_q, a.seq_k, kMaxLength);
+  if (a.sinks < 0 || !(a.scale > 0.0f) || a.scale > 1e30f)
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: sinks %d, scale %g", a.sinks, static_cast<double>(a.scale));
+  if (a.sequences != nullptr) {
+    if (a.batch != 1 || a.kv_lengths != nullptr || a.n_sequences < 1 || a.longest_q < 1 || a.longest_q > a.seq_q ||
+        a.longest_k < 0 || a.longest_k > a.seq_k || a.n_q_blocks_256 < 1 || a.n_q_blocks_128 < a.n_q_blocks_256 ||
+        a.n_k_blocks_128 < 0)
+      return host_fail(MUP_ERR_BAD_ARG, "window attention: inconsistent packed sequences");
+  }
+  return MUP_OK;
+}
+
+int check_tensor(const char* name, const void* base, const int64_t strides[3]) {
+  if (base == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0)
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: %s is null or not 16-byte aligned", name);
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] <= 0 || strides[i] % 8 != 0 || strides[i] >= (1ll << 39))
+      return host_fail(MUP_ERR_BAD_ARG, "window attention: %s stride %lld is no positive multiple of 16 bytes", name,
+                       static_cast<long long>(strides[i]));
+  return MUP_OK;
+}
+
+AttnShape make_shape(const mup_window_attention& a, uint32_t* status) {
+  AttnShape s{};
+  s.batch = a.batch, s.heads_q = a.heads_q, s.heads_kv = a.heads_kv;
+  s.seq_q = a.seq_q, s.seq_k = a.seq_k, s.head_dim = a.head_dim;
+  s.causal = a.causal != 0;
+  s.left = a.left < 0 ? kNoLimit : std::min(a.left, kNoLimit);
+  s.right = s.causal ? 0 : a.right < 0 ? kNoLimit : std::min(a.right, kNoLimit);
+  // a window without a left limit holds the sinks that a causal row may see
+  s.sinks = s.causal && s.left == kNoLimit ? 0 : a.sinks;
+  s.scale = a.scale, s.scale_log2 = a.scale * kLog2e;
+  s.kv_lengths = a.kv_lengths;
+  s.sequences = reinterpret_cast<const int4*>(a.sequences);
+  s.status = status;
+  s.timeout_ns = a.timeout_ns != 0 ? a.timeout_ns : 5000000000ull;
+  return s;
+}
+
+// How a forward pass is cut into CTAs.
+struct ForwardPlan {
+  int packed_heads, pair_heads, single, head_sets, blocks, splits;
+  bool small_blocks;  // packed lists: blocks of 128 rows instead of 256
+};
+
+ForwardPlan plan_forward(const mup_window_attention& a) {
+  ForwardPlan f{};
+  const int group = a.heads_q / a.heads_kv;
+  const bool packed = a.sequences != nullptr;
+  const int queries = packed ? a.longest_q : a.seq_q;
+  // Few queries: the heads of a group share a sub-tile's 128 rows.
+  f.packed_heads = 1;
+  while (group % (2 * f.packed_heads) == 0 && 2 * f.packed_heads * queries <= kTileRows) f.packed_heads *= 2;
+  const int rows = kTileRows / f.packed_heads;
+  const int sets = group / f.packed_heads;
+  f.pair_heads = sets % 2 == 0;
+  f.single = !f.pair_heads && queries <= rows;
+  f.head_sets = a.heads_q / (f.packed_heads * (f.pair_heads ? 2 : 1));
+  f.small_blocks = f.pair_heads || f.single;
+  const int block_rows = f.small_blocks ? rows : 2 * rows;
+  f.blocks = packed ? (f.small_blocks ? a.n_q_blocks_128 : a.n_q_blocks_256) : a.batch * ceil_div(a.seq_q, block_rows);
+  // Too few CTAs for the GPU: several share a block's key tiles.
+  const AttnShape s = make_shape(a, nullptr);
+  const int keys = packed ? a.longest_k : a.seq_k;
+  const int64_t window = static_cast<int64_t>(s.left) + s.right + std::min(block_rows, queries);
+  const int tiles = std::max(1, std::min(ceil_div(keys, kTileRows),
+                                         ceil_div(std::min<int64_t>(window, keys), kTileRows) + 1 + ceil_div(std::min(s.sinks, keys), kTileRows)));
+  const int64_t ctas = static_cast<int64_t>(f.blocks) * f.head_sets;
+  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms / std::max<int64_t>(ctas, 1), ceil_div(tiles, 2))));
+  return f;
+}
+
+uint64_t forward_workspace(const mup_window_attention& a, const ForwardPlan& f) {
+  if (f.splits <= 1) return 0;
+  return static_cast<uint64_t>(f.splits) * total_rows(a) * (padded_dim(a) + 1) * sizeof(float);
+}
+
+int encode_rows(CUtensorMap* map, const mup_window_attention& a, const void* base, const int64_t strides[3], int rows,
+                int heads, int box_rows, int box_heads) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(a.head_dim), static_cast<uint64_t>(rows),
+                            static_cast<uint64_t>(heads), static_cast<uint64_t>(a.batch)};
+  const int64_t order[3] = {strides[1], strides[2], strides[0]};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(box_heads), 1};
+  return encode_map_4d(map, base, dims, order, box);
+}
+
+template <int DP>
+int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
+  const ForwardPlan f = plan_forward(a);
+  if (forward_workspace(a, f) > a.workspace_bytes || (f.splits > 1 && a.workspace == nullptr))
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: the workspace has %llu bytes, %llu are needed",
+                     static_cast<unsigned long long>(a.workspace_bytes),
+                     static_cast<unsigned long long>(forward_workspace(a, f)));
+  CUtensorMap q_map, k_map, v_map;
+  int rc = encode_rows(&q_map, a, a.q, a.q_strides, a.seq_q, a.heads_q, kTileRows / f.packed_heads, f.packed_heads);
+  if (rc == MUP_OK) rc = encode_rows(&k_map, a, a.k, a.k_strides, a.seq_k, a.heads_kv, kTileRows, 1);
+  if (rc == MUP_OK) rc = encode_rows(&v_map, a, a.v, a.v_strides, a.seq_k, a.heads_kv, kTileRows, 1);
+  if (rc != MUP_OK) return rc;
+  AttnForward p{};
+  p.shape = make_shape(a, status);
+  if (a.sequences != nullptr)
+    p.tiles = reinterpret_cast<const int2*>(f.small_blocks ? a.q_blocks_128 : a.q_blocks_256);
+  p.blocks_per_sequence = f.blocks / a.batch;
+  p.head_sets = f.head_sets, p.packed_heads = f.packed_heads, p.pair_heads = f.pair_heads;
+  p.splits = f.splits, p.single = f.single;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out_batch = a.out_strides[0], p.out_seq = a.out_strides[1], p.out_head = a.out_strides[2];
+  p.lse = a.lse;
+  p.total_rows = total_rows(a);
+  p.partial_out = static_cast<float*>(a.workspace);
+  p.partial_lse = p.partial_out + (f.splits > 1 ? f.splits * p.total_rows * DP : 0);
+  using Cfg = AttnForwardConfig<DP>;
+  static uint64_t ready = 0;
+  MUP_HOST_CUDA(allow_smem_once(attention_forward_kernel<DP>, Cfg::kSmemBytes, a.device, &ready));
+  const int64_t grid = static_cast<int64_t>(f.blocks) * f.head_sets * f.splits;
+  if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many row blocks");
+  attention_forward_kernel<DP><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map);
+  MUP_HOST_CUDA(cudaGetLastError());
+  if (f.splits > 1) {
+    AttnCombine c{};
+    c.partial_out = p.partial_out, c.partial_lse = p.partial_lse, c.splits = f.splits;
+    c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = p.total_rows;
+    c.out = p.out, c.out_batch = p.out_batch, c.out_seq = p.out_seq, c.out_head = p.out_head, c.lse = p.lse;
+    attention_combine_kernel<DP><<<ceil_div(p.total_rows, 4), 128, 0, stream>>>(c);
+    MUP_HOST_CUDA(cudaGetLastError());
+  }
+  return MUP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mup_window_attention_workspace(const mup_window_attention* args, uint64_t* forward_bytes,
+                                   uint64_t* backward_bytes) {
+  const int rc = check_problem(args);
+  if (rc != MUP_OK) return rc;
+  if (forward_bytes != nullptr) *forward_bytes = forward_workspace(*args, plan_forward(*args));
+  if (backward_bytes != nullptr) *backward_bytes = 0;
+  return MUP_OK;
+}
+
+int mup_window_attention_forward(const mup_window_attention* args, void* stream) {
+  int rc = check_problem(args);
+  if (rc == MUP_OK) rc = check_tensor("q", args->q, args->q_strides);
+  if (rc == MUP_OK) rc = check_tensor("k", args->k, args->k_strides);
+  if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
+  if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
+  if (rc != MUP_OK) return rc;
+  DeviceScope scope(args->device);
+  MUP_HOST_CUDA(scope.error());
+  uint32_t* status = nullptr;
+  rc = device_status_word(args->device, &status);
+  if (rc != MUP_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return args->head_dim <= 64 ? launch_forward<64>(*args, s, status) : launch_forward<128>(*args, s, status);
+}
+
+int mup_window_attention_backward(const mup_window_attention* args, void* stream) {
+  (void)stream;
+  return check_problem(args) != MUP_OK ? MUP_ERR_BAD_ARG
+                                       : host_fail(MUP_ERR_UNSUPPORTED, "window attention: no backward pass yet");
+}
+
+}  // extern "C"

@@ -1,0 +1,456 @@
+// Forward pass of the sliding-window attention with sinks.
+//
+// A CTA computes two sub-tiles of 128 query rows against one stream of key and
+// value tiles of 128 rows: S = Q K^T and O += P V are tcgen05 products with
+// their accumulators in TMEM (2 x 128 columns of S, 2 x DP of O), P stays in
+// TMEM as the second product's left operand. While four warps turn one
+// sub-tile's S into P, the tensor pipe works on the other's.
+#pragma once
+
+#include "mup_attn_common.cuh"
+
+namespace mup {
+
+struct AttnForward {
+  AttnShape shape;
+  const int2* tiles;        // packed: {sequence, first row} per row block; null when dense
+  int blocks_per_sequence;  // dense: row blocks per sequence
+  int head_sets;            // heads_q / heads per CTA
+  int packed_heads;         // heads per sub-tile (a power of two): rows of a sub-tile = heads x rows_per_head
+  int pair_heads;           // sub-tile 1 holds the next heads (1) or the next rows (0)
+  int splits;               // CTAs that share one block's key tiles
+  int single;               // only sub-tile 0 exists
+  __nv_bfloat16* out;
+  int64_t out_batch, out_seq, out_head;
+  float* lse;               // [batch, heads, rows] or null
+  float* partial_out;       // [splits, total rows, DP], splits > 1
+  float* partial_lse;       // [splits, total rows], base 2
+  int64_t total_rows;       // batch * heads_q * seq_q
+};
+
+template <int DP>
+struct AttnForwardConfig {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kTileBytes = kPanels * kPanelBytes;
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffStages = 2 * kTileBytes;
+  static constexpr int kOffBars = kOffStages + kStages * kTileBytes;
+  // q full [2], stage full, stage empty, s full [2], p full [2], o done [2], drain
+  static constexpr int kBars = 2 + 2 * kStages + 6 + 1;
+  static constexpr int kOffWords = kOffBars + kBars * 8;
+  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kThreads = 384;
+  static constexpr int kTmemO = 256;
+};
+
+// Raise of the row maximum, in powers of two, up to which the old reference is kept: P is then at most 2^8, which
+// neither its BF16 rounding (relative) nor the FP32 sums mind, and O is rescaled only where it has to be.
+constexpr float kKeepMaximum = 8.0f;
+
+template <int DP>
+__global__ void __launch_bounds__(384, 1)
+    attention_forward_kernel(const __grid_constant__ AttnForward p, const __grid_constant__ CUtensorMap q_map,
+                             const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using Cfg = AttnForwardConfig<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto bar = [&](int i) { return base + Cfg::kOffBars + i * 8; };
+  const auto q_full = [&](int t) { return bar(t); };
+  const auto full = [&](int s) { return bar(2 + s); };
+  const auto empty = [&](int s) { return bar(2 + Cfg::kStages + s); };
+  const auto s_full = [&](int t) { return bar(2 + 2 * Cfg::kStages + t); };
+  const auto p_full = [&](int t) { return bar(4 + 2 * Cfg::kStages + t); };
+  const auto o_done = [&](int t) { return bar(6 + 2 * Cfg::kStages + t); };
+  const uint32_t drain = bar(8 + 2 * Cfg::kStages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
+
+  // ---- this CTA's block of rows, heads and share of the key tiles
+  int w = blockIdx.x;
+  const int split = w % p.splits;
+  w /= p.splits;
+  const int head_set = w % p.head_sets;
+  w /= p.head_sets;
+  int sequence, row0;
+  const int rows = kTileRows / p.packed_heads;  // rows of a head in a sub-tile
+  const int row_step = p.pair_heads ? 0 : rows;
+  if (p.tiles != nullptr) {
+    const int2 tile = p.tiles[w];
+    sequence = tile.x, row0 = tile.y;
+  } else {
+    // the last rows first: under a causal mask they have the most keys
+    sequence = w % p.shape.batch;
+    row0 = (p.blocks_per_sequence - 1 - w / p.shape.batch) * (p.single || p.pair_heads ? rows : 2 * rows);
+  }
+  const AttnSeq seq = load_sequence(p.shape, sequence);
+  const int batch = p.shape.sequences != nullptr ? 0 : sequence;
+  const int head0 = head_set * p.packed_heads * (p.pair_heads ? 2 : 1);
+  const int kv_head = head0 / (p.shape.heads_q / p.shape.heads_kv);
+  // a row block behind the sequence's end (packed lists hold none; an empty second sub-tile is usual)
+  bool exists[2];
+  RowSpan first[2], last[2];
+  TileList own[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r = row0 + t * row_step;
+    exists[t] = r < seq.nq && !(t == 1 && p.single);
+    first[t] = row_span(p.shape, seq, r);
+    last[t] = row_span(p.shape, seq, min(r + rows, seq.nq) - 1);
+    own[t] = make_tile_list(first[t], last[t]);
+    if (!exists[t]) own[t].sink_end = 0, own[t].low = 0, own[t].high = -1;
+  }
+  const TileList all = make_tile_list(first[0], exists[1] ? last[1] : last[0]);
+  const int per_split = (all.count + p.splits - 1) / p.splits;
+  const int begin = min(split * per_split, all.count), end = min(begin + per_split, all.count);
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    mbar_init(q_full(0), 1);
+    mbar_init(q_full(1), 1);
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), 128);
+      mbar_init(o_done(t), 1);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 9) {
+    tmem_alloc<1>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    fewer_registers<40>();
+    if (warp == 8 && elect_one_sync()) {
+      // ------------------------------------------------------------ TMA loads
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+      int loads = 0;
+      bool ok = true;
+      auto load_tile = [&](const CUtensorMap& map, int kt) {
+        const int s = loads % Cfg::kStages, use = loads / Cfg::kStages;
+        if (use > 0 && !ctl.wait(empty(s), (use - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) return false;
+        mbar_arrive_expect_tx(full(s), Cfg::kTileBytes);
+        const uint32_t dst = base + Cfg::kOffStages + s * Cfg::kTileBytes;
+#pragma unroll
+        for (int panel = 0; panel < Cfg::kPanels; ++panel)
+          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, seq.k0 + kt * kTileRows, kv_head, batch, full(s));
+        ++loads;
+        return true;
+      };
+      if (begin < end) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!exists[t]) continue;
+          mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
+#pragma unroll
+          for (int panel = 0; panel < Cfg::kPanels; ++panel)
+            tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
+                        seq.q0 + row0 + t * row_step, head0 + (p.pair_heads ? t * p.packed_heads : 0), batch,
+                        q_full(t));
+          if (t == 0) ok = load_tile(k_map, all.tile(begin));
+        }
+        for (int i = begin + 1; ok && i <= end; ++i) {
+          if (i < end) ok = load_tile(k_map, all.tile(i));
+          if (ok) ok = load_tile(v_map, all.tile(i - 1));
+        }
+      }
+      if (!ok) {  // the copies in flight end before this CTA's shared memory is given up
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (exists[t]) drain_barrier(q_full(t), 0);
+        for (int n = max(0, loads - Cfg::kStages); n < loads; ++n)
+          drain_barrier(full(n % Cfg::kStages), (n / Cfg::kStages) & 1);
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ products
+      const bool leader = elect_one_sync();
+      int loads = 0, steps[2] = {0, 0};
+      bool ok = true, pending[2] = {false, false};
+      for (int i = begin; ok && begin < end && i <= end; ++i) {
+        const int k_load = loads, v_load = i < end ? loads + 1 : loads;
+        const int ks = k_load % Cfg::kStages, vs = v_load % Cfg::kStages;
+        const uint32_t k_tile = base + Cfg::kOffStages + ks * Cfg::kTileBytes;
+        const uint32_t v_tile = base + Cfg::kOffStages + vs * Cfg::kTileBytes;
+        bool k_there = false, v_there = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t s_tmem = tmem + t * kTileRows;
+          if (i > begin && pending[t]) {
+            ok = ok && ctl.wait(p_full(t), (steps[t] - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
+            if (ok && !v_there) {
+              ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+              v_there = true;
+              // A value row that none of the block's rows sees (another sequence's, one behind the cache's filled
+              // part) has to be finite where P is 0: it becomes 0.
+              const int j0 = all.tile(i - 1) * kTileRows;
+              const bool inside = j0 >= all.low && j0 + kTileRows - 1 <= all.high;
+              if (ok && !inside && j0 + kTileRows > all.sink_end) {
+                const bool window = all.high >= all.low;
+                const int sinks = min(max(all.sink_end - j0, 0), kTileRows);
+                const int from = window ? min(max(all.low - j0, 0), kTileRows) : kTileRows;
+                const int to = window ? min(max(all.high + 1 - j0, 0), kTileRows) : kTileRows;
+                uint8_t* tile = smem + Cfg::kOffStages + vs * Cfg::kTileBytes;
+                zero_tile_rows<DP>(tile, sinks, max(sinks, from), lane);
+                zero_tile_rows<DP>(tile, max(sinks, to), kTileRows, lane);
+                fence_proxy_async_smem();
+                __syncwarp();
+              }
+            }
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (leader) {
+              umma_tmem_by_cols<DP>(tmem + Cfg::kTmemO + t * DP, s_tmem, 32, v_tile, steps[t] > 1);
+              umma_commit_1(o_done(t));
+            }
+            pending[t] = false;
+          }
+          if (i < end && exists[t] && sees_tile(own[t], all.tile(i))) {
+            if (steps[t] == 0) ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
+            if (ok && !k_there) {
+              ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+              k_there = true;
+            }
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (leader) {
+              umma_rows_by_rows<DP>(s_tmem, base + Cfg::kOffQ + t * Cfg::kTileBytes, k_tile);
+              umma_commit_1(s_full(t));
+            }
+            pending[t] = true;
+            ++steps[t];
+          }
+        }
+        if (!ok) break;
+        // tiles that neither sub-tile used are waited for all the same: their stage is refilled next
+        if (i < end && !k_there) ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+        if (ok && i > begin && !v_there) ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+        if (ok && leader) {
+          if (i < end) umma_commit_1(empty(ks));
+          if (i > begin) umma_commit_1(empty(vs));
+        }
+        loads += (i < end) + (i > begin);
+      }
+      if (!ok) {
+        if (leader) umma_commit_1(drain);
+        __syncwarp();
+        drain_barrier(drain, 0);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    more_registers<232>();
+    const int t = warp / 4;
+    const int quarter = warp % 4;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem + t * kTileRows + lane_base;
+    const uint32_t o_tmem = tmem + Cfg::kTmemO + t * DP + lane_base;
+    const int row = row0 + t * row_step + r % rows;
+    const int head = head0 + (p.pair_heads ? t * p.packed_heads : 0) + r / rows;
+    const bool mine = t == 0 ? exists[0] : exists[1];
+    const RowSpan my_first = t == 0 ? first[0] : first[1], my_last = t == 0 ? last[0] : last[1];
+    const TileList my_tiles = t == 0 ? own[0] : own[1];
+    const bool valid = mine && row < seq.nq;
+    const RowSpan span = row_span(p.shape, seq, row);
+    const float c = p.shape.scale_log2;
+    float top = -INFINITY, sum = 0.0f;
+    int steps = 0;
+    bool ok = true;
+    for (int i = begin; mine && i < end; ++i) {
+      const int j0 = all.tile(i) * kTileRows;
+      if (!sees_tile(my_tiles, all.tile(i))) continue;
+      if (!ctl.wait(s_full(t), steps & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      uint32_t raw[4][32];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) tmem_ld_32x32(s_tmem + b * 32, raw[b]);
+      tmem_ld_wait();
+      if (!tile_is_full(my_first, my_last, j0)) {
+        const int low = span.low - j0, high = span.high - j0, sink = span.sink - j0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const int j = b * 32 + x;
+            const bool seen = (j >= low && j <= high) || j < sink;
+            raw[b][x] = seen ? raw[b][x] : 0xff800000u;
+          }
+      }
+      float m4[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        float m = __uint_as_float(raw[b][0]);
+#pragma unroll
+        for (int x = 1; x < 32; ++x) m = fmaxf(m, __uint_as_float(raw[b][x]));
+        m4[b] = m;
+      }
+      const float seen_top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      // the reference of the exponents: kept while the maximum grows little
+      float factor = 1.0f;
+      bool rescale = false;
+      if (top == -INFINITY) {
+        top = seen_top;  // nothing was added yet
+      } else if ((seen_top - top) * c > kKeepMaximum) {
+        factor = exp2_sfu((top - seen_top) * c);
+        top = seen_top;
+        rescale = true;
+      }
+      if (__any_sync(0xffffffffu, rescale)) {
+        // all products into O so far have ended
+        if (!ctl.wait(o_done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        sum *= factor;
+#pragma unroll 1
+        for (int b = 0; b < DP / 16; ++b) {
+          uint32_t o[16];
+          tmem_ld_32x16(o_tmem + b * 16, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+          tmem_st_32x16(o_tmem + b * 16, o);
+        }
+      }
+      const float shift = top == -INFINITY ? 0.0f : -top * c;
+      const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
+      float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t(&packed)[16] = reinterpret_cast<uint32_t(&)[16]>(raw[b]);  // in place: entry x replaces a used one
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          float2 e = fma2(make_float2(__uint_as_float(raw[b][2 * x]), __uint_as_float(raw[b][2 * x + 1])), c2, shift2);
+          e.x = exp2_sfu(e.x);
+          e.y = exp2_sfu(e.y);
+          sums[x & 1] = add2(sums[x & 1], e);
+          packed[x] = pack_bf16(e.x, e.y);
+        }
+        tmem_st_32x16(s_tmem + b * 16, packed);
+      }
+      sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(p_full(t));
+      ++steps;
+    }
+    if (ok && steps > 0) ok = ctl.wait(o_done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT);
+    // ---- O / sum, rounded once
+    if (ok) {
+      tc_fence_after_sync();
+      const int64_t index = (static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + seq.q0 + row;
+      const float log2_sum = top * c + log2f(sum);
+      const float scale = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+      if (valid) {
+        const float lse2 = sum == 0.0f ? -INFINITY : log2_sum;
+        if (p.splits > 1)
+          p.partial_lse[split * p.total_rows + index] = lse2;
+        else if (p.lse != nullptr)
+          p.lse[index] = lse2 * 0.69314718055994531f;
+      }
+      __nv_bfloat16* out = p.out + batch * p.out_batch + (seq.q0 + row) * p.out_seq + head * p.out_head;
+      float* partial = p.partial_out + (split * p.total_rows + index) * DP;
+#pragma unroll 1
+      for (int b = 0; b < DP / 32; ++b) {
+        uint32_t o[32];
+        if (steps > 0) {
+          tmem_ld_32x32(o_tmem + b * 32, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0u;
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int x = 0; x < 32; x += 8) {
+          if (b * 32 + x >= p.shape.head_dim) break;
+          float v[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) v[y] = sum == 0.0f ? 0.0f : __uint_as_float(o[x + y]) * scale;
+          if (p.splits > 1) {
+            float4* dst = reinterpret_cast<float4*>(partial + b * 32 + x);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+            uint4 packed;
+            packed.x = pack_bf16(v[0], v[1]);
+            packed.y = pack_bf16(v[2], v[3]);
+            packed.z = pack_bf16(v[4], v[5]);
+            packed.w = pack_bf16(v[6], v[7]);
+            *reinterpret_cast<uint4*>(out + b * 32 + x) = packed;
+          }
+        }
+      }
+    }
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// Joins the partial results of `splits` CTAs per row, always in the same order: one warp per row.
+struct AttnCombine {
+  const float* partial_out;
+  const float* partial_lse;
+  int splits, row_floats, head_dim, heads_q, seq_q;
+  int64_t total_rows;
+  __nv_bfloat16* out;
+  int64_t out_batch, out_seq, out_head;
+  float* lse;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(128) attention_combine_kernel(const AttnCombine p) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (row >= p.total_rows) return;
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.partial_lse[s * p.total_rows + row]);
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  constexpr int kEach = DP / 32;
+  float acc[kEach] = {}, sum = 0.0f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float l = p.partial_lse[s * p.total_rows + row];
+    const float weight = l == -INFINITY ? 0.0f : exp2_sfu(l - top);
+    if (l == -INFINITY) continue;
+    sum += weight;
+    const float* src = p.partial_out + (s * p.total_rows + row) * DP + lane * kEach;
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) acc[x] += weight * src[x];
+  }
+  const int seq = static_cast<int>(row % p.seq_q);
+  const int64_t bh = row / p.seq_q;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+  __nv_bfloat16* out = p.out + (bh / p.heads_q) * p.out_batch + seq * p.out_seq + (bh % p.heads_q) * p.out_head;
+#pragma unroll
+  for (int x = 0; x < kEach; x += 2) {
+    const int d = lane * kEach + x;
+    if (d < p.head_dim) *reinterpret_cast<uint32_t*>(out + d) = pack_bf16(acc[x] * scale, acc[x + 1] * scale);
+  }
+}
+
+}  // namespace mup

@@ -1,0 +1,66 @@
+// Host-side helpers that the translation units of libmegaup.so share: the
+// thread's error message, 4-D tensor maps, and the word a kernel without a
+// caller-provided status word reports a failed wait in.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/megaup.h"
+
+namespace mup {
+
+// Stores the calling thread's error message and returns `code`.
+int host_fail(int code, const char* fmt, ...);
+
+#define MUP_HOST_CUDA(expr)                                                                       \
+  do {                                                                                            \
+    cudaError_t e_ = (expr);                                                                      \
+    if (e_ != cudaSuccess)                                                                        \
+      return ::mup::host_fail(MUP_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e_));      \
+  } while (0)
+
+// BF16 tensor [dim3, dim2, dim1, dim0] with dim0 contiguous -> 4-D tiled map
+// with the 128-byte swizzle; box dim0 is 64 elements. Strides in elements.
+int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const int64_t strides[3],
+                  const uint32_t box[4]);
+
+// The library's own status word of a device (pinned, device-mapped, created at
+// the device's first use, also under stream capture). Reports and clears a
+// failure that an earlier kernel of this device left there.
+int device_status_word(int device, uint32_t** device_ptr);
+
+// Makes `device` current for a scope.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&previous_) != cudaSuccess) previous_ = -1;
+    error_ = previous_ == device ? cudaSuccess : cudaSetDevice(device);
+    changed_ = error_ == cudaSuccess && previous_ != device && previous_ >= 0;
+  }
+  ~DeviceScope() {
+    if (changed_) cudaSetDevice(previous_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  cudaError_t error() const { return error_; }
+
+ private:
+  int previous_ = -1;
+  bool changed_ = false;
+  cudaError_t error_ = cudaSuccess;
+};
+
+// Launch attributes of a kernel are set once per device; `mask` is the static
+// word of one kernel.
+template <typename Kernel>
+inline cudaError_t allow_smem_once(Kernel kernel, int bytes, int device, uint64_t* mask) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (__atomic_load_n(mask, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(mask, bit, __ATOMIC_RELEASE);
+  return e;
+}
+
+}  // namespace mup
