@@ -2,6 +2,7 @@
 // argument checks, tensor maps, the split of the work and the launches.
 #include <algorithm>
 
+#include "mup_attn_backward.cuh"
 #include "mup_attn_forward.cuh"
 #include "mup_host.cuh"
 
@@ -155,6 +156,114 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
   return MUP_OK;
 }
 
+// How a backward pass is cut into CTAs.
+struct BackwardPlan {
+  int shared_tiles, shares;
+};
+
+BackwardPlan plan_backward(const mup_window_attention& a) {
+  const bool packed = a.sequences != nullptr;
+  const AttnShape s = make_shape(a, nullptr);
+  const int group = a.heads_q / a.heads_kv;
+  const int queries = packed ? a.longest_q : a.seq_q, keys = packed ? a.longest_k : a.seq_k;
+  const int key_tiles = ceil_div(keys, kTileRows);
+  const int64_t tiles = packed ? a.n_k_blocks_128 : static_cast<int64_t>(a.batch) * key_tiles;
+  const int64_t all_rows = static_cast<int64_t>(group) * ceil_div(queries, kTileRows);
+  const int64_t window = static_cast<int64_t>(s.left) + s.right + kTileRows;
+  const int64_t window_rows =
+      std::min(all_rows, static_cast<int64_t>(group) * (ceil_div(std::min<int64_t>(window, queries), kTileRows) + 1));
+  // A sink's tile is seen by every later row, other tiles by a window's rows: it is cut into shares of about as many
+  // query tiles. Too few key tiles for the GPU: all of them are cut.
+  const int64_t ctas = std::max<int64_t>(1, tiles * a.heads_kv);
+  BackwardPlan b{};
+  if (2 * ctas <= kSms) {
+    b.shared_tiles = key_tiles;
+    b.shares = static_cast<int>(std::min<int64_t>(kSms / ctas, ceil_div(all_rows, 2)));
+  } else if (s.sinks > 0 && keys > 0) {
+    const int64_t per_cta = std::max(window_rows, ctas * window_rows / (4 * kSms));
+    b.shared_tiles = ceil_div(std::min(s.sinks, keys), kTileRows);
+    b.shares = static_cast<int>(std::min<int64_t>(64, ceil_div(all_rows, per_cta)));
+  }
+  if (b.shares <= 1 || keys == 0) b.shared_tiles = 0, b.shares = 1;
+  return b;
+}
+
+uint64_t partial_floats(const mup_window_attention& a, const BackwardPlan& b) {
+  const int64_t sequences = a.sequences != nullptr ? a.n_sequences : a.batch;
+  return static_cast<uint64_t>(sequences) * a.heads_kv * b.shared_tiles * b.shares * 2 * kTileRows * padded_dim(a);
+}
+
+// lse2 and delta, then (16-byte aligned) the shares.
+uint64_t stat_floats(const mup_window_attention& a) { return (2 * static_cast<uint64_t>(total_rows(a)) + 3) / 4 * 4; }
+
+uint64_t backward_workspace(const mup_window_attention& a, const BackwardPlan& b) {
+  return (stat_floats(a) + partial_floats(a, b)) * sizeof(float);
+}
+
+template <int DP>
+int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
+  const BackwardPlan plan = plan_backward(a);
+  if (backward_workspace(a, plan) > a.workspace_bytes || a.workspace == nullptr)
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: the workspace has %llu bytes, %llu are needed",
+                     static_cast<unsigned long long>(a.workspace_bytes),
+                     static_cast<unsigned long long>(backward_workspace(a, plan)));
+  CUtensorMap q_map, k_map, v_map, do_map;
+  int rc = encode_rows(&q_map, a, a.q, a.q_strides, a.seq_q, a.heads_q, kTileRows, 1);
+  if (rc == MUP_OK) rc = encode_rows(&do_map, a, a.dout, a.dout_strides, a.seq_q, a.heads_q, kTileRows, 1);
+  if (rc == MUP_OK) rc = encode_rows(&k_map, a, a.k, a.k_strides, a.seq_k, a.heads_kv, kTileRows, 1);
+  if (rc == MUP_OK) rc = encode_rows(&v_map, a, a.v, a.v_strides, a.seq_k, a.heads_kv, kTileRows, 1);
+  if (rc != MUP_OK) return rc;
+  float* workspace = static_cast<float*>(a.workspace);
+
+  AttnDelta d{};
+  d.out = static_cast<const __nv_bfloat16*>(a.out), d.dout = static_cast<const __nv_bfloat16*>(a.dout);
+  d.out_batch = a.out_strides[0], d.out_seq = a.out_strides[1], d.out_head = a.out_strides[2];
+  d.dout_batch = a.dout_strides[0], d.dout_seq = a.dout_strides[1], d.dout_head = a.dout_strides[2];
+  d.lse = a.lse, d.lse2 = workspace, d.delta = workspace + total_rows(a);
+  d.total_rows = total_rows(a), d.heads_q = a.heads_q, d.seq_q = a.seq_q, d.head_dim = a.head_dim;
+
+  AttnBackward p{};
+  p.shape = make_shape(a, status);
+  const bool packed = a.sequences != nullptr;
+  p.q_blocks = reinterpret_cast<const int2*>(packed ? a.q_blocks_128 : nullptr);
+  p.k_blocks = reinterpret_cast<const int2*>(packed ? a.k_blocks_128 : nullptr);
+  p.n_q_blocks = packed ? a.n_q_blocks_128 : ceil_div(a.seq_q, kTileRows);
+  p.n_k_blocks = packed ? a.n_k_blocks_128 : ceil_div(a.seq_k, kTileRows);
+  p.n_sequences = packed ? a.n_sequences : a.batch;
+  p.shared_tiles = plan.shared_tiles, p.shares = plan.shares;
+  p.lse2 = d.lse2, p.delta = d.delta, p.partial = workspace + stat_floats(a);
+  p.dq = static_cast<__nv_bfloat16*>(a.dq), p.dk = static_cast<__nv_bfloat16*>(a.dk), p.dv = static_cast<__nv_bfloat16*>(a.dv);
+  p.dq_batch = a.dq_strides[0], p.dq_seq = a.dq_strides[1], p.dq_head = a.dq_strides[2];
+  p.dk_batch = a.dk_strides[0], p.dk_seq = a.dk_strides[1], p.dk_head = a.dk_strides[2];
+  p.dv_batch = a.dv_strides[0], p.dv_seq = a.dv_strides[1], p.dv_head = a.dv_strides[2];
+
+  const int64_t q_grid = static_cast<int64_t>(p.n_q_blocks) * (packed ? 1 : a.batch) * a.heads_q;
+  const int64_t shared_jobs = static_cast<int64_t>(p.n_sequences) * a.heads_kv * plan.shared_tiles * plan.shares;
+  const int64_t k_grid = shared_jobs + static_cast<int64_t>(a.heads_kv) *
+                                           (packed ? p.n_k_blocks : a.batch * (p.n_k_blocks - plan.shared_tiles));
+  if (std::max(q_grid, k_grid) > 0x7fffffff || total_rows(a) / 16 > 0x7fffffff)
+    return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many row blocks");
+  using DqCfg = AttnDqConfig<DP>;
+  using DkvCfg = AttnDkvConfig<DP>;
+  static uint64_t dq_ready = 0, dkv_ready = 0;
+  MUP_HOST_CUDA(allow_smem_once(attention_dq_kernel<DP>, DqCfg::kSmemBytes, a.device, &dq_ready));
+  MUP_HOST_CUDA(allow_smem_once(attention_dkv_kernel<DP>, DkvCfg::kSmemBytes, a.device, &dkv_ready));
+  attention_delta_kernel<<<ceil_div(total_rows(a), 16), 256, 0, stream>>>(d);
+  MUP_HOST_CUDA(cudaGetLastError());
+  attention_dq_kernel<DP><<<static_cast<unsigned>(q_grid), 384, DqCfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map, do_map);
+  MUP_HOST_CUDA(cudaGetLastError());
+  if (k_grid > 0) {
+    attention_dkv_kernel<DP><<<static_cast<unsigned>(k_grid), 384, DkvCfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map, do_map);
+    MUP_HOST_CUDA(cudaGetLastError());
+  }
+  if (plan.shared_tiles > 0) {
+    const int64_t quads = static_cast<int64_t>(p.n_sequences) * a.heads_kv * plan.shared_tiles * 2 * kTileRows * (DP / 4);
+    attention_dkv_join_kernel<DP><<<ceil_div(quads, 256), 256, 0, stream>>>(p);
+    MUP_HOST_CUDA(cudaGetLastError());
+  }
+  return MUP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -164,7 +273,7 @@ int mup_window_attention_workspace(const mup_window_attention* args, uint64_t* f
   const int rc = check_problem(args);
   if (rc != MUP_OK) return rc;
   if (forward_bytes != nullptr) *forward_bytes = forward_workspace(*args, plan_forward(*args));
-  if (backward_bytes != nullptr) *backward_bytes = 0;
+  if (backward_bytes != nullptr) *backward_bytes = backward_workspace(*args, plan_backward(*args));
   return MUP_OK;
 }
 
@@ -185,9 +294,26 @@ int mup_window_attention_forward(const mup_window_attention* args, void* stream)
 }
 
 int mup_window_attention_backward(const mup_window_attention* args, void* stream) {
-  (void)stream;
-  return check_problem(args) != MUP_OK ? MUP_ERR_BAD_ARG
-                                       : host_fail(MUP_ERR_UNSUPPORTED, "window attention: no backward pass yet");
+  int rc = check_problem(args);
+  if (rc != MUP_OK) return rc;
+  if (args->kv_lengths != nullptr) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: no gradient with kv_lengths");
+  if (args->lse == nullptr) return host_fail(MUP_ERR_BAD_ARG, "window attention: the backward pass needs lse");
+  rc = check_tensor("q", args->q, args->q_strides);
+  if (rc == MUP_OK) rc = check_tensor("k", args->k, args->k_strides);
+  if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
+  if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
+  if (rc == MUP_OK) rc = check_tensor("dout", args->dout, args->dout_strides);
+  if (rc == MUP_OK) rc = check_tensor("dq", args->dq, args->dq_strides);
+  if (rc == MUP_OK) rc = check_tensor("dk", args->dk, args->dk_strides);
+  if (rc == MUP_OK) rc = check_tensor("dv", args->dv, args->dv_strides);
+  if (rc != MUP_OK) return rc;
+  DeviceScope scope(args->device);
+  MUP_HOST_CUDA(scope.error());
+  uint32_t* status = nullptr;
+  rc = device_status_word(args->device, &status);
+  if (rc != MUP_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return args->head_dim <= 64 ? launch_backward<64>(*args, s, status) : launch_backward<128>(*args, s, status);
 }
 
 }  // extern "C"

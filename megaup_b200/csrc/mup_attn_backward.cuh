@@ -1,0 +1,736 @@
+// Backward pass of the sliding-window attention with sinks. With P = exp(S - lse) and delta = rowsum(dO * O):
+//     dP = dO V^T,  dS = P (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
+//
+// Two kernels recompute S and dP: one walks the key tiles of a block of query rows and sums dQ, one walks the query
+// tiles of a block of key rows (over all heads of the group) and sums dK and dV. That is seven products per pair of
+// tiles where a single kernel with a shared dQ would need five, but every sum stays in one CTA's TMEM: no atomics, no
+// FP32 gradient in memory, the same bits every time.
+#pragma once
+
+#include "mup_attn_common.cuh"
+
+namespace mup {
+
+struct AttnBackward {
+  AttnShape shape;
+  const int2* q_blocks;  // packed: {sequence, first row} per 128 query rows
+  const int2* k_blocks;  // packed: the same of the key rows
+  int n_q_blocks, n_k_blocks;  // packed: of the lists; dense: per sequence
+  int n_sequences;
+  // The first `shared_tiles` key tiles of every sequence are each computed by `shares` CTAs.
+  int shared_tiles, shares;
+  const float* lse2;   // [batch, heads, rows], base 2; +inf where a row sees nothing
+  const float* delta;  // the same shape
+  float* partial;      // [sequence, kv head, shared tile, share, {dV, dK}, 128, DP]
+  __nv_bfloat16 *dq, *dk, *dv;
+  int64_t dq_batch, dq_seq, dq_head, dk_batch, dk_seq, dk_head, dv_batch, dv_seq, dv_head;
+};
+
+// ---------------------------------------------------------------------------
+// delta and the base-2 log-sum-exp of every row: 16 lanes per row.
+// ---------------------------------------------------------------------------
+
+struct AttnDelta {
+  const __nv_bfloat16 *out, *dout;
+  int64_t out_batch, out_seq, out_head, dout_batch, dout_seq, dout_head;
+  const float* lse;
+  float *lse2, *delta;
+  int64_t total_rows;
+  int heads_q, seq_q, head_dim;
+};
+
+__device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float sum) {
+  sum = fmaf(__uint_as_float(a << 16), __uint_as_float(b << 16), sum);
+  return fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), sum);
+}
+
+__global__ void __launch_bounds__(256) attention_delta_kernel(const AttnDelta p) {
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 16;
+  const int part = threadIdx.x % 16;
+  // neighbouring half-warps take the heads of one row: their rows lie next to each other
+  const int64_t per_batch = static_cast<int64_t>(p.heads_q) * p.seq_q;
+  const int64_t b = item / per_batch;
+  const int64_t rest = item - b * per_batch;
+  const int64_t row = rest / p.heads_q;
+  const int head = static_cast<int>(rest - row * p.heads_q);
+  float sum = 0.0f;
+  if (item < p.total_rows && part * 8 < p.head_dim) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p.out + b * p.out_batch + row * p.out_seq + head * p.out_head + part * 8);
+    const uint4 y = *reinterpret_cast<const uint4*>(p.dout + b * p.dout_batch + row * p.dout_seq + head * p.dout_head + part * 8);
+    sum = dot_bf16x2(x.x, y.x, sum);
+    sum = dot_bf16x2(x.y, y.y, sum);
+    sum = dot_bf16x2(x.z, y.z, sum);
+    sum = dot_bf16x2(x.w, y.w, sum);
+  }
+#pragma unroll
+  for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (item < p.total_rows && part == 0) {
+    const int64_t index = (b * p.heads_q + head) * p.seq_q + row;
+    const float l = p.lse[index];
+    p.delta[index] = sum;
+    p.lse2[index] = l == -INFINITY ? INFINITY : l * kLog2e;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dQ
+// ---------------------------------------------------------------------------
+
+template <int DP>
+struct AttnDqConfig {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kTileBytes = kPanels * kPanelBytes;
+  static constexpr int kKStages = 3, kVStages = 2;
+  static constexpr int kOffQ = 0, kOffDo = kTileBytes, kOffK = 2 * kTileBytes;
+  static constexpr int kOffV = kOffK + kKStages * kTileBytes;
+  static constexpr int kOffBars = kOffV + kVStages * kTileBytes;
+  // q and dO full, k full/empty, v full/empty, s full [2], dp full, ds full, done, drain
+  static constexpr int kBars = 1 + 2 * kKStages + 2 * kVStages + 6;
+  static constexpr int kOffWords = kOffBars + kBars * 8;
+  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kTmemDp = 256, kTmemDq = 384;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(384, 1)
+    attention_dq_kernel(const __grid_constant__ AttnBackward p, const __grid_constant__ CUtensorMap q_map,
+                        const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                        const __grid_constant__ CUtensorMap do_map) {
+  using Cfg = AttnDqConfig<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto bar = [&](int i) { return base + Cfg::kOffBars + i * 8; };
+  const uint32_t q_full = bar(0);
+  const auto k_full = [&](int s) { return bar(1 + s); };
+  const auto k_empty = [&](int s) { return bar(1 + Cfg::kKStages + s); };
+  constexpr int kV = 1 + 2 * Cfg::kKStages;
+  const auto v_full = [&](int s) { return bar(kV + s); };
+  const auto v_empty = [&](int s) { return bar(kV + Cfg::kVStages + s); };
+  constexpr int kS = kV + 2 * Cfg::kVStages;
+  const auto s_full = [&](int b) { return bar(kS + b); };
+  const uint32_t dp_full = bar(kS + 2), ds_full = bar(kS + 3), done = bar(kS + 4), drain = bar(kS + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
+
+  const int head = blockIdx.x % p.shape.heads_q;
+  const int w = blockIdx.x / p.shape.heads_q;
+  int sequence, row0;
+  if (p.q_blocks != nullptr) {
+    const int2 block = p.q_blocks[w];
+    sequence = block.x, row0 = block.y;
+  } else {
+    sequence = w % p.shape.batch, row0 = (p.n_q_blocks - 1 - w / p.shape.batch) * kTileRows;
+  }
+  const AttnSeq seq = load_sequence(p.shape, sequence);
+  const int batch = p.shape.sequences != nullptr ? 0 : sequence;
+  const int kv_head = head / (p.shape.heads_q / p.shape.heads_kv);
+  const RowSpan first = row_span(p.shape, seq, row0);
+  const RowSpan last = row_span(p.shape, seq, min(row0 + kTileRows, seq.nq) - 1);
+  const TileList tiles = make_tile_list(first, last);
+  const int n = tiles.count;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    for (int i = 0; i < Cfg::kBars; ++i) mbar_init(bar(i), bar(i) == ds_full ? 256 : 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 9) {
+    tmem_alloc<1>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    fewer_registers<72>();
+    if (warp == 8 && elect_one_sync() && n > 0) {
+      bool ok = true;
+      int i = 0;
+      auto load = [&](const CUtensorMap& map, uint32_t dst, uint32_t full, int row, int h) {
+#pragma unroll
+        for (int panel = 0; panel < Cfg::kPanels; ++panel)
+          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, row, h, batch, full);
+      };
+      mbar_arrive_expect_tx(q_full, 2 * Cfg::kTileBytes);
+      load(q_map, base + Cfg::kOffQ, q_full, seq.q0 + row0, head);
+      load(do_map, base + Cfg::kOffDo, q_full, seq.q0 + row0, head);
+      for (; i < n; ++i) {
+        const int ks = i % Cfg::kKStages, vs = i % Cfg::kVStages;
+        const int row = seq.k0 + tiles.tile(i) * kTileRows;
+        if (i >= Cfg::kKStages && !ctl.wait(k_empty(ks), (i / Cfg::kKStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(k_full(ks), Cfg::kTileBytes);
+        load(k_map, base + Cfg::kOffK + ks * Cfg::kTileBytes, k_full(ks), row, kv_head);
+        if (i >= Cfg::kVStages && !ctl.wait(v_empty(vs), (i / Cfg::kVStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
+          drain_barrier(k_full(ks), (i / Cfg::kKStages) & 1);
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(v_full(vs), Cfg::kTileBytes);
+        load(v_map, base + Cfg::kOffV + vs * Cfg::kTileBytes, v_full(vs), row, kv_head);
+      }
+      if (!ok) {
+        drain_barrier(q_full, 0);
+        for (int m = max(0, i - Cfg::kKStages); m < i; ++m)
+          drain_barrier(k_full(m % Cfg::kKStages), (m / Cfg::kKStages) & 1);
+        for (int m = max(0, i - Cfg::kVStages); m < i; ++m)
+          drain_barrier(v_full(m % Cfg::kVStages), (m / Cfg::kVStages) & 1);
+      }
+    } else if (warp == 9 && n > 0) {
+      const bool leader = elect_one_sync();
+      // S of tile i goes to buffer i % 2, where dS replaces it; dP has one buffer.
+      auto score = [&](int i) {
+        const int ks = i % Cfg::kKStages;
+        if (!ctl.wait(k_full(ks), (i / Cfg::kKStages) & 1, MUP_ST_MMA_FULL_TIMEOUT)) return false;
+        zero_unseen_rows<DP>(smem + Cfg::kOffK + ks * Cfg::kTileBytes, tiles, tiles.tile(i) * kTileRows, lane);
+        tc_fence_after_sync();
+        if (leader) {
+          umma_rows_by_rows<DP>(tmem + (i & 1) * kTileRows, base + Cfg::kOffQ, base + Cfg::kOffK + ks * Cfg::kTileBytes);
+          umma_commit_1(s_full(i & 1));
+        }
+        return true;
+      };
+      auto score_gradient = [&](int i) {
+        const int vs = i % Cfg::kVStages;
+        if (!ctl.wait(v_full(vs), (i / Cfg::kVStages) & 1, MUP_ST_MMA_FULL_TIMEOUT)) return false;
+        tc_fence_after_sync();
+        if (leader) {
+          umma_rows_by_rows<DP>(tmem + Cfg::kTmemDp, base + Cfg::kOffDo, base + Cfg::kOffV + vs * Cfg::kTileBytes);
+          umma_commit_1(dp_full);
+          umma_commit_1(v_empty(vs));
+        }
+        return true;
+      };
+      bool ok = ctl.wait(q_full, 0, MUP_ST_MMA_FULL_TIMEOUT);
+      ok = ok && score(0) && score_gradient(0);
+      for (int i = 0; ok && i < n; ++i) {
+        if (i + 1 < n) ok = score(i + 1);
+        ok = ok && ctl.wait(ds_full, i & 1, MUP_ST_MMA_ACC_TIMEOUT);
+        if (ok && i + 1 < n) ok = score_gradient(i + 1);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          const int ks = i % Cfg::kKStages;
+          umma_tmem_by_cols<DP>(tmem + Cfg::kTmemDq, tmem + (i & 1) * kTileRows, 64,
+                                base + Cfg::kOffK + ks * Cfg::kTileBytes, i > 0);
+          umma_commit_1(k_empty(ks));
+          if (i + 1 == n) umma_commit_1(done);
+        }
+      }
+      if (!ok) {
+        if (leader) umma_commit_1(drain);
+        __syncwarp();
+        drain_barrier(drain, 0);
+      }
+    }
+  } else {
+    more_registers<216>();
+    // Two warpgroups share a tile's columns: thread = query row, 64 keys each.
+    const int half = warp / 4, quarter = warp % 4;
+    const int row = row0 + quarter * 32 + lane;
+    const bool valid = row < seq.nq;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const RowSpan span = row_span(p.shape, seq, row);
+    const int64_t index = (static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + seq.q0 + row;
+    const float c = p.shape.scale_log2;
+    const float shift = valid ? -p.lse2[index] : -INFINITY;
+    const float delta = valid ? p.delta[index] : 0.0f;
+    const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift), delta2 = make_float2(-delta, -delta);
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int j0 = tiles.tile(i) * kTileRows + half * 64;
+      const uint32_t s_tmem = tmem + (i & 1) * kTileRows + half * 64 + lane_base;
+      if (!ctl.wait(s_full(i & 1), (i >> 1) & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      const bool full = tile_is_full(first, last, tiles.tile(i) * kTileRows);
+      uint32_t s[2][32];
+      tmem_ld_32x32(s_tmem, s[0]);
+      tmem_ld_32x32(s_tmem + 32, s[1]);
+      tmem_ld_wait();
+      if (!full) {
+        const int low = span.low - j0, high = span.high - j0, sink = span.sink - j0;
+#pragma unroll
+        for (int x = 0; x < 64; ++x) {
+          const bool seen = (x >= low && x <= high) || x < sink;
+          s[x / 32][x % 32] = seen ? s[x / 32][x % 32] : 0xff800000u;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 64; x += 2) {
+        uint32_t& s0 = s[x / 32][x % 32];
+        uint32_t& s1 = s[x / 32][x % 32 + 1];
+        const float2 e = fma2(make_float2(__uint_as_float(s0), __uint_as_float(s1)), c2, shift2);
+        s0 = __float_as_uint(exp2_sfu(e.x));
+        s1 = __float_as_uint(exp2_sfu(e.y));
+      }
+      if (!ctl.wait(dp_full, i & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t g[32];
+        tmem_ld_32x32(tmem + Cfg::kTmemDp + half * 64 + b * 32 + lane_base, g);
+        tmem_ld_wait();
+        if (!full) {  // where P is 0 the value row may hold anything
+#pragma unroll
+          for (int x = 0; x < 32; ++x) g[x] = s[b][x] == 0u ? 0u : g[x];
+        }
+        uint32_t packed[16];
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) {
+          const float2 d = mul2(make_float2(__uint_as_float(s[b][x]), __uint_as_float(s[b][x + 1])),
+                                add2(make_float2(__uint_as_float(g[x]), __uint_as_float(g[x + 1])), delta2));
+          packed[x / 2] = pack_bf16(d.x, d.y);
+        }
+        tmem_st_32x16(s_tmem + b * 16, packed);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(ds_full);
+    }
+    if (ok && n > 0) ok = ctl.wait(done, 0, MUP_ST_EPILOGUE_TIMEOUT);
+    if (ok) {
+      tc_fence_after_sync();
+      __nv_bfloat16* dst = p.dq + batch * p.dq_batch + (seq.q0 + row) * p.dq_seq + head * p.dq_head;
+#pragma unroll 1
+      for (int b = 0; b < DP / 64; ++b) {
+        const int col = half * (DP / 2) + b * 32;
+        uint32_t g[32];
+        if (n > 0) {
+          tmem_ld_32x32(tmem + Cfg::kTmemDq + col + lane_base, g);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) g[x] = 0u;
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int x = 0; x < 32; x += 8) {
+          if (col + x >= p.shape.head_dim) break;
+          uint4 v;
+          uint32_t* words = &v.x;
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            words[y] = pack_bf16(__uint_as_float(g[x + 2 * y]) * p.shape.scale, __uint_as_float(g[x + 2 * y + 1]) * p.shape.scale);
+          *reinterpret_cast<uint4*>(dst + col + x) = v;
+        }
+      }
+    }
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV
+// ---------------------------------------------------------------------------
+
+template <int DP>
+struct AttnDkvConfig {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kTileBytes = kPanels * kPanelBytes;
+  static constexpr int kQStages = 3, kDoStages = 2, kStatStages = 2;
+  static constexpr int kOffK = 0, kOffV = kTileBytes, kOffQ = 2 * kTileBytes;
+  static constexpr int kOffDo = kOffQ + kQStages * kTileBytes;
+  static constexpr int kOffStats = kOffDo + kDoStages * kTileBytes;  // per stage: 128 lse2, 128 delta
+  static constexpr int kOffBars = kOffStats + kStatStages * 1024;
+  // k and v full, q full/empty, dO full/empty, stats full/empty, s, dp, p, ds full, done, drain
+  static constexpr int kBars = 1 + 2 * kQStages + 2 * kDoStages + 2 * kStatStages + 6;
+  static constexpr int kOffWords = kOffBars + kBars * 8;
+  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kTmemDp = 128, kTmemDv = 256, kTmemDk = 384;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(384, 1)
+    attention_dkv_kernel(const __grid_constant__ AttnBackward p, const __grid_constant__ CUtensorMap q_map,
+                         const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                         const __grid_constant__ CUtensorMap do_map) {
+  using Cfg = AttnDkvConfig<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto bar = [&](int i) { return base + Cfg::kOffBars + i * 8; };
+  const uint32_t kv_full = bar(0);
+  const auto q_full = [&](int s) { return bar(1 + s); };
+  const auto q_empty = [&](int s) { return bar(1 + Cfg::kQStages + s); };
+  constexpr int kD = 1 + 2 * Cfg::kQStages;
+  const auto do_full = [&](int s) { return bar(kD + s); };
+  const auto do_empty = [&](int s) { return bar(kD + Cfg::kDoStages + s); };
+  constexpr int kT = kD + 2 * Cfg::kDoStages;
+  const auto stat_full = [&](int s) { return bar(kT + s); };
+  const auto stat_empty = [&](int s) { return bar(kT + Cfg::kStatStages + s); };
+  constexpr int kS = kT + 2 * Cfg::kStatStages;
+  const uint32_t s_full = bar(kS), dp_full = bar(kS + 1), p_full = bar(kS + 2), ds_full = bar(kS + 3);
+  const uint32_t done = bar(kS + 4), drain = bar(kS + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
+
+  // ---- the key tile, and this CTA's share of the query tiles that see it
+  const int heads_kv = p.shape.heads_kv, group = p.shape.heads_q / heads_kv;
+  const int shared_jobs = p.n_sequences * heads_kv * p.shared_tiles * p.shares;
+  int job = blockIdx.x, sequence, tile, kv_head, share = 0, shares = 1;
+  if (job < shared_jobs) {
+    share = job % p.shares, shares = p.shares;
+    job /= p.shares;
+    tile = job % p.shared_tiles;
+    kv_head = job / p.shared_tiles % heads_kv;
+    sequence = job / p.shared_tiles / heads_kv;
+  } else {
+    job -= shared_jobs;
+    kv_head = job % heads_kv;
+    job /= heads_kv;
+    if (p.k_blocks != nullptr) {
+      const int2 block = p.k_blocks[job];
+      sequence = block.x, tile = block.y / kTileRows;
+      if (tile < p.shared_tiles) return;
+    } else {
+      sequence = job % p.shape.batch, tile = p.shared_tiles + job / p.shape.batch;
+    }
+  }
+  const AttnSeq seq = load_sequence(p.shape, sequence);
+  const int batch = p.shape.sequences != nullptr ? 0 : sequence;
+  const int j0 = tile * kTileRows;
+  if (j0 >= seq.nk) return;  // packed: a shared tile that this sequence does not have
+  // rows at `at` with at_low <= at <= at_high see something of the tile
+  const bool has_sinks = j0 < p.shape.sinks;
+  int i_low = (has_sinks && !p.shape.causal ? 0 : max(0, j0 - p.shape.right - seq.off));
+  if (has_sinks && p.shape.causal) i_low = max(0, j0 - seq.off);
+  const int j1 = min(j0 + kTileRows, seq.nk) - 1;
+  const int i_high = has_sinks ? seq.nq - 1 : min(seq.nq - 1, j1 + p.shape.left - seq.off);
+  const int q_tile0 = i_low / kTileRows;
+  const int q_tiles = i_high < i_low ? 0 : i_high / kTileRows - q_tile0 + 1;
+  const int steps = q_tiles * group;
+  const int per_share = (steps + shares - 1) / shares;
+  const int begin = min(share * per_share, steps), n = min(begin + per_share, steps) - begin;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    for (int i = 0; i < Cfg::kBars; ++i) {
+      const uint32_t b = bar(i);
+      const bool all_threads = b == p_full || b == ds_full || (b >= stat_empty(0) && b < s_full);
+      mbar_init(b, all_threads ? 256 : b >= stat_full(0) && b < stat_empty(0) ? 32 : 1);
+    }
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 9) {
+    tmem_alloc<1>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    fewer_registers<72>();
+    if (warp == 8 && elect_one_sync() && n > 0) {
+      bool ok = true;
+      int i = 0;
+      auto load = [&](const CUtensorMap& map, uint32_t dst, uint32_t full, int row, int h) {
+#pragma unroll
+        for (int panel = 0; panel < Cfg::kPanels; ++panel)
+          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, row, h, batch, full);
+      };
+      mbar_arrive_expect_tx(kv_full, 2 * Cfg::kTileBytes);
+      load(k_map, base + Cfg::kOffK, kv_full, seq.k0 + j0, kv_head);
+      load(v_map, base + Cfg::kOffV, kv_full, seq.k0 + j0, kv_head);
+      for (; i < n; ++i) {
+        const int qs = i % Cfg::kQStages, ds = i % Cfg::kDoStages;
+        const int head = kv_head * group + (begin + i) / q_tiles;
+        const int row = seq.q0 + (q_tile0 + (begin + i) % q_tiles) * kTileRows;
+        if (i >= Cfg::kQStages && !ctl.wait(q_empty(qs), (i / Cfg::kQStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(q_full(qs), Cfg::kTileBytes);
+        load(q_map, base + Cfg::kOffQ + qs * Cfg::kTileBytes, q_full(qs), row, head);
+        if (i >= Cfg::kDoStages && !ctl.wait(do_empty(ds), (i / Cfg::kDoStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
+          drain_barrier(q_full(qs), (i / Cfg::kQStages) & 1);
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(do_full(ds), Cfg::kTileBytes);
+        load(do_map, base + Cfg::kOffDo + ds * Cfg::kTileBytes, do_full(ds), row, head);
+      }
+      if (!ok) {
+        drain_barrier(kv_full, 0);
+        for (int m = max(0, i - Cfg::kQStages); m < i; ++m)
+          drain_barrier(q_full(m % Cfg::kQStages), (m / Cfg::kQStages) & 1);
+        for (int m = max(0, i - Cfg::kDoStages); m < i; ++m)
+          drain_barrier(do_full(m % Cfg::kDoStages), (m / Cfg::kDoStages) & 1);
+      }
+    } else if (warp == 10) {
+      // ------------------------------------------- lse and delta of the query rows
+      for (int i = 0; i < n; ++i) {
+        const int st = i % Cfg::kStatStages;
+        const int head = kv_head * group + (begin + i) / q_tiles;
+        const int row0 = (q_tile0 + (begin + i) % q_tiles) * kTileRows;
+        const int64_t index = (static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + seq.q0 + row0;
+        float lse2[4], delta[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // rows behind the sequence's end weigh nothing
+          const bool valid = row0 + x * 32 + lane < seq.nq;
+          lse2[x] = valid ? p.lse2[index + x * 32 + lane] : INFINITY;
+          delta[x] = valid ? p.delta[index + x * 32 + lane] : 0.0f;
+        }
+        if (i >= Cfg::kStatStages && !ctl.wait(stat_empty(st), (i / Cfg::kStatStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT))
+          break;
+        float* dst = reinterpret_cast<float*>(smem + Cfg::kOffStats + st * 1024);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          dst[x * 32 + lane] = -lse2[x];
+          dst[128 + x * 32 + lane] = -delta[x];
+        }
+        mbar_arrive(stat_full(st));
+      }
+    } else if (warp == 9 && n > 0) {
+      const bool leader = elect_one_sync();
+      // the rows of a query tile behind the sequence's end (packed: the next sequence's) become 0
+      auto clean = [&](int i, uint8_t* where) {
+        const int row0 = (q_tile0 + (begin + i) % q_tiles) * kTileRows;
+        if (p.shape.sequences == nullptr || row0 + kTileRows <= seq.nq) return;
+        zero_tile_rows<DP>(where, seq.nq - row0, kTileRows, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      auto score = [&](int i) {
+        const int qs = i % Cfg::kQStages;
+        if (!ctl.wait(q_full(qs), (i / Cfg::kQStages) & 1, MUP_ST_MMA_FULL_TIMEOUT)) return false;
+        clean(i, smem + Cfg::kOffQ + qs * Cfg::kTileBytes);
+        tc_fence_after_sync();
+        if (leader) {
+          umma_rows_by_rows<DP>(tmem, base + Cfg::kOffK, base + Cfg::kOffQ + qs * Cfg::kTileBytes);
+          umma_commit_1(s_full);
+        }
+        return true;
+      };
+      auto score_gradient = [&](int i) {
+        const int ds = i % Cfg::kDoStages;
+        if (!ctl.wait(do_full(ds), (i / Cfg::kDoStages) & 1, MUP_ST_MMA_FULL_TIMEOUT)) return false;
+        clean(i, smem + Cfg::kOffDo + ds * Cfg::kTileBytes);
+        tc_fence_after_sync();
+        if (leader) {
+          umma_rows_by_rows<DP>(tmem + Cfg::kTmemDp, base + Cfg::kOffV, base + Cfg::kOffDo + ds * Cfg::kTileBytes);
+          umma_commit_1(dp_full);
+        }
+        return true;
+      };
+      bool ok = ctl.wait(kv_full, 0, MUP_ST_MMA_FULL_TIMEOUT);
+      ok = ok && score(0) && score_gradient(0);
+      for (int i = 0; ok && i < n; ++i) {
+        const int qs = i % Cfg::kQStages, ds = i % Cfg::kDoStages;
+        // P(i) -> dV and S(i + 1) while dS(i) is computed, dS(i) -> dK and dP(i + 1) while P(i + 1) is
+        ok = ctl.wait(p_full, i & 1, MUP_ST_MMA_ACC_TIMEOUT);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          umma_tmem_by_cols<DP>(tmem + Cfg::kTmemDv, tmem, 64, base + Cfg::kOffDo + ds * Cfg::kTileBytes, i > 0);
+          umma_commit_1(do_empty(ds));
+        }
+        if (i + 1 < n) ok = score(i + 1);
+        ok = ok && ctl.wait(ds_full, i & 1, MUP_ST_MMA_ACC_TIMEOUT);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (leader) {
+          umma_tmem_by_cols<DP>(tmem + Cfg::kTmemDk, tmem + Cfg::kTmemDp, 64, base + Cfg::kOffQ + qs * Cfg::kTileBytes, i > 0);
+          umma_commit_1(q_empty(qs));
+          if (i + 1 == n) umma_commit_1(done);
+        }
+        if (i + 1 < n) ok = score_gradient(i + 1);
+      }
+      if (!ok) {
+        if (leader) umma_commit_1(drain);
+        __syncwarp();
+        drain_barrier(drain, 0);
+      }
+    }
+  } else {
+    more_registers<216>();
+    // Two warpgroups share a tile's columns: thread = key row, 64 queries each.
+    const int half = warp / 4, quarter = warp % 4;
+    const int j = j0 + quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const float2 c2 = make_float2(p.shape.scale_log2, p.shape.scale_log2);
+    // the query rows that see key j: [see_low, see_high]
+    const bool is_sink = j < p.shape.sinks;
+    int see_low = (is_sink && !p.shape.causal ? -kNoLimit : j - (is_sink ? 0 : p.shape.right)) - seq.off;
+    int see_high = is_sink ? kNoLimit : j - seq.off + p.shape.left;
+    if (j >= seq.nk) see_low = kNoLimit, see_high = -1;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int row0 = (q_tile0 + (begin + i) % q_tiles) * kTileRows;
+      // every row of the query tile sees every key of the tile
+      const int at_first = row0 + seq.off, at_last = min(row0 + kTileRows, seq.nq) - 1 + seq.off;
+      bool full = j0 + kTileRows <= seq.nk;
+      if (j0 + kTileRows <= p.shape.sinks)
+        full = full && (!p.shape.causal || at_first >= j0 + kTileRows - 1);
+      else
+        full = full && !has_sinks && at_first + p.shape.right >= j0 + kTileRows - 1 && at_last - p.shape.left <= j0;
+      const int st = i % Cfg::kStatStages;
+      const float4* stats = reinterpret_cast<const float4*>(smem + Cfg::kOffStats + st * 1024) + half * 16;
+      if (!ctl.wait(stat_full(st), (i / Cfg::kStatStages) & 1, MUP_ST_EPILOGUE_TIMEOUT) ||
+          !ctl.wait(s_full, i & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      uint32_t s[2][32];
+      tmem_ld_32x32(tmem + half * 64 + lane_base, s[0]);
+      tmem_ld_32x32(tmem + half * 64 + 32 + lane_base, s[1]);
+      tmem_ld_wait();
+      if (!full) {
+        const int low = see_low - row0 - half * 64, high = see_high - row0 - half * 64;
+#pragma unroll
+        for (int x = 0; x < 64; ++x) {
+          const bool seen = x >= low && x <= high;
+          s[x / 32][x % 32] = seen ? s[x / 32][x % 32] : 0xff800000u;
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          const float4 shift = stats[b * 8 + x / 4];
+          const float2 e0 = fma2(make_float2(__uint_as_float(s[b][x]), __uint_as_float(s[b][x + 1])), c2, make_float2(shift.x, shift.y));
+          const float2 e1 = fma2(make_float2(__uint_as_float(s[b][x + 2]), __uint_as_float(s[b][x + 3])), c2, make_float2(shift.z, shift.w));
+          const float p0 = exp2_sfu(e0.x), p1 = exp2_sfu(e0.y), p2 = exp2_sfu(e1.x), p3 = exp2_sfu(e1.y);
+          s[b][x] = __float_as_uint(p0), s[b][x + 1] = __float_as_uint(p1);
+          s[b][x + 2] = __float_as_uint(p2), s[b][x + 3] = __float_as_uint(p3);
+          packed[x / 2] = pack_bf16(p0, p1);
+          packed[x / 2 + 1] = pack_bf16(p2, p3);
+        }
+        tmem_st_32x16(tmem + half * 64 + b * 16 + lane_base, packed);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(p_full);
+      if (!ctl.wait(dp_full, i & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t g[32];
+        tmem_ld_32x32(tmem + Cfg::kTmemDp + half * 64 + b * 32 + lane_base, g);
+        tmem_ld_wait();
+        uint32_t packed[16];
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          const float4 delta = stats[32 + b * 8 + x / 4];
+          const float2 d0 = mul2(make_float2(__uint_as_float(s[b][x]), __uint_as_float(s[b][x + 1])),
+                                 add2(make_float2(__uint_as_float(g[x]), __uint_as_float(g[x + 1])), make_float2(delta.x, delta.y)));
+          const float2 d1 = mul2(make_float2(__uint_as_float(s[b][x + 2]), __uint_as_float(s[b][x + 3])),
+                                 add2(make_float2(__uint_as_float(g[x + 2]), __uint_as_float(g[x + 3])), make_float2(delta.z, delta.w)));
+          packed[x / 2] = pack_bf16(d0.x, d0.y);
+          packed[x / 2 + 1] = pack_bf16(d1.x, d1.y);
+        }
+        tmem_st_32x16(tmem + Cfg::kTmemDp + half * 64 + b * 16 + lane_base, packed);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      mbar_arrive(ds_full);
+      mbar_arrive(stat_empty(st));
+    }
+    if (ok && n > 0) ok = ctl.wait(done, 0, MUP_ST_EPILOGUE_TIMEOUT);
+    if (ok) {
+      tc_fence_after_sync();
+      // one warpgroup writes dV, the other dK
+      const float scale = half == 0 ? 1.0f : p.shape.scale;
+      const uint32_t src = tmem + (half == 0 ? Cfg::kTmemDv : Cfg::kTmemDk) + lane_base;
+      __nv_bfloat16* dst = half == 0 ? p.dv + batch * p.dv_batch + (seq.k0 + j) * p.dv_seq + kv_head * p.dv_head
+                                     : p.dk + batch * p.dk_batch + (seq.k0 + j) * p.dk_seq + kv_head * p.dk_head;
+      const int64_t slot = ((static_cast<int64_t>(sequence) * heads_kv + kv_head) * p.shared_tiles + tile) * shares + share;
+      float* partial = p.partial + ((slot * 2 + half) * kTileRows + quarter * 32 + lane) * DP;
+#pragma unroll 1
+      for (int b = 0; b < DP / 32; ++b) {
+        uint32_t g[32];
+        if (n > 0) {
+          tmem_ld_32x32(src + b * 32, g);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) g[x] = 0u;
+        }
+        if (j >= seq.nk) continue;
+#pragma unroll
+        for (int x = 0; x < 32; x += 8) {
+          if (b * 32 + x >= p.shape.head_dim) break;
+          if (shares > 1) {
+            uint4* to = reinterpret_cast<uint4*>(partial + b * 32 + x);
+            to[0] = make_uint4(g[x], g[x + 1], g[x + 2], g[x + 3]);
+            to[1] = make_uint4(g[x + 4], g[x + 5], g[x + 6], g[x + 7]);
+          } else {
+            uint4 v;
+            uint32_t* words = &v.x;
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              words[y] = pack_bf16(__uint_as_float(g[x + 2 * y]) * scale, __uint_as_float(g[x + 2 * y + 1]) * scale);
+            *reinterpret_cast<uint4*>(dst + b * 32 + x) = v;
+          }
+        }
+      }
+    }
+    tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// Sums the shares of the shared key tiles, always in the same order: one thread per four columns of dV or dK.
+template <int DP>
+__global__ void __launch_bounds__(256) attention_dkv_join_kernel(const __grid_constant__ AttnBackward p) {
+  constexpr int kQuads = DP / 4;
+  int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
+  const int quad = static_cast<int>(item % kQuads);
+  item /= kQuads;
+  const int r = static_cast<int>(item % kTileRows);
+  item /= kTileRows;
+  const int which = static_cast<int>(item % 2);
+  item /= 2;
+  const int tile = static_cast<int>(item % p.shared_tiles);
+  item /= p.shared_tiles;
+  const int kv_head = static_cast<int>(item % p.shape.heads_kv);
+  const int sequence = static_cast<int>(item / p.shape.heads_kv);
+  if (sequence >= p.n_sequences || quad * 4 >= p.shape.head_dim) return;
+  const AttnSeq seq = load_sequence(p.shape, sequence);
+  const int j = tile * kTileRows + r;
+  if (j >= seq.nk) return;
+  const int64_t slot = ((static_cast<int64_t>(sequence) * p.shape.heads_kv + kv_head) * p.shared_tiles + tile) * p.shares;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < p.shares; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(p.partial + (((slot + s) * 2 + which) * kTileRows + r) * DP + quad * 4);
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  const float scale = which == 0 ? 1.0f : p.shape.scale;
+  const int batch = p.shape.sequences != nullptr ? 0 : sequence;
+  __nv_bfloat16* dst = which == 0 ? p.dv + batch * p.dv_batch + (seq.k0 + j) * p.dv_seq + kv_head * p.dv_head
+                                  : p.dk + batch * p.dk_batch + (seq.k0 + j) * p.dk_seq + kv_head * p.dk_head;
+  *reinterpret_cast<uint2*>(dst + quad * 4) =
+      make_uint2(pack_bf16(sum.x * scale, sum.y * scale), pack_bf16(sum.z * scale, sum.w * scale));
+}
+
+}  // namespace mup

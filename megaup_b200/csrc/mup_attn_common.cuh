@@ -288,4 +288,20 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, 
   }
 }
 
+// A row of a key or value tile that none of the block's rows sees (another sequence's, one behind the filled part of a
+// cache, one between the sinks and the window) has to be finite where its weight is 0: it becomes 0. The whole warp
+// calls this between the tile's arrival and its first product.
+template <int DP>
+__device__ __forceinline__ void zero_unseen_rows(uint8_t* tile, const TileList& seen, int j0, int lane) {
+  if ((j0 >= seen.low && j0 + kTileRows - 1 <= seen.high) || j0 + kTileRows <= seen.sink_end) return;
+  const bool window = seen.high >= seen.low;
+  const int sinks = min(max(seen.sink_end - j0, 0), kTileRows);
+  const int from = window ? min(max(seen.low - j0, 0), kTileRows) : kTileRows;
+  const int to = window ? min(max(seen.high + 1 - j0, 0), kTileRows) : kTileRows;
+  zero_tile_rows<DP>(tile, sinks, max(sinks, from), lane);
+  zero_tile_rows<DP>(tile, max(sinks, to), kTileRows, lane);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 }  // namespace mup

@@ -194,21 +194,9 @@ __global__ void __launch_bounds__(384, 1)
             if (ok && !v_there) {
               ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
               v_there = true;
-              // A value row that none of the block's rows sees (another sequence's, one behind the cache's filled
-              // part) has to be finite where P is 0: it becomes 0.
-              const int j0 = all.tile(i - 1) * kTileRows;
-              const bool inside = j0 >= all.low && j0 + kTileRows - 1 <= all.high;
-              if (ok && !inside && j0 + kTileRows > all.sink_end) {
-                const bool window = all.high >= all.low;
-                const int sinks = min(max(all.sink_end - j0, 0), kTileRows);
-                const int from = window ? min(max(all.low - j0, 0), kTileRows) : kTileRows;
-                const int to = window ? min(max(all.high + 1 - j0, 0), kTileRows) : kTileRows;
-                uint8_t* tile = smem + Cfg::kOffStages + vs * Cfg::kTileBytes;
-                zero_tile_rows<DP>(tile, sinks, max(sinks, from), lane);
-                zero_tile_rows<DP>(tile, max(sinks, to), kTileRows, lane);
-                fence_proxy_async_smem();
-                __syncwarp();
-              }
+              if (ok)
+                zero_unseen_rows<DP>(smem + Cfg::kOffStages + vs * Cfg::kTileBytes, all, all.tile(i - 1) * kTileRows,
+                                     lane);
             }
             if (!ok) break;
             tc_fence_after_sync();
