@@ -374,6 +374,44 @@ int mup_window_attention_forward(const mup_window_attention *args, void *stream)
  * no part become 0). Deterministic. kv_lengths must be NULL. */
 int mup_window_attention_backward(const mup_window_attention *args, void *stream);
 
+/* ---- rotary positions with several axes ------------------------------------------ */
+
+#define MUP_ROTARY_INT32 0
+#define MUP_ROTARY_INT64 1
+#define MUP_ROTARY_FLOAT32 2
+
+/* Rotates pairs of head elements by position-dependent angles, for one or two
+ * tensors of the same rows (q and k) in one launch; stands between a peer-write
+ * projection and the attention (the reference leaves it to the caller). Pair p of
+ * a head turns by positions[axis of p] * frequencies[p] radians:
+ *     (x, y) -> (x cos - y sin, x sin + y cos), `inverse`: by minus the angle.
+ * Pairs are neighbours (2p, 2p + 1) when interleaved, else (p, p + pairs). Elements
+ * from 2 * pairs on are copied. Angles are reduced in 64 bits, sine and cosine in
+ * 32; each element is rounded once. Strides in elements for {sequence of the batch,
+ * row, head}, multiples of 8 like the addresses; an output may be its own input. */
+typedef struct mup_axial_rotary {
+  int32_t device;
+  int32_t batch;
+  int32_t rows; /* per sequence of the batch */
+  int32_t head_dim; /* a multiple of 8, at most 512 */
+  int32_t pairs; /* 2 * pairs <= head_dim; a multiple of 8 unless interleaved */
+  int32_t axes;
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t heads[2]; /* heads[1] == 0: one tensor */
+  const void *x[2];
+  void *y[2];
+  int64_t x_strides[2][3];
+  int64_t y_strides[2][3];
+  const void *positions; /* element of axis a, sequence b, row r at a * pos_strides[0] + b * [1] + r * [2] */
+  int64_t pos_strides[3];
+  int32_t position_type; /* MUP_ROTARY_* */
+  const double *turns; /* device [pairs]: frequency / (2 pi), turns per unit of position */
+  const int32_t *pair_axis; /* device [pairs] */
+} mup_axial_rotary;
+
+int mup_axial_rotary_launch(const mup_axial_rotary *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

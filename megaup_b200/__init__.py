@@ -45,6 +45,13 @@ from .ops import (
     prepare_peer_write_gemm_thd,
     prepare_thd_layout,
 )
+from .rotary import (
+    AxialRotary,
+    axial_rotary_bshd,
+    axial_rotary_sbhd,
+    axial_rotary_thd,
+    prepare_axial_rotary,
+)
 from .runtime import (
     DEFAULT_MAX_ROWS,
     SUPPORTED_UP_DEGREES,
@@ -58,6 +65,7 @@ from .runtime import (
 __version__ = "0.1.0"
 
 __all__ = [
+    "AxialRotary",
     "DEFAULT_MAX_ROWS",
     "SUPPORTED_UP_DEGREES",
     "MegaUPRuntime",
@@ -69,6 +77,9 @@ __all__ = [
     "PreparedPeerWriteGemmSBHD",
     "PreparedPeerWriteGemmTHD",
     "THDLayout",
+    "axial_rotary_bshd",
+    "axial_rotary_sbhd",
+    "axial_rotary_thd",
     "emulated_peer_write",
     "emulated_pull",
     "headshard_pull_gemm_bshd",
@@ -79,6 +90,7 @@ __all__ = [
     "peer_write_gemm_bshd",
     "peer_write_gemm_sbhd",
     "peer_write_gemm_thd",
+    "prepare_axial_rotary",
     "prepare_headshard_pull_gemm_bshd",
     "prepare_headshard_pull_gemm_sbhd",
     "prepare_headshard_pull_gemm_thd",

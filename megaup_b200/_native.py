@@ -73,6 +73,26 @@ class MupWindowAttention(ctypes.Structure):
     ]
 
 
+class MupAxialRotary(ctypes.Structure):
+    """``mup_axial_rotary`` of include/megaup.h."""
+
+    _fields_ = [
+        *((name, c_int32) for name in (
+            "device", "batch", "rows", "head_dim", "pairs", "axes", "interleaved", "inverse",
+        )),
+        ("heads", c_int32 * 2),
+        ("x", c_void_p * 2),
+        ("y", c_void_p * 2),
+        ("x_strides", c_int64 * 6),
+        ("y_strides", c_int64 * 6),
+        ("positions", c_void_p),
+        ("pos_strides", c_int64 * 3),
+        ("position_type", c_int32),
+        ("turns", c_void_p),
+        ("pair_axis", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); must list every symbol include/megaup.h declares.
 SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "mup_abi_version": (c_int, ()),
@@ -158,6 +178,7 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
         (POINTER(MupWindowAttention), POINTER(c_uint64), POINTER(c_uint64)),
     ),
     "mup_window_attention_forward": (c_int, (POINTER(MupWindowAttention), c_void_p)),
+    "mup_axial_rotary_launch": (c_int, (POINTER(MupAxialRotary), c_void_p)),
     "mup_window_attention_backward": (c_int, (POINTER(MupWindowAttention), c_void_p)),
 }
 

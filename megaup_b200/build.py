@@ -18,7 +18,7 @@ INCLUDE = PACKAGE_DIR.parent / "include"
 LIB_DIR = PACKAGE_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmegaup.so"
 
-SOURCES = (CSRC / "mup_api.cu", CSRC / "mup_attention.cu")
+SOURCES = (CSRC / "mup_api.cu", CSRC / "mup_attention.cu", CSRC / "mup_rotary.cu")
 HEADERS = (*sorted(CSRC.glob("*.cuh")), INCLUDE / "megaup.h")
 
 NVCC_FLAGS = (

@@ -1,0 +1,259 @@
+"""Rotary positions with several axes on head-parallel BSHD, SBHD and packed THD tensors.
+
+This is the step between a peer-write projection, which delivers ``q`` and ``k``
+with the whole sequence and a rank's share of the heads, and the attention
+(``window_attention_*``). One launch turns both tensors; slices of a fused
+projection may be passed as they are.
+
+Pair ``p`` of a head belongs to one axis (time, height, width, ...) and turns by
+``positions[axis, row] * frequency[p]`` radians: ``(x, y) -> (x cos - y sin,
+x sin + y cos)``. BF16 in and out; the angle is reduced in 64 bits (positions of
+millions keep their fraction of a turn), sine, cosine and the products are FP32,
+each element is rounded once. The gradient is the rotation by minus the angle.
+Kernel: ``csrc/mup_rotary.cu``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from collections.abc import Sequence
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from . import _native
+from .attention import _AXES, _check_heads_tensor, _rows_are_loadable, _strides
+from .ops import _tensor_signature
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_POSITIONS_LABEL = {"bshd": "[axes,S] or [axes,B,S]", "sbhd": "[axes,S] or [axes,S,B]", "thd": "[axes,T]"}
+
+
+@dataclass(frozen=True)
+class AxialRotary:
+    """Frequencies of every pair, on the device; see ``prepare_axial_rotary``."""
+
+    axis_dims: tuple[int, ...]
+    theta: float
+    interleaved: bool
+    shared_frequencies: bool
+    turns: Tensor
+    pair_axis: Tensor
+
+    @property
+    def pairs(self) -> int:
+        return sum(self.axis_dims) // 2
+
+    @property
+    def device(self) -> torch.device:
+        return self.turns.device
+
+
+def prepare_axial_rotary(
+    axis_dims: Sequence[int],
+    *,
+    theta: float = 10000.0,
+    interleaved: bool = True,
+    shared_frequencies: bool = False,
+    device: torch.device | str,
+) -> AxialRotary:
+    """Frequencies for heads whose first ``sum(axis_dims)`` elements are turned, the
+    pairs of axis 0 first, ``axis_dims[a]`` (even) elements for axis ``a``; the
+    elements behind them stay as they are. Build once and use for every layer.
+
+    ``interleaved``: pairs are neighbours ``(2p, 2p + 1)``; otherwise ``(p, p +
+    sum / 2)``, and ``sum`` must be a multiple of 16. ``shared_frequencies``: pair
+    ``p`` of the head turns with ``theta ** (-2p / sum)``; otherwise every axis has
+    a row of its own, ``theta ** (-2i / axis_dims[a])`` for its pair ``i``.
+    """
+
+    dims = tuple(int(d) for d in axis_dims)
+    if not dims or min(dims) <= 0 or any(d % 2 for d in dims):
+        raise ValueError(f"axis_dims must be positive even numbers, got {tuple(axis_dims)}")
+    total = sum(dims)
+    if total > 512:
+        raise ValueError(f"at most 512 elements of a head can be turned, got {total}")
+    if not interleaved and total % 16:
+        raise ValueError(f"rotated halves need sum(axis_dims) to be a multiple of 16, got {total}")
+    theta = float(theta)
+    if not (0.0 < theta < math.inf):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    exponents = (
+        [2 * p / total for p in range(total // 2)]
+        if shared_frequencies
+        else [2 * i / d for d in dims for i in range(d // 2)]
+    )
+    turns = [theta**-e / (2.0 * math.pi) for e in exponents]
+    axis = [a for a, d in enumerate(dims) for _ in range(d // 2)]
+    return AxialRotary(
+        axis_dims=dims,
+        theta=theta,
+        interleaved=bool(interleaved),
+        shared_frequencies=bool(shared_frequencies),
+        turns=torch.tensor(turns, dtype=torch.float64).to(device),
+        pair_axis=torch.tensor(axis, dtype=torch.int32).to(device),
+    )
+
+
+def _check(kind: str, q: Tensor, k: Tensor | None, rotary: object, positions: object) -> None:
+    if not isinstance(rotary, AxialRotary):
+        raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
+    _check_heads_tensor(q, "q", kind, None)
+    batch_axis, row_axis, _ = _AXES[kind]
+    head_dim = q.shape[-1]
+    if head_dim % 8 or head_dim > 512 or 2 * rotary.pairs > head_dim:
+        raise ValueError(
+            f"head_dim must be a multiple of 8 up to 512 and hold the {2 * rotary.pairs} turned elements, got {head_dim}"
+        )
+    if k is not None:
+        _check_heads_tensor(k, "k", kind, q.device)
+        if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != head_dim:
+            raise ValueError(f"q and k must differ in their heads only, got {tuple(q.shape)} and {tuple(k.shape)}")
+    for name, tensor in (("q", q), ("k", k)):
+        if tensor is not None and not _rows_are_loadable(tensor):
+            raise ValueError(
+                f"{name} must have contiguous heads at 16-byte aligned, positive strides, got strides "
+                f"{tensor.stride()} at address {tensor.data_ptr():#x}; pass {name}.contiguous()"
+            )
+    if rotary.device != q.device:
+        raise ValueError(f"rotary lives on {rotary.device}, q on {q.device}")
+    axes, rows = len(rotary.axis_dims), int(q.shape[row_axis])
+    shapes = [(axes, rows)]
+    if batch_axis is not None:
+        shapes.append((axes, *q.shape[:2]))
+    if (
+        not isinstance(positions, Tensor)
+        or positions.dtype not in _POSITION_TYPES
+        or positions.device != q.device
+        or tuple(positions.shape) not in shapes
+    ):
+        raise ValueError(
+            f"positions must be int32, int64 or float32 {_POSITIONS_LABEL[kind]} on {q.device}, here "
+            f"{' or '.join(map(str, shapes))}, got {_tensor_signature(positions)}"
+        )
+
+
+def _check_outputs(out: object, tensors: Sequence[Tensor]) -> None:
+    if not isinstance(out, Sequence) or len(out) != len(tensors):
+        raise ValueError(f"out must hold {len(tensors)} tensors")
+    for given, x in zip(out, tensors):
+        if not isinstance(given, Tensor) or given.shape != x.shape or given.dtype != x.dtype or given.device != x.device:
+            raise ValueError(f"out must be BF16 {tuple(x.shape)} on {x.device}, got {_tensor_signature(given)}")
+        if not _rows_are_loadable(given):
+            raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {given.stride()}")
+
+
+def _turn(
+    kind: str, tensors: Sequence[Tensor], outputs: Sequence[Tensor], rotary: AxialRotary, positions: Tensor,
+    inverse: bool,
+) -> None:
+    a = _native.MupAxialRotary()
+    x = tensors[0]
+    batch_axis, row_axis, head_axis = _AXES[kind]
+    a.device = x.device.index
+    a.batch = 1 if batch_axis is None else x.shape[batch_axis]
+    a.rows, a.head_dim = x.shape[row_axis], x.shape[-1]
+    a.pairs, a.axes = rotary.pairs, len(rotary.axis_dims)
+    a.interleaved, a.inverse = rotary.interleaved, inverse
+    n = len(tensors)
+    a.heads[:n] = [t.shape[head_axis] for t in tensors]
+    a.x[:n] = [t.data_ptr() for t in tensors]
+    a.y[:n] = [t.data_ptr() for t in outputs]
+    a.x_strides[: 3 * n] = [s for t in tensors for s in _strides(t, kind)]
+    a.y_strides[: 3 * n] = [s for t in outputs for s in _strides(t, kind)]
+    a.positions, a.position_type = positions.data_ptr(), _POSITION_TYPES[positions.dtype]
+    strides = positions.stride()
+    if positions.ndim == 2:
+        a.pos_strides[:] = (strides[0], 0, strides[1])
+    else:
+        a.pos_strides[:] = (strides[0], strides[1 + batch_axis], strides[1 + row_axis])
+    a.turns, a.pair_axis = rotary.turns.data_ptr(), rotary.pair_axis.data_ptr()
+    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(x.device).cuda_stream)
+
+
+def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
+    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+
+
+class _AxialRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, kind, rotary, positions, *tensors):
+        outputs = _fresh(tensors)
+        _turn(kind, tensors, outputs, rotary, positions, False)
+        ctx.kind, ctx.rotary = kind, rotary
+        ctx.save_for_backward(positions)
+        return tuple(outputs)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        (positions,) = ctx.saved_tensors
+        # a broadcast or transposed gradient is laid out first
+        grads = [g if _rows_are_loadable(g) else g.clone(memory_format=torch.contiguous_format) for g in grads]
+        outputs = _fresh(grads)
+        _turn(ctx.kind, grads, outputs, ctx.rotary, positions, True)
+        return (None, None, None, *outputs)
+
+
+def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: Tensor, out: object):
+    _check(kind, q, k, rotary, positions)
+    tensors = (q,) if k is None else (q, k)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        if out is not None:
+            raise ValueError("out cannot be given when a gradient is wanted")
+        outputs = _AxialRotary.apply(kind, rotary, positions, *tensors)
+    else:
+        if out is None:
+            outputs = _fresh(tensors)
+        else:
+            _check_outputs(out, tensors)
+            outputs = out
+        _turn(kind, tensors, outputs, rotary, positions, False)
+    return outputs[0], outputs[1] if k is not None else None
+
+
+def axial_rotary_bshd(
+    q: Tensor,
+    k: Tensor | None,
+    rotary: AxialRotary,
+    positions: Tensor,
+    *,
+    out: tuple[Tensor, ...] | None = None,
+) -> tuple[Tensor, Tensor | None]:
+    """Turn ``q [B,S,H,D]`` and, unless ``None``, ``k [B,S,Hkv,D]`` by their positions;
+    returns both.
+
+    ``positions`` (int32, int64 or float32 on the device) are ``[axes,S]``, shared
+    by the batch, or ``[axes,B,S]``. ``out``: tensors of the same shapes to write,
+    which may be the inputs themselves. Differentiable in ``q`` and ``k``.
+    """
+
+    return _rotate("bshd", q, k, rotary, positions, out)
+
+
+def axial_rotary_sbhd(
+    q: Tensor,
+    k: Tensor | None,
+    rotary: AxialRotary,
+    positions: Tensor,
+    *,
+    out: tuple[Tensor, ...] | None = None,
+) -> tuple[Tensor, Tensor | None]:
+    """Sequence-first variant: ``q [S,B,H,D]``, ``positions [axes,S]`` or ``[axes,S,B]``."""
+
+    return _rotate("sbhd", q, k, rotary, positions, out)
+
+
+def axial_rotary_thd(
+    q: Tensor,
+    k: Tensor | None,
+    rotary: AxialRotary,
+    positions: Tensor,
+    *,
+    out: tuple[Tensor, ...] | None = None,
+) -> tuple[Tensor, Tensor | None]:
+    """Packed variant: ``q [T,H,D]``, ``positions [axes,T]``."""
+
+    return _rotate("thd", q, k, rotary, positions, out)
