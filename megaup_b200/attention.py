@@ -56,6 +56,7 @@ class PackedSequences:
     k_blocks_128: Tensor
     longest_q: int
     longest_k: int
+    plans: dict = field(default_factory=dict, init=False, repr=False, compare=False)
 
     @property
     def num_sequences(self) -> int:
@@ -124,26 +125,35 @@ def _check_heads_tensor(tensor: object, name: str, kind: str, device: torch.devi
         raise ValueError(f"all dimensions of {name} must be positive, got {tuple(tensor.shape)}")
 
 
-def _rows_are_loadable(tensor: Tensor) -> bool:
-    """Contiguous heads at 16-byte steps: what the kernels' copies need. A dimension
-    of size 1 may have any stride."""
+def _strides_are_loadable(tensor: Tensor) -> bool:
+    """Contiguous heads at steps of whole 16 bytes: what the kernels' copies need. A
+    dimension of size 1 may have any stride."""
 
     strides = tensor.stride()
-    return (
-        strides[-1] == 1
-        and tensor.data_ptr() % 16 == 0
-        and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(tensor.shape[:-1], strides[:-1]))
+    return strides[-1] == 1 and all(
+        n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(tensor.shape[:-1], strides[:-1])
     )
 
 
-def _strides(tensor: Tensor, kind: str) -> tuple[int, int, int]:
+def _rows_are_loadable(tensor: Tensor) -> bool:
+    return tensor.data_ptr() % 16 == 0 and _strides_are_loadable(tensor)
+
+
+def _dense_strides(shape: Sequence[int]) -> list[int]:
+    strides = [1]
+    for n in reversed(shape[1:]):
+        strides.insert(0, strides[0] * n)
+    return strides
+
+
+def _row_strides(shape: Sequence[int], strides: Sequence[int], kind: str) -> list[int]:
     """{sequence, row, head} strides; a harmless one where the dimension has size 1."""
 
-    shape, strides = tensor.shape, tensor.stride()
-    dim = -(-int(shape[-1]) // 8) * 8
-    return tuple(
-        dim if axis is None or shape[axis] == 1 else strides[axis] for axis in _AXES[kind]
-    )  # type: ignore[return-value]
+    return [shape[-1] if axis is None or shape[axis] == 1 else strides[axis] for axis in _AXES[kind]]
+
+
+def _stride_array(shape: Sequence[int], strides: Sequence[int], kind: str) -> ctypes.Array:
+    return (ctypes.c_int64 * 3)(*_row_strides(shape, strides, kind))
 
 
 def _window_sides(window: object, causal: bool) -> tuple[int, int]:
@@ -166,193 +176,207 @@ def _window_sides(window: object, causal: bool) -> tuple[int, int]:
     )
 
 
-@dataclass(frozen=True)
-class _Options:
-    """What a call fixes apart from its tensors."""
+class _Plan:
+    """The checks and the host arithmetic of a call, kept per set of shapes, strides
+    and settings: the argument block without addresses, and the workspace sizes."""
 
-    kind: str
-    causal: bool
-    left: int
-    right: int
-    sinks: int
-    scale: float
-    kv_lengths: Tensor | None = field(default=None, compare=False)
-    sequences: PackedSequences | None = field(default=None, compare=False)
+    __slots__ = ("kind", "block", "lse_shape", "forward_bytes", "backward_bytes", "device", "tables")
 
-
-def _options(
-    kind: str, q: Tensor, k: Tensor, v: Tensor, *, causal: bool, window: object, sinks: int, scale: float | None,
-    kv_lengths: Tensor | None, sequences: PackedSequences | None,
-) -> _Options:
-    _check_heads_tensor(q, "q", kind, None)
-    _check_heads_tensor(k, "k", kind, q.device)
-    _check_heads_tensor(v, "v", kind, q.device)
-    if k.shape != v.shape:
-        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    batch_axis, row_axis, _ = _AXES[kind]
-    head_dim = int(q.shape[-1])
-    if head_dim != k.shape[-1] or head_dim % 8 or head_dim > 128:
-        raise ValueError(
-            f"head_dim must be one multiple of 8 up to 128, got {head_dim} and {int(k.shape[-1])}"
+    def __init__(
+        self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
+        scale: float | None, sequences: PackedSequences | None,
+    ) -> None:
+        _check_heads_tensor(q, "q", kind, None)
+        _check_heads_tensor(k, "k", kind, q.device)
+        _check_heads_tensor(v, "v", kind, q.device)
+        if k.shape != v.shape:
+            raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+        batch_axis, row_axis, head_axis = _AXES[kind]
+        head_dim = int(q.shape[-1])
+        if head_dim != k.shape[-1] or head_dim % 8 or head_dim > 128:
+            raise ValueError(f"head_dim must be one multiple of 8 up to 128, got {head_dim} and {int(k.shape[-1])}")
+        heads, heads_kv = int(q.shape[head_axis]), int(k.shape[head_axis])
+        if heads % heads_kv:
+            raise ValueError(f"heads of q ({heads}) must be a multiple of those of k and v ({heads_kv})")
+        batch = 1 if batch_axis is None else int(q.shape[batch_axis])
+        if batch_axis is not None and batch != k.shape[batch_axis]:
+            raise ValueError(f"q holds {batch} sequences, k and v {k.shape[batch_axis]}")
+        rows, keys = int(q.shape[row_axis]), int(k.shape[row_axis])
+        if max(rows, keys) > _MAX_LENGTH:
+            raise ValueError(f"at most {_MAX_LENGTH} rows, got {rows} and {keys}")
+        for name, tensor in (("q", q), ("k", k), ("v", v)):
+            if not _strides_are_loadable(tensor):
+                raise ValueError(
+                    f"{name} must have contiguous heads at positive strides of whole 16 bytes, got strides "
+                    f"{tensor.stride()}; pass {name}.contiguous()"
+                )
+        if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
+            raise ValueError(f"sinks must be a non-negative int, got {sinks!r}")
+        scale = head_dim**-0.5 if scale is None else float(scale)
+        if not 0.0 < scale <= 1e30:
+            raise ValueError(f"scale must be positive and finite, got {scale}")
+        left, right = _window_sides(window, bool(causal))
+        if sequences is not None:
+            if sequences.device != q.device:
+                raise ValueError(f"sequences live on {sequences.device}, q on {q.device}")
+            if sequences.cu_seqlens_q[-1] != rows or sequences.cu_seqlens_k[-1] != keys:
+                raise ValueError(
+                    f"sequences describe {sequences.cu_seqlens_q[-1]} query and {sequences.cu_seqlens_k[-1]} key "
+                    f"rows, got {rows} and {keys}"
+                )
+        a = _native.MupWindowAttention()
+        a.device = q.device.index
+        a.batch, a.heads_q, a.heads_kv, a.head_dim, a.seq_q, a.seq_k = batch, heads, heads_kv, head_dim, rows, keys
+        a.causal, a.left, a.right, a.sinks, a.scale = causal, left, right, min(sinks, _MAX_LENGTH), scale
+        for name, tensor in (("q", q), ("k", k), ("v", v)):
+            setattr(a, name + "_strides", _stride_array(tensor.shape, tensor.stride(), kind))
+        # results and gradients are dense
+        for name, shape in (("out", q.shape), ("dout", q.shape), ("dq", q.shape), ("dk", k.shape), ("dv", k.shape)):
+            setattr(a, name + "_strides", _stride_array(shape, _dense_strides(shape), kind))
+        if sequences is not None:
+            a.sequences, a.n_sequences = sequences.sequences.data_ptr(), sequences.num_sequences
+            for name in ("q_blocks_256", "q_blocks_128", "k_blocks_128"):
+                blocks = getattr(sequences, name)
+                setattr(a, name, blocks.data_ptr())
+                setattr(a, "n_" + name, len(blocks))
+            a.longest_q, a.longest_k = sequences.longest_q, sequences.longest_k
+        a.timeout_ns = _KERNEL_TIMEOUT_NS
+        forward, backward = ctypes.c_uint64(), ctypes.c_uint64()
+        _native.call(
+            "mup_window_attention_workspace", ctypes.byref(a), ctypes.byref(forward), ctypes.byref(backward)
         )
-    if q.shape[-2] % k.shape[-2]:
-        raise ValueError(f"heads of q ({q.shape[-2]}) must be a multiple of those of k and v ({k.shape[-2]})")
-    if batch_axis is not None and q.shape[batch_axis] != k.shape[batch_axis]:
-        raise ValueError(f"q holds {q.shape[batch_axis]} sequences, k and v {k.shape[batch_axis]}")
-    if max(q.shape[row_axis], k.shape[row_axis]) > _MAX_LENGTH:
-        raise ValueError(f"at most {_MAX_LENGTH} rows, got {q.shape[row_axis]} and {k.shape[row_axis]}")
-    for name, tensor in (("q", q), ("k", k), ("v", v)):
-        if not _rows_are_loadable(tensor):
-            raise ValueError(
-                f"{name} must have contiguous heads at 16-byte aligned, positive strides, got strides "
-                f"{tensor.stride()} at address {tensor.data_ptr():#x}; pass {name}.contiguous()"
-            )
-    if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
-        raise ValueError(f"sinks must be a non-negative int, got {sinks!r}")
-    scale = head_dim**-0.5 if scale is None else float(scale)
-    if not (0.0 < scale <= 1e30):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    left, right = _window_sides(window, bool(causal))
-    if kv_lengths is not None:
-        if (
-            not isinstance(kv_lengths, Tensor)
-            or kv_lengths.dtype != torch.int32
-            or kv_lengths.device != q.device
-            or tuple(kv_lengths.shape) != (q.shape[batch_axis],)
-            or not kv_lengths.is_contiguous()
-        ):
-            raise ValueError(
-                f"kv_lengths must be contiguous int32 [{q.shape[batch_axis]}] on {q.device}, "
-                f"got {_tensor_signature(kv_lengths)}"
-            )
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            raise ValueError("kv_lengths is for tokens over a cache: there is no gradient through it")
-    if kind == "thd":
-        if not isinstance(sequences, PackedSequences):
-            raise TypeError("sequences must be PackedSequences from prepare_packed_sequences")
-        if sequences.device != q.device:
-            raise ValueError(f"sequences live on {sequences.device}, q on {q.device}")
-        if sequences.cu_seqlens_q[-1] != q.shape[0] or sequences.cu_seqlens_k[-1] != k.shape[0]:
-            raise ValueError(
-                f"sequences describe {sequences.cu_seqlens_q[-1]} query and {sequences.cu_seqlens_k[-1]} key rows, "
-                f"got {q.shape[0]} and {k.shape[0]}"
-            )
-    return _Options(kind, bool(causal), left, right, min(sinks, _MAX_LENGTH), scale, kv_lengths, sequences)
+        self.kind, self.block, self.device = kind, bytes(a), q.device
+        # a plan that a backward pass still holds keeps the tables whose addresses it knows
+        self.tables = None if sequences is None else (
+            sequences.sequences, sequences.q_blocks_256, sequences.q_blocks_128, sequences.k_blocks_128,
+        )
+        self.lse_shape = (heads, rows) if batch_axis is None else (batch, heads, rows)
+        self.forward_bytes, self.backward_bytes = forward.value, backward.value
+
+    def arguments(self, q: Tensor, k: Tensor, v: Tensor) -> _native.MupWindowAttention:
+        a = _native.MupWindowAttention.from_buffer_copy(self.block)
+        a.q, a.k, a.v = addresses = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        if (addresses[0] | addresses[1] | addresses[2]) % 16:
+            raise ValueError(f"q, k and v must be 16-byte aligned, got addresses {[hex(x) for x in addresses]}")
+        return a
+
+    def launch(self, function: str, a: _native.MupWindowAttention, workspace_bytes: int) -> None:
+        """On the current stream of the tensors' device."""
+
+        if workspace_bytes:
+            # freed with this frame: the allocator hands it out again in stream order
+            workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace_bytes
+        _native.call(function, ctypes.byref(a), torch.cuda.current_stream(self.device).cuda_stream)
 
 
-def _check_out(out: object, q: Tensor, *inputs: Tensor) -> None:
-    if out is None:
-        return
+_PLANS: dict[object, _Plan] = {}
+_MAX_PLANS = 512
+
+
+def _plan(
+    kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
+    sequences: PackedSequences | None,
+) -> _Plan:
+    plans = _PLANS if sequences is None else sequences.plans
+    try:
+        key = (
+            kind, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
+            q.device, k.device, v.device, causal, window, sinks, type(sinks), scale,
+        )
+        return plans[key]
+    except (KeyError, TypeError, AttributeError):  # new, a list as the window, not a tensor
+        plan = _Plan(kind, q, k, v, causal, window, sinks, scale, sequences)
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[(*key[:14], tuple(window), *key[15:]) if isinstance(window, list) else key] = plan
+    return plan
+
+
+def _check_kv_lengths(kv_lengths: object, q: Tensor, kind: str) -> None:
+    batch = q.shape[_AXES[kind][0]]
+    if (
+        not isinstance(kv_lengths, Tensor)
+        or kv_lengths.dtype != torch.int32
+        or kv_lengths.device != q.device
+        or kv_lengths.shape != (batch,)
+        or not kv_lengths.is_contiguous()
+    ):
+        raise ValueError(f"kv_lengths must be contiguous int32 [{batch}] on {q.device}, got {_tensor_signature(kv_lengths)}")
+
+
+def _check_out(out: object, q: Tensor) -> None:
     if not isinstance(out, Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be BF16 {tuple(q.shape)} on {q.device}, got {_tensor_signature(out)}")
     if not _rows_are_loadable(out):
         raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {out.stride()}")
 
 
-# --------------------------------------------------------------------------- calls of the library
-
-
-def _arguments(o: _Options, q: Tensor, k: Tensor, v: Tensor) -> _native.MupWindowAttention:
-    a = _native.MupWindowAttention()
-    batch_axis, row_axis, head_axis = _AXES[o.kind]
-    a.device = q.device.index
-    a.batch = 1 if batch_axis is None else q.shape[batch_axis]
-    a.heads_q, a.heads_kv, a.head_dim = q.shape[head_axis], k.shape[head_axis], q.shape[-1]
-    a.seq_q, a.seq_k = q.shape[row_axis], k.shape[row_axis]
-    a.causal, a.left, a.right, a.sinks, a.scale = o.causal, o.left, o.right, o.sinks, o.scale
-    for name, tensor in (("q", q), ("k", k), ("v", v)):
-        _bind(a, name, tensor, o.kind)
-    if o.kv_lengths is not None:
-        a.kv_lengths = o.kv_lengths.data_ptr()
-    if o.sequences is not None:
-        s = o.sequences
-        a.sequences, a.n_sequences = s.sequences.data_ptr(), s.num_sequences
-        for name in ("q_blocks_256", "q_blocks_128", "k_blocks_128"):
-            blocks = getattr(s, name)
-            setattr(a, name, blocks.data_ptr())
-            setattr(a, "n_" + name, len(blocks))
-        a.longest_q, a.longest_k = s.longest_q, s.longest_k
-    a.timeout_ns = _KERNEL_TIMEOUT_NS
-    return a
-
-
-def _bind(a: _native.MupWindowAttention, name: str, tensor: Tensor, kind: str) -> None:
-    setattr(a, name, tensor.data_ptr())
-    setattr(a, name + "_strides", (ctypes.c_int64 * 3)(*_strides(tensor, kind)))
-
-
-def _launch(function: str, a: _native.MupWindowAttention, device: torch.device, which: int) -> None:
-    """Give the call its workspace and launch it on the current stream of ``device``."""
-
-    sizes = (ctypes.c_uint64 * 2)()
-    address = ctypes.addressof(sizes)
-    pointer = ctypes.POINTER(ctypes.c_uint64)
-    _native.call(
-        "mup_window_attention_workspace", ctypes.byref(a), ctypes.cast(address, pointer),
-        ctypes.cast(address + 8, pointer),
-    )
-    if sizes[which]:
-        # freed with this frame: the allocator hands it out again in stream order
-        workspace = torch.empty(sizes[which], dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), sizes[which]
-    _native.call(function, ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream)
-
-
-def _lse_shape(o: _Options, q: Tensor) -> tuple[int, ...]:
-    batch_axis, row_axis, head_axis = _AXES[o.kind]
-    tail = (int(q.shape[head_axis]), int(q.shape[row_axis]))
-    return tail if batch_axis is None else (int(q.shape[batch_axis]), *tail)
-
-
 def _forward(
-    o: _Options, q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, need_lse: bool
+    plan: _Plan, q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, need_lse: bool, kv_lengths: Tensor | None
 ) -> tuple[Tensor, Tensor | None]:
+    a = plan.arguments(q, k, v)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(_lse_shape(o, q), dtype=torch.float32, device=q.device) if need_lse else None
-    a = _arguments(o, q, k, v)
-    _bind(a, "out", out, o.kind)
-    a.lse = None if lse is None else lse.data_ptr()
-    _launch("mup_window_attention_forward", a, q.device, 0)
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=plan.device)
+    else:
+        a.out_strides = _stride_array(out.shape, out.stride(), plan.kind)
+    a.out = out.data_ptr()
+    lse = None
+    if need_lse:
+        lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=plan.device)
+        a.lse = lse.data_ptr()
+    if kv_lengths is not None:
+        a.kv_lengths = kv_lengths.data_ptr()
+    plan.launch("mup_window_attention_forward", a, plan.forward_bytes)
     return out, lse
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, options):
-        out, lse = _forward(options, q, k, v, None, True)
+    def forward(ctx, q, k, v, plan):
+        ctx.set_materialize_grads(False)
+        out, lse = _forward(plan, q, k, v, None, True, None)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.options = options
+        ctx.plan = plan
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return None, None, None, None
         q, k, v, out, lse = ctx.saved_tensors
-        o = ctx.options
-        if not _rows_are_loadable(dout):
-            dout = dout.contiguous()  # a broadcast or transposed gradient
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v)]
-        a = _arguments(o, q, k, v)
-        for name, tensor in zip(("out", "dout", "dq", "dk", "dv"), (out, dout, *grads)):
-            _bind(a, name, tensor, o.kind)
-        a.lse = lse.data_ptr()
-        _launch("mup_window_attention_backward", a, q.device, 1)
+        plan: _Plan = ctx.plan
+        a = plan.arguments(q, k, v)
+        if not _rows_are_loadable(dout):  # a broadcast or transposed gradient
+            dout = dout.clone(memory_format=torch.contiguous_format)
+        elif not dout.is_contiguous():
+            a.dout_strides = _stride_array(dout.shape, dout.stride(), plan.kind)
+        dq, dk, dv = grads = [torch.empty(x.shape, dtype=torch.bfloat16, device=plan.device) for x in (q, k, v)]
+        a.out, a.lse, a.dout = out.data_ptr(), lse.data_ptr(), dout.data_ptr()
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        plan.launch("mup_window_attention_backward", a, plan.backward_bytes)
         return (*grads, None)
 
 
-def _attend(kind, q, k, v, *, out, return_lse, **settings):
-    o = _options(kind, q, k, v, **settings)
-    _check_out(out, q)
+def _attend(
+    kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
+    kv_lengths: Tensor | None, sequences: PackedSequences | None, out: Tensor | None, return_lse: bool,
+):
+    plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences)
+    if kv_lengths is not None:
+        _check_kv_lengths(kv_lengths, q, kind)
+    if out is not None:
+        _check_out(out, q)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
-        result, lse = _WindowAttention.apply(q, k, v, o)
+        if kv_lengths is not None:
+            raise ValueError("kv_lengths is for tokens over a cache: there is no gradient through it")
+        result, lse = _WindowAttention.apply(q, k, v, plan)
     else:
-        result, lse = _forward(o, q, k, v, out, return_lse)
+        result, lse = _forward(plan, q, k, v, out, return_lse, kv_lengths)
     return (result, lse) if return_lse else result
 
 
@@ -383,10 +407,7 @@ def window_attention_bshd(
     Differentiable in ``q``, ``k`` and ``v``.
     """
 
-    return _attend(
-        "bshd", q, k, v, causal=causal, window=window, sinks=sinks, scale=scale, kv_lengths=kv_lengths,
-        sequences=None, out=out, return_lse=return_lse,
-    )
+    return _attend("bshd", q, k, v, causal, window, sinks, scale, kv_lengths, None, out, return_lse)
 
 
 def window_attention_sbhd(
@@ -405,10 +426,7 @@ def window_attention_sbhd(
     """Sequence-first variant: ``q [Sq,B,H,D]``, ``k, v [Sk,B,Hkv,D]`` -> ``[Sq,B,H,D]``
     (log-sum-exp ``[B,H,Sq]``)."""
 
-    return _attend(
-        "sbhd", q, k, v, causal=causal, window=window, sinks=sinks, scale=scale, kv_lengths=kv_lengths,
-        sequences=None, out=out, return_lse=return_lse,
-    )
+    return _attend("sbhd", q, k, v, causal, window, sinks, scale, kv_lengths, None, out, return_lse)
 
 
 def window_attention_thd(
@@ -427,7 +445,6 @@ def window_attention_thd(
     """Packed variant: ``q [Tq,H,D]``, ``k, v [Tk,Hkv,D]`` -> ``[Tq,H,D]`` (log-sum-exp
     ``[H,Tq]``), every sequence of ``sequences`` (``prepare_packed_sequences``) by itself."""
 
-    return _attend(
-        "thd", q, k, v, causal=causal, window=window, sinks=sinks, scale=scale, kv_lengths=None,
-        sequences=sequences, out=out, return_lse=return_lse,
-    )
+    if not isinstance(sequences, PackedSequences):
+        raise TypeError("sequences must be PackedSequences from prepare_packed_sequences")
+    return _attend("thd", q, k, v, causal, window, sinks, scale, None, sequences, out, return_lse)

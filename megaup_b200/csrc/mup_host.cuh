@@ -31,12 +31,13 @@ int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], co
 // failure that an earlier kernel of this device left there.
 int device_status_word(int device, uint32_t** device_ptr);
 
-// Makes `device` current for a scope.
+// Makes `device` current for a scope. Set even where it is current already: a thread that made no CUDA call yet (an
+// autograd thread's first one) has no context, which the driver's tensor-map encoder needs.
 class DeviceScope {
  public:
   explicit DeviceScope(int device) {
     if (cudaGetDevice(&previous_) != cudaSuccess) previous_ = -1;
-    error_ = previous_ == device ? cudaSuccess : cudaSetDevice(device);
+    error_ = cudaSetDevice(device);
     changed_ = error_ == cudaSuccess && previous_ != device && previous_ >= 0;
   }
   ~DeviceScope() {

@@ -18,13 +18,13 @@ from __future__ import annotations
 import ctypes
 import math
 from collections.abc import Sequence
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 from torch import Tensor
 
 from . import _native
-from .attention import _AXES, _check_heads_tensor, _rows_are_loadable, _strides
+from .attention import _AXES, _check_heads_tensor, _dense_strides, _row_strides, _rows_are_loadable, _strides_are_loadable
 from .ops import _tensor_signature
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -41,6 +41,7 @@ class AxialRotary:
     shared_frequencies: bool
     turns: Tensor
     pair_axis: Tensor
+    plans: dict = field(default_factory=dict, init=False, repr=False, compare=False)
 
     @property
     def pairs(self) -> int:
@@ -97,9 +98,7 @@ def prepare_axial_rotary(
     )
 
 
-def _check(kind: str, q: Tensor, k: Tensor | None, rotary: object, positions: object) -> None:
-    if not isinstance(rotary, AxialRotary):
-        raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
+def _check(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: object) -> None:
     _check_heads_tensor(q, "q", kind, None)
     batch_axis, row_axis, _ = _AXES[kind]
     head_dim = q.shape[-1]
@@ -112,10 +111,10 @@ def _check(kind: str, q: Tensor, k: Tensor | None, rotary: object, positions: ob
         if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != head_dim:
             raise ValueError(f"q and k must differ in their heads only, got {tuple(q.shape)} and {tuple(k.shape)}")
     for name, tensor in (("q", q), ("k", k)):
-        if tensor is not None and not _rows_are_loadable(tensor):
+        if tensor is not None and not _strides_are_loadable(tensor):
             raise ValueError(
-                f"{name} must have contiguous heads at 16-byte aligned, positive strides, got strides "
-                f"{tensor.stride()} at address {tensor.data_ptr():#x}; pass {name}.contiguous()"
+                f"{name} must have contiguous heads at positive strides of whole 16 bytes, got strides "
+                f"{tensor.stride()}; pass {name}.contiguous()"
             )
     if rotary.device != q.device:
         raise ValueError(f"rotary lives on {rotary.device}, q on {q.device}")
@@ -145,32 +144,43 @@ def _check_outputs(out: object, tensors: Sequence[Tensor]) -> None:
             raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {given.stride()}")
 
 
-def _turn(
-    kind: str, tensors: Sequence[Tensor], outputs: Sequence[Tensor], rotary: AxialRotary, positions: Tensor,
-    inverse: bool,
-) -> None:
+def _block(kind: str, tensors: Sequence[Tensor], rotary: AxialRotary, positions: Tensor) -> bytes:
+    """The argument block of a call without its tensors' addresses, the outputs dense."""
+
     a = _native.MupAxialRotary()
     x = tensors[0]
     batch_axis, row_axis, head_axis = _AXES[kind]
     a.device = x.device.index
     a.batch = 1 if batch_axis is None else x.shape[batch_axis]
     a.rows, a.head_dim = x.shape[row_axis], x.shape[-1]
-    a.pairs, a.axes = rotary.pairs, len(rotary.axis_dims)
-    a.interleaved, a.inverse = rotary.interleaved, inverse
+    a.pairs, a.axes, a.interleaved = rotary.pairs, len(rotary.axis_dims), rotary.interleaved
     n = len(tensors)
     a.heads[:n] = [t.shape[head_axis] for t in tensors]
-    a.x[:n] = [t.data_ptr() for t in tensors]
-    a.y[:n] = [t.data_ptr() for t in outputs]
-    a.x_strides[: 3 * n] = [s for t in tensors for s in _strides(t, kind)]
-    a.y_strides[: 3 * n] = [s for t in outputs for s in _strides(t, kind)]
-    a.positions, a.position_type = positions.data_ptr(), _POSITION_TYPES[positions.dtype]
+    a.x_strides[: 3 * n] = [s for t in tensors for s in _row_strides(t.shape, t.stride(), kind)]
+    a.y_strides[: 3 * n] = [s for t in tensors for s in _row_strides(t.shape, _dense_strides(t.shape), kind)]
     strides = positions.stride()
     if positions.ndim == 2:
         a.pos_strides[:] = (strides[0], 0, strides[1])
     else:
         a.pos_strides[:] = (strides[0], strides[1 + batch_axis], strides[1 + row_axis])
+    a.position_type = _POSITION_TYPES[positions.dtype]
     a.turns, a.pair_axis = rotary.turns.data_ptr(), rotary.pair_axis.data_ptr()
-    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(x.device).cuda_stream)
+    return bytes(a)
+
+
+def _turn(
+    block: bytes, kind: str, tensors: Sequence[Tensor], outputs: Sequence[Tensor], positions: Tensor, inverse: bool,
+    *, dense: bool = True,
+) -> None:
+    a = _native.MupAxialRotary.from_buffer_copy(block)
+    for i, (x, y) in enumerate(zip(tensors, outputs)):
+        a.x[i], a.y[i] = source, _ = x.data_ptr(), y.data_ptr()
+        if source % 16:
+            raise ValueError(f"q and k must be 16-byte aligned, got address {source:#x}")
+    if not dense:
+        a.y_strides[: 3 * len(outputs)] = [s for t in outputs for s in _row_strides(t.shape, t.stride(), kind)]
+    a.positions, a.inverse = positions.data_ptr(), inverse
+    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(tensors[0].device).cuda_stream)
 
 
 def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
@@ -179,9 +189,9 @@ def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
 
 class _AxialRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, kind, rotary, positions, *tensors):
+    def forward(ctx, block, kind, rotary, positions, *tensors):
         outputs = _fresh(tensors)
-        _turn(kind, tensors, outputs, rotary, positions, False)
+        _turn(block, kind, tensors, outputs, positions, False)
         ctx.kind, ctx.rotary = kind, rotary
         ctx.save_for_backward(positions)
         return tuple(outputs)
@@ -193,24 +203,46 @@ class _AxialRotary(torch.autograd.Function):
         # a broadcast or transposed gradient is laid out first
         grads = [g if _rows_are_loadable(g) else g.clone(memory_format=torch.contiguous_format) for g in grads]
         outputs = _fresh(grads)
-        _turn(ctx.kind, grads, outputs, ctx.rotary, positions, True)
-        return (None, None, None, *outputs)
+        _turn(_plan(ctx.kind, grads, ctx.rotary, positions), ctx.kind, grads, outputs, positions, True)
+        return (None, None, None, None, *outputs)
+
+
+_MAX_PLANS = 512
+
+
+def _plan(kind: str, tensors: Sequence[Tensor | None], rotary: AxialRotary, positions: Tensor) -> bytes:
+    """The checked argument block of a call, kept per set of shapes and strides."""
+
+    try:
+        key = (
+            kind, positions.shape, positions.stride(), positions.dtype, positions.device,
+            *((t.shape, t.stride(), t.dtype, t.device) for t in tensors),
+        )
+        return rotary.plans[key]
+    except (KeyError, AttributeError):  # new, not a tensor
+        _check(kind, tensors[0], tensors[1] if len(tensors) > 1 else None, rotary, positions)
+    if len(rotary.plans) >= _MAX_PLANS:
+        rotary.plans.clear()
+    block = rotary.plans[key] = _block(kind, tensors, rotary, positions)
+    return block
 
 
 def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: Tensor, out: object):
-    _check(kind, q, k, rotary, positions)
+    if not isinstance(rotary, AxialRotary):
+        raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
     tensors = (q,) if k is None else (q, k)
+    block = _plan(kind, tensors, rotary, positions)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
-        outputs = _AxialRotary.apply(kind, rotary, positions, *tensors)
+        outputs = _AxialRotary.apply(block, kind, rotary, positions, *tensors)
     else:
         if out is None:
             outputs = _fresh(tensors)
         else:
             _check_outputs(out, tensors)
             outputs = out
-        _turn(kind, tensors, outputs, rotary, positions, False)
+        _turn(block, kind, tensors, outputs, positions, False, dense=out is None)
     return outputs[0], outputs[1] if k is not None else None
 
 
