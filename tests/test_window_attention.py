@@ -1,0 +1,465 @@
+"""Sliding-window attention with sinks: the arguments it refuses (no GPU needed) and its results against 64 bits."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import megaup_b200 as mega_up
+from _attention_reference import HALF_BF16, assert_within, attention, visible
+from megaup_b200 import _native, attention as module, build
+
+DEVICE = torch.device("cuda", 0)
+BF16 = torch.bfloat16
+
+# --------------------------------------------------------------------------- without a GPU
+
+
+@pytest.fixture(scope="module")
+def library() -> ctypes.CDLL:
+    build.ensure_built()
+    return _native.lib()
+
+
+def _block(**changes) -> _native.MupWindowAttention:
+    """A call that every check accepts; nothing behind the addresses is touched before they fail."""
+
+    a = _native.MupWindowAttention()
+    a.batch, a.heads_q, a.heads_kv, a.head_dim, a.seq_q, a.seq_k = 2, 4, 2, 64, 100, 300
+    a.causal, a.left, a.right, a.sinks, a.scale = 1, 50, 0, 4, 0.125
+    for name in ("q", "k", "v", "out", "dout", "dq", "dk", "dv"):
+        setattr(a, name, 4096)
+        setattr(a, name + "_strides", (ctypes.c_int64 * 3)(300 * 256, 256, 64))
+    a.lse = 4096
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize(
+    "changes",
+    [
+        dict(head_dim=0), dict(head_dim=12), dict(head_dim=136), dict(heads_q=3), dict(heads_kv=0), dict(batch=0),
+        dict(seq_q=0), dict(seq_k=0), dict(seq_k=(1 << 29) + 1), dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0),
+        dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(k=4104), dict(v=4098), dict(out=0),
+        dict(q_strides=(ctypes.c_int64 * 3)(0, 256, 64)), dict(k_strides=(ctypes.c_int64 * 3)(1024, 257, 64)),
+        dict(v_strides=(ctypes.c_int64 * 3)(1024, 256, -64)),
+        dict(sequences=4096), dict(sequences=4096, batch=1, n_sequences=1, longest_q=101),
+    ],
+    ids=str,
+)
+def test_the_library_refuses(library, changes) -> None:
+    for name in ("mup_window_attention_forward", "mup_window_attention_backward"):
+        assert getattr(library, name)(ctypes.byref(_block(**changes)), None) in (-1, -3), changes
+        assert b"window attention" in library.mup_last_error()
+
+
+def test_the_library_refuses_a_gradient_it_cannot_compute(library) -> None:
+    assert library.mup_window_attention_backward(ctypes.byref(_block(kv_lengths=4096)), None) == -3
+    assert library.mup_window_attention_backward(ctypes.byref(_block(lse=0)), None) == -1
+    assert library.mup_window_attention_backward(ctypes.byref(_block(dq=4097)), None) == -1
+    assert library.mup_window_attention_forward(None, None) == -1
+    assert library.mup_window_attention_workspace(None, None, None) == -1
+
+
+def test_workspace_sizes(library) -> None:
+    forward, backward = ctypes.c_uint64(), ctypes.c_uint64()
+
+    def sizes(**changes):
+        code = library.mup_window_attention_workspace(
+            ctypes.byref(_block(**changes)), ctypes.byref(forward), ctypes.byref(backward)
+        )
+        assert code == 0
+        return forward.value, backward.value
+
+    # enough row blocks for the GPU: nothing to join; the backward pass keeps two floats per row
+    assert sizes(batch=64, seq_q=4096, seq_k=4096, heads_q=4, sinks=0) == (0, 2 * 64 * 4 * 4096 * 4)
+    few, _ = sizes(batch=1, seq_q=1, seq_k=1 << 20, left=-1, sinks=0)
+    assert few > 0 and few % (4 * (64 + 1)) == 0
+
+
+def test_window_sides() -> None:
+    assert module._window_sides(None, True) == (-1, 0)
+    assert module._window_sides(None, False) == (-1, -1)
+    assert module._window_sides(7, True) == (7, 0)
+    assert module._window_sides(7, False) == (7, 7)
+    assert module._window_sides((3, None), False) == (3, -1)
+    assert module._window_sides((3, 0), True) == (3, 0)
+    assert module._window_sides([1 << 40, 2], False) == (1 << 29, 2)
+    for window, causal in ((-1, True), ((1, 2), True), ((1, 2, 3), False), ("x", False), (1.5, True), (True, False),
+                           ((None, True), False)):
+        with pytest.raises(ValueError):
+            module._window_sides(window, causal)
+
+
+def test_packed_sequences_on_the_host() -> None:
+    s = mega_up.prepare_packed_sequences([0, 300, 300, 301], [0, 0, 5, 140], device="cpu")
+    assert s.sequences.tolist() == [[0, 300, 0, 0], [300, 0, 0, 5], [300, 1, 5, 135]]
+    assert s.q_blocks_256.tolist() == [[0, 256], [0, 0], [2, 0]]
+    assert s.q_blocks_128.tolist() == [[0, 256], [0, 128], [0, 0], [2, 0]]
+    assert sorted(map(tuple, s.k_blocks_128.tolist())) == [(1, 0), (2, 0), (2, 128)]
+    assert (s.longest_q, s.longest_k, s.num_sequences) == (300, 135, 3)
+    layout = mega_up.prepare_packed_sequences(torch.tensor([0, 4], dtype=torch.int32), device="cpu")
+    assert layout.cu_seqlens_k == (0, 4)
+    for bad in (([1, 2],), ([0, 2, 1],), ([0],), ([0, 0],), ([0, 4], [0, 2, 4])):
+        with pytest.raises(ValueError):
+            mega_up.prepare_packed_sequences(*bad, device="cpu")
+
+
+def test_host_tensors_are_refused() -> None:
+    x = torch.zeros(1, 4, 2, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        mega_up.window_attention_bshd(x, x, x)
+    with pytest.raises(ValueError):
+        mega_up.window_attention_bshd(x, 3, x)
+    with pytest.raises(TypeError):
+        mega_up.window_attention_thd(x[0], x[0], x[0], [0, 4])
+
+
+# --------------------------------------------------------------------------- on the GPU
+
+
+def _normal(shape, seed, factor=1.0):
+    generator = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=generator) * factor).to(BF16).to(DEVICE)
+
+
+def _rows(x, kind, b):
+    """[rows, heads, dim] of sequence ``b``."""
+
+    return x[b] if kind == "bshd" else x[:, b]
+
+
+def _shape(kind, batch, rows, heads, dim):
+    return (batch, rows, heads, dim) if kind == "bshd" else (rows, batch, heads, dim)
+
+
+def _window(causal, left, right):
+    return left if causal else (left, right)
+
+
+CASES = [
+    # kind, batch, queries, keys, heads, kv heads, dim, causal, left, right, sinks
+    ("bshd", 1, 1, 1, 1, 1, 64, True, None, 0, 0),
+    ("bshd", 2, 1, 1, 4, 2, 128, False, 0, 0, 0),
+    ("sbhd", 2, 127, 127, 2, 2, 64, True, None, 0, 0),
+    ("bshd", 1, 128, 128, 2, 1, 128, True, 0, 0, 0),
+    ("bshd", 1, 129, 257, 3, 1, 128, True, 64, 0, 1),
+    ("sbhd", 3, 255, 255, 4, 4, 64, False, 17, 40, 0),
+    ("bshd", 1, 257, 129, 2, 2, 128, True, None, 0, 0),  # the first 128 rows see nothing
+    ("bshd", 1, 300, 40, 2, 1, 64, False, 10, 10, 0),  # rows at negative positions see nothing
+    ("bshd", 1, 300, 40, 2, 1, 64, False, 10, 10, 3),  # ... but the sinks
+    ("bshd", 1, 384, 384, 8, 1, 128, True, 100, 0, 200),  # a sink tile that is cut
+    ("bshd", 2, 200, 650, 6, 3, 96, True, 128, 0, 4),
+    ("sbhd", 1, 513, 513, 2, 2, 40, False, None, 0, 0),
+    ("bshd", 1, 513, 513, 2, 2, 8, False, 0, None, 130),
+    ("bshd", 1, 90, 1000, 5, 5, 128, False, None, None, 0),
+    ("bshd", 1, 640, 640, 2, 1, 72, True, 127, 0, 1000),  # more sinks than keys
+    ("bshd", 1, 1000, 1000, 4, 2, 128, True, 1 << 40, 0, 0),
+    ("sbhd", 2, 700, 700, 2, 1, 120, False, 130, 5, 129),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("factor", [1.0, 6.0], ids=["flat", "peaked"])
+def test_forward_and_backward(case, factor) -> None:
+    kind, batch, queries, keys, heads, kv_heads, dim, causal, left, right, sinks = case
+    q = _normal(_shape(kind, batch, queries, heads, dim), 1, factor).requires_grad_()
+    k = _normal(_shape(kind, batch, keys, kv_heads, dim), 2).requires_grad_()
+    v = _normal(_shape(kind, batch, keys, kv_heads, dim), 3).requires_grad_()
+    dout = _normal(_shape(kind, batch, queries, heads, dim), 4)
+    call = getattr(mega_up, f"window_attention_{kind}")
+    out, lse = call(q, k, v, causal=causal, window=_window(causal, left, right), sinks=sinks, return_lse=True)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    again = torch.autograd.grad(call(q, k, v, causal=causal, window=_window(causal, left, right), sinks=sinks), (q, k, v), dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again)), "two runs differ"
+    with torch.no_grad():
+        plain = call(q, k, v, causal=causal, window=_window(causal, left, right), sinks=sinks)
+    assert torch.equal(plain, out)
+    seen = visible(queries, keys, causal=causal, left=left, right=right, sinks=sinks)
+    for b in range(batch):
+        e = attention(*(_rows(x, kind, b) for x in (q, k, v)), seen, dout=_rows(dout, kind, b))
+        assert_within(_rows(out, kind, b), e.out, e.out_error, "out")
+        assert_within(lse[b], e.lse, e.lse_error, "lse")
+        for name, got, want, error in zip(("dq", "dk", "dv"), grads, (e.dq, e.dk, e.dv), (e.dq_error, e.dk_error, e.dv_error)):
+            assert_within(_rows(got, kind, b), want, error, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (5, 5, 64), (12, 4, 128), (16, 1, 80), (1, 1, 128)], ids=str)
+@pytest.mark.parametrize("queries", [1, 2, 9, 33])
+@pytest.mark.parametrize("kind", ["bshd", "sbhd"])
+def test_tokens_over_a_cache(kind, queries, heads, kv_heads, dim) -> None:
+    """Every length from nothing to the whole cache; what lies behind a length, and between the sinks and the
+    window of the whole call, is NaN."""
+
+    capacity, left, sinks = 700, 100, 5
+    lengths = [0, 1, queries, 64, 128, 129, 640, capacity, capacity + 50, -3]
+    batch = len(lengths)
+    q = _normal(_shape(kind, batch, queries, heads, dim), 1)
+    k = _normal(_shape(kind, batch, capacity, kv_heads, dim), 2)
+    v = _normal(_shape(kind, batch, capacity, kv_heads, dim), 3)
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), capacity)
+        for x in (k, v):
+            rows = _rows(x, kind, b)
+            rows[n:] = float("nan")
+            rows[sinks : max(sinks, n - queries - left)] = float("nan")
+    out = torch.full(_shape(kind, batch, queries, heads, dim), 7.0, dtype=BF16, device=DEVICE)
+    call = getattr(mega_up, f"window_attention_{kind}")
+    device_lengths = torch.tensor(lengths, dtype=torch.int32, device=DEVICE)
+    got, lse = call(q, k, v, window=left, sinks=sinks, kv_lengths=device_lengths, out=out, return_lse=True)
+    assert got.data_ptr() == out.data_ptr()
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), capacity)
+        seen = visible(queries, n, causal=True, left=left, right=0, sinks=sinks)
+        e = attention(_rows(q, kind, b), _rows(k, kind, b)[:n], _rows(v, kind, b)[:n], seen)
+        assert_within(_rows(out, kind, b), e.out, e.out_error, f"out of length {n}")
+        assert_within(lse[b], e.lse, e.lse_error, f"lse of length {n}")
+
+
+def _packed(lengths_q, lengths_k, heads, kv_heads, dim, *, seed=0, factor=1.0):
+    q = _normal((sum(lengths_q), heads, dim), seed + 1, factor)
+    k = _normal((sum(lengths_k), kv_heads, dim), seed + 2)
+    v = _normal((sum(lengths_k), kv_heads, dim), seed + 3)
+    dout = _normal((sum(lengths_q), heads, dim), seed + 4)
+    cu = lambda n: [0] + torch.tensor(n).cumsum(0).tolist()  # noqa: E731
+    return q, k, v, dout, mega_up.prepare_packed_sequences(cu(lengths_q), cu(lengths_k), device=DEVICE)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize(
+    "lengths_q,lengths_k,heads,kv_heads,dim,causal,left,right,sinks",
+    [
+        ([1, 0, 128, 129, 300, 5], [1, 7, 128, 129, 300, 5], 4, 2, 128, True, 60, 0, 3),
+        ([100, 28, 1, 500], [100, 0, 400, 130], 3, 3, 64, False, 100, 20, 140),
+        ([1, 1, 1, 1], [900, 1, 0, 257], 8, 1, 128, True, None, 0, 0),
+        ([2, 1, 3], [900, 100, 257], 10, 2, 96, True, 300, 0, 1),
+        ([640], [640], 2, 1, 64, False, None, None, 0),
+        ([31, 7], [31, 7], 8, 2, 64, True, 4, 0, 2),
+    ],
+    ids=str,
+)
+def test_packed_sequences(lengths_q, lengths_k, heads, kv_heads, dim, causal, left, right, sinks) -> None:
+    q, k, v, dout, sequences = _packed(lengths_q, lengths_k, heads, kv_heads, dim)
+    for x in (q, k, v):
+        x.requires_grad_()
+    out, lse = mega_up.window_attention_thd(
+        q, k, v, sequences, causal=causal, window=_window(causal, left, right), sinks=sinks, return_lse=True
+    )
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    a = c = 0
+    for n, m in zip(lengths_q, lengths_k):
+        qs, ks = slice(a, a + n), slice(c, c + m)
+        seen = visible(n, m, causal=causal, left=left, right=right, sinks=sinks)
+        e = attention(q[qs], k[ks], v[ks], seen, dout=dout[qs])
+        assert_within(out[qs], e.out, e.out_error, "out")
+        assert_within(lse[:, qs], e.lse, e.lse_error, "lse")
+        assert_within(grads[0][qs], e.dq, e.dq_error, "dq")
+        assert_within(grads[1][ks], e.dk, e.dk_error, "dk")
+        assert_within(grads[2][ks], e.dv, e.dv_error, "dv")
+        a, c = a + n, c + m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), torch.finfo(BF16).min])
+def test_a_sequence_keeps_to_itself(poison) -> None:
+    lengths = [130, 200, 70, 300]
+    q, k, v, dout, sequences = _packed(lengths, lengths, 4, 2, 128, seed=7)
+    settings = dict(window=50, sinks=2)
+
+    def run():
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = mega_up.window_attention_thd(*leaves, sequences, **settings)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    before = [x.detach().clone() for x in run()]
+    for x in (q, k, v, dout):
+        x[130:330] = poison
+    after = run()
+    for a, b in zip(before, after):
+        assert torch.equal(a[:130], b[:130]) and torch.equal(a[330:], b[330:])
+
+
+@pytest.mark.gpu
+def test_unseen_keys_may_hold_anything() -> None:
+    q, k, v = (_normal((1, 300, 2, 64), s) for s in (1, 2, 3))
+    k = torch.cat((_normal((1, 700, 2, 64), 5), k), 1)
+    v = torch.cat((_normal((1, 700, 2, 64), 6), v), 1)
+    want = mega_up.window_attention_bshd(q, k, v, window=90, sinks=6)
+    for x in (k, v):
+        x[:, 6:610] = float("nan")  # before the first row's window
+    assert torch.equal(mega_up.window_attention_bshd(q, k, v, window=90, sinks=6), want)
+
+
+@pytest.mark.gpu
+def test_slices_of_a_fused_projection_and_out() -> None:
+    heads, kv_heads, dim, rows = 4, 2, 64, 333
+    fused = _normal((rows, 2, heads + 2 * kv_heads, dim), 1)
+    q, k, v = fused.split((heads, kv_heads, kv_heads), dim=2)
+    want = mega_up.window_attention_sbhd(q.contiguous(), k.contiguous(), v.contiguous(), window=40)
+    assert torch.equal(mega_up.window_attention_sbhd(q, k, v, window=40), want)
+    room = torch.full((rows + 2, 2, heads + 3, dim), 5.0, dtype=BF16, device=DEVICE)
+    out = room[1:-1, :, 1 : 1 + heads]
+    assert mega_up.window_attention_sbhd(q, k, v, window=40, out=out) is out
+    assert torch.equal(out, want)
+    room[1:-1, :, 1 : 1 + heads] = 5.0
+    assert bool((room == 5.0).all()), "something outside of out was written"
+
+
+@pytest.mark.gpu
+def test_gradients_that_are_broadcast_or_transposed() -> None:
+    q, k, v = (_normal((2, 150, 2, 64), s).requires_grad_() for s in (1, 2, 3))
+    out = mega_up.window_attention_bshd(q, k, v, window=30)
+    ones = torch.autograd.grad(out, (q, k, v), torch.ones_like(out), retain_graph=True)
+    for a, b in zip(ones, torch.autograd.grad(out.float().sum(), (q, k, v), retain_graph=True)):
+        assert torch.equal(a, b)
+    for a, b in zip(ones, torch.autograd.grad(out, (q, k, v), torch.ones((), dtype=BF16, device=DEVICE).expand_as(out), retain_graph=True)):
+        assert torch.equal(a, b)
+    dout = _normal((2, 150, 2, 64), 9)
+    strided = torch.empty(2, 2, 150, 64, dtype=BF16, device=DEVICE).transpose(1, 2).copy_(dout)
+    assert not strided.is_contiguous()
+    for a, b in zip(torch.autograd.grad(out, (q, k, v), dout, retain_graph=True), torch.autograd.grad(out, (q, k, v), strided)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_the_gradient_is_the_slope() -> None:
+    """Along a direction, the central difference of the 64-bit loss against the kernel's gradient."""
+
+    queries, keys, heads, kv_heads, dim = 140, 200, 4, 2, 64
+    q, k, v = _normal((queries, heads, dim), 1), _normal((keys, kv_heads, dim), 2), _normal((keys, kv_heads, dim), 3)
+    dout = _normal((queries, heads, dim), 4)
+    seen = visible(queries, keys, causal=True, left=70, right=0, sinks=3)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = mega_up.window_attention_bshd(*(x[None] for x in leaves), window=70, sinks=3)
+    grads = torch.autograd.grad(out, leaves, dout[None])
+    e = attention(q, k, v, seen, dout=dout)
+    errors = (e.dq_error, e.dk_error, e.dv_error)
+    h = 2.0**-10
+    for i, x in enumerate((q, k, v)):
+        direction = torch.randn(x.shape, generator=torch.Generator().manual_seed(20 + i), dtype=torch.float64)
+
+        def loss(step):
+            moved = [y.double().cpu() for y in (q, k, v)]
+            moved[i] = moved[i] + step * direction
+            return float((attention(*moved, seen).out * dout.double().cpu()).sum())
+
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        curve = abs(loss(2 * h) - loss(-2 * h) - 2 * (loss(h) - loss(-h))) / (4 * h)  # the difference's own error
+        allowed = float((errors[i] * direction.abs()).sum()) + curve + 1e-9 * abs(slope)
+        got = float((grads[i].double().cpu() * direction).sum())
+        assert abs(got - slope) <= allowed, (i, got, slope, allowed)
+
+
+@pytest.mark.gpu
+def test_another_stream_and_a_captured_graph() -> None:
+    q, k, v = (_normal((1, 400, 2, 128), s).requires_grad_() for s in (1, 2, 3))
+    dout = _normal((1, 400, 2, 128), 4)
+
+    def step():
+        out = mega_up.window_attention_bshd(q, k, v, window=100, sinks=2)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), dout))
+
+    want = [x.clone() for x in step()]
+    token = _normal((1, 1, 2, 128), 5)
+    want_token = mega_up.window_attention_bshd(token, k.detach(), v.detach())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [x.clone() for x in step()]
+        got_token = mega_up.window_attention_bshd(token, k.detach(), v.detach())
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and torch.equal(want_token, got_token)
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graphs, captured = [], []
+    for _ in range(2):  # two graphs of one call: each has its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured.append((*step(), mega_up.window_attention_bshd(token, k.detach(), v.detach())))
+        graphs.append(graph)
+    for x in (q, k, v):
+        x.data.copy_(_normal(x.shape, 11))
+    want = [x.clone() for x in (*step(), mega_up.window_attention_bshd(token, k.detach(), v.detach()))]
+    for graph in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in captured:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_offsets_behind_32_bits() -> None:
+    """A cache of more than 2^31 elements: the last sequence and the last rows."""
+
+    rows, kv_heads, dim = 2100, 2, 128
+    stride = (1 << 31) // 4 + 4096
+    store = torch.empty(5 * stride, dtype=BF16, device=DEVICE)
+    k = store.as_strided((5, rows, kv_heads, dim), (stride, kv_heads * dim, dim, 1))
+    v = store.as_strided((5, rows, kv_heads, dim), (stride, kv_heads * dim, dim, 1), rows * kv_heads * dim)
+    k.copy_(_normal((1, rows, kv_heads, dim), 1).expand_as(k))
+    v.copy_(_normal((1, rows, kv_heads, dim), 2).expand_as(v))
+    q = _normal((1, 3, 8, dim), 3).expand(5, -1, -1, -1).contiguous()
+    out = mega_up.window_attention_bshd(q, k, v, window=1000, sinks=4)
+    for b in range(1, 5):
+        assert torch.equal(out[b], out[0])
+    e = attention(q[4], k[4], v[4], visible(3, rows, causal=True, left=1000, right=0, sinks=4))
+    assert_within(out[4], e.out, e.out_error, "out")
+
+
+@pytest.mark.gpu
+def test_refusals() -> None:
+    q, k = _normal((2, 40, 4, 64), 1), _normal((2, 50, 2, 64), 2)
+    call = mega_up.window_attention_bshd
+    bad = [
+        (q, k, k[:, :40]), (q, k[:1], k[:1]), (q[..., :32], k, k), (q[:, :, :3], k, k), (q.float(), k, k), (q, k.cpu(), k),
+        (q[0], k, k), (q[:, :0], k, k), (q, k[:, :0], k[:, :0]), (q.transpose(2, 3).contiguous().transpose(2, 3), k, k),
+        (q[:, :1].expand(-1, 40, -1, -1), k, k), (q[..., :60], k[..., :60], k[..., :60]),
+        (_normal((2, 40, 4, 136), 1), _normal((2, 40, 4, 136), 1), _normal((2, 40, 4, 136), 1)),
+    ]
+    for arguments in bad:
+        with pytest.raises(ValueError):
+            call(*arguments)
+    shifted = torch.empty(q.numel() + 8, dtype=BF16, device=DEVICE)[1 : 1 + q.numel()].view(q.shape)
+    with pytest.raises(ValueError, match="aligned"):
+        call(shifted, k, k)
+    for settings in (
+        dict(window=-1), dict(window=(1, 1)), dict(sinks=-1), dict(sinks=1.0), dict(sinks=True), dict(scale=0.0),
+        dict(scale=float("nan")), dict(scale=-1.0), dict(kv_lengths=torch.zeros(2, device=DEVICE)),
+        dict(kv_lengths=torch.zeros(3, dtype=torch.int32, device=DEVICE)), dict(kv_lengths=torch.zeros(2, dtype=torch.int32)),
+        dict(out=torch.empty_like(k)), dict(out=q.float()), dict(out=q.transpose(2, 3).contiguous().transpose(2, 3)),
+    ):
+        with pytest.raises(ValueError):
+            call(q, k, k, **settings)
+    call(q, k, k, sinks=1)
+    with pytest.raises(ValueError):
+        call(q, k, k, sinks=True)  # also after the same call with 1
+    leaf = q.clone().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        call(leaf, k, k, out=torch.empty_like(q))
+    with pytest.raises(ValueError, match="gradient"):
+        call(leaf, k, k, kv_lengths=torch.full((2,), 50, dtype=torch.int32, device=DEVICE))
+    out = call(leaf, k, k)
+    (gradient,) = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)
+    with pytest.raises(RuntimeError):
+        gradient.sum().backward()
+    sequences = mega_up.prepare_packed_sequences([0, 40], [0, 50], device=DEVICE)
+    mega_up.window_attention_thd(q[0], k[0], k[0], sequences)
+    with pytest.raises(ValueError):
+        mega_up.window_attention_thd(q[0], k[0, :49], k[0, :49], sequences)
+    with pytest.raises(ValueError):
+        mega_up.window_attention_thd(q[0], k[0], k[0], mega_up.prepare_packed_sequences([0, 40], [0, 50], device="cpu"))
+
+
+@pytest.mark.gpu
+def test_scale_is_used() -> None:
+    q, k, v = _normal((1, 100, 2, 64), 1), _normal((1, 100, 2, 64), 2), _normal((1, 100, 2, 64), 3)
+    out = mega_up.window_attention_bshd(q, k, v, scale=0.5)
+    e = attention(q[0], k[0], v[0], visible(100, 100, causal=True, left=None, right=0, sinks=0), scale=0.5)
+    assert_within(out[0], e.out, e.out_error, "out")
+    assert e.out_error.max() < 32 * HALF_BF16
