@@ -260,10 +260,7 @@ __global__ void __launch_bounds__(384, 1)
       if (!full) {
         const int low = span.low - j0, high = span.high - j0, sink = span.sink - j0;
 #pragma unroll
-        for (int x = 0; x < 64; ++x) {
-          const bool seen = (x >= low && x <= high) || x < sink;
-          s[x / 32][x % 32] = seen ? s[x / 32][x % 32] : 0xff800000u;
-        }
+        for (int b = 0; b < 2; ++b) hide_scores(s[b], span_bits(low - b * 32, high - b * 32, sink - b * 32));
       }
 #pragma unroll
       for (int x = 0; x < 64; x += 2) {
@@ -600,10 +597,7 @@ __global__ void __launch_bounds__(384, 1)
       if (!full) {
         const int low = see_low - row0 - half * 64, high = see_high - row0 - half * 64;
 #pragma unroll
-        for (int x = 0; x < 64; ++x) {
-          const bool seen = x >= low && x <= high;
-          s[x / 32][x % 32] = seen ? s[x / 32][x % 32] : 0xff800000u;
-        }
+        for (int b = 0; b < 2; ++b) hide_scores(s[b], span_bits(low - b * 32, high - b * 32, 0));
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {

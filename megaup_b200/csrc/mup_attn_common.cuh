@@ -98,6 +98,18 @@ __device__ __forceinline__ bool tile_is_full(const RowSpan& first, const RowSpan
   return (j0 >= last.low && j0 + kTileRows - 1 <= first.high) || j0 + kTileRows <= first.sink;
 }
 
+// Bit x of the result: x < n (n may be anything).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+// Bit x: x < sink or low <= x <= high.
+__device__ __forceinline__ uint32_t span_bits(int low, int high, int sink) {
+  return (bits_below(high + 1) & ~bits_below(low)) | bits_below(sink);
+}
+// Scores whose bit is not set become -inf.
+__device__ __forceinline__ void hide_scores(uint32_t (&score)[32], uint32_t seen) {
+#pragma unroll
+  for (int x = 0; x < 32; ++x) score[x] = (seen >> x) & 1u ? score[x] : 0xff800000u;
+}
+
 // ---------------------------------------------------------------------------
 // PTX
 // ---------------------------------------------------------------------------

@@ -44,6 +44,59 @@ struct AttnForwardConfig {
   static constexpr int kTmemO = 256;
 };
 
+// What a CTA computes: decoded by each role for itself, so that no role holds what only another needs.
+struct ForwardBlock {
+  AttnSeq seq;
+  int batch, head0, kv_head, rows, row0, row_step, head_step, split;
+
+  __device__ __forceinline__ explicit ForwardBlock(const AttnForward& p) {
+    int w = blockIdx.x;
+    split = w % p.splits;
+    w /= p.splits;
+    const int head_set = w % p.head_sets;
+    w /= p.head_sets;
+    int sequence;
+    rows = kTileRows / p.packed_heads;  // rows of a head in a sub-tile
+    row_step = p.pair_heads ? 0 : rows;
+    head_step = p.pair_heads ? p.packed_heads : 0;
+    if (p.tiles != nullptr) {
+      const int2 tile = p.tiles[w];
+      sequence = tile.x, row0 = tile.y;
+    } else {
+      // the last rows first: under a causal mask they have the most keys
+      sequence = w % p.shape.batch;
+      row0 = (p.blocks_per_sequence - 1 - w / p.shape.batch) * (p.single || p.pair_heads ? rows : 2 * rows);
+    }
+    seq = load_sequence(p.shape, sequence);
+    batch = p.shape.sequences != nullptr ? 0 : sequence;
+    head0 = head_set * p.packed_heads * (p.pair_heads ? 2 : 1);
+    kv_head = head0 / (p.shape.heads_q / p.shape.heads_kv);
+  }
+  // the second sub-tile may lie behind the sequence's end
+  __device__ __forceinline__ bool exists(const AttnForward& p, int t) const {
+    return row0 + t * row_step < seq.nq && !(t == 1 && p.single);
+  }
+  __device__ __forceinline__ RowSpan first(const AttnForward& p, int t) const {
+    return row_span(p.shape, seq, row0 + t * row_step);
+  }
+  __device__ __forceinline__ RowSpan last(const AttnForward& p, int t) const {
+    return row_span(p.shape, seq, min(row0 + t * row_step + rows, seq.nq) - 1);
+  }
+  __device__ __forceinline__ TileList tiles(const AttnForward& p, int t) const {
+    return make_tile_list(first(p, t), last(p, t));
+  }
+  // the key tiles of both sub-tiles
+  __device__ __forceinline__ TileList all(const AttnForward& p) const {
+    return make_tile_list(first(p, 0), last(p, exists(p, 1) ? 1 : 0));
+  }
+  // this CTA's share of them
+  __device__ __forceinline__ void share(const AttnForward& p, int count, int& begin, int& end) const {
+    const int each = (count + p.splits - 1) / p.splits;
+    begin = min(split * each, count);
+    end = min(begin + each, count);
+  }
+};
+
 // Raise of the row maximum, in powers of two, up to which the old reference is kept: P is then at most 2^8, which
 // neither its BF16 rounding (relative) nor the FP32 sums mind, and O is rescaled only where it has to be.
 constexpr float kKeepMaximum = 8.0f;
@@ -67,44 +120,6 @@ __global__ void __launch_bounds__(384, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
-
-  // ---- this CTA's block of rows, heads and share of the key tiles
-  int w = blockIdx.x;
-  const int split = w % p.splits;
-  w /= p.splits;
-  const int head_set = w % p.head_sets;
-  w /= p.head_sets;
-  int sequence, row0;
-  const int rows = kTileRows / p.packed_heads;  // rows of a head in a sub-tile
-  const int row_step = p.pair_heads ? 0 : rows;
-  if (p.tiles != nullptr) {
-    const int2 tile = p.tiles[w];
-    sequence = tile.x, row0 = tile.y;
-  } else {
-    // the last rows first: under a causal mask they have the most keys
-    sequence = w % p.shape.batch;
-    row0 = (p.blocks_per_sequence - 1 - w / p.shape.batch) * (p.single || p.pair_heads ? rows : 2 * rows);
-  }
-  const AttnSeq seq = load_sequence(p.shape, sequence);
-  const int batch = p.shape.sequences != nullptr ? 0 : sequence;
-  const int head0 = head_set * p.packed_heads * (p.pair_heads ? 2 : 1);
-  const int kv_head = head0 / (p.shape.heads_q / p.shape.heads_kv);
-  // a row block behind the sequence's end (packed lists hold none; an empty second sub-tile is usual)
-  bool exists[2];
-  RowSpan first[2], last[2];
-  TileList own[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int r = row0 + t * row_step;
-    exists[t] = r < seq.nq && !(t == 1 && p.single);
-    first[t] = row_span(p.shape, seq, r);
-    last[t] = row_span(p.shape, seq, min(r + rows, seq.nq) - 1);
-    own[t] = make_tile_list(first[t], last[t]);
-    if (!exists[t]) own[t].sink_end = 0, own[t].low = 0, own[t].high = -1;
-  }
-  const TileList all = make_tile_list(first[0], exists[1] ? last[1] : last[0]);
-  const int per_split = (all.count + p.splits - 1) / p.splits;
-  const int begin = min(split * per_split, all.count), end = min(begin + per_split, all.count);
 
   if (threadIdx.x == 0) {
     *abort_flag = 0u;
@@ -133,8 +148,12 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
-    fewer_registers<40>();
+    fewer_registers<72>();
     if (warp == 8 && elect_one_sync()) {
+      const ForwardBlock block(p);
+      const TileList all = block.all(p);
+      int begin, end;
+      block.share(p, all.count, begin, end);
       // ------------------------------------------------------------ TMA loads
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
@@ -147,19 +166,20 @@ __global__ void __launch_bounds__(384, 1)
         const uint32_t dst = base + Cfg::kOffStages + s * Cfg::kTileBytes;
 #pragma unroll
         for (int panel = 0; panel < Cfg::kPanels; ++panel)
-          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, seq.k0 + kt * kTileRows, kv_head, batch, full(s));
+          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, block.seq.k0 + kt * kTileRows, block.kv_head, block.batch,
+                      full(s));
         ++loads;
         return true;
       };
       if (begin < end) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (!exists[t]) continue;
+          if (!block.exists(p, t)) continue;
           mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
 #pragma unroll
           for (int panel = 0; panel < Cfg::kPanels; ++panel)
             tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
-                        seq.q0 + row0 + t * row_step, head0 + (p.pair_heads ? t * p.packed_heads : 0), batch,
+                        block.seq.q0 + block.row0 + t * block.row_step, block.head0 + t * block.head_step, block.batch,
                         q_full(t));
           if (t == 0) ok = load_tile(k_map, all.tile(begin));
         }
@@ -171,13 +191,19 @@ __global__ void __launch_bounds__(384, 1)
       if (!ok) {  // the copies in flight end before this CTA's shared memory is given up
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (exists[t]) drain_barrier(q_full(t), 0);
+          if (block.exists(p, t)) drain_barrier(q_full(t), 0);
         for (int n = max(0, loads - Cfg::kStages); n < loads; ++n)
           drain_barrier(full(n % Cfg::kStages), (n / Cfg::kStages) & 1);
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------ products
       const bool leader = elect_one_sync();
+      const ForwardBlock block(p);
+      const TileList all = block.all(p);
+      const TileList own[2] = {block.tiles(p, 0), block.tiles(p, 1)};
+      const bool exists[2] = {block.exists(p, 0), block.exists(p, 1)};
+      int begin, end;
+      block.share(p, all.count, begin, end);
       int loads = 0, steps[2] = {0, 0};
       bool ok = true, pending[2] = {false, false};
       for (int i = begin; ok && begin < end && i <= end; ++i) {
@@ -240,27 +266,28 @@ __global__ void __launch_bounds__(384, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    more_registers<232>();
+    more_registers<216>();
     const int t = warp / 4;
     const int quarter = warp % 4;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem + t * kTileRows + lane_base;
     const uint32_t o_tmem = tmem + Cfg::kTmemO + t * DP + lane_base;
-    const int row = row0 + t * row_step + r % rows;
-    const int head = head0 + (p.pair_heads ? t * p.packed_heads : 0) + r / rows;
-    const bool mine = t == 0 ? exists[0] : exists[1];
-    const RowSpan my_first = t == 0 ? first[0] : first[1], my_last = t == 0 ? last[0] : last[1];
-    const TileList my_tiles = t == 0 ? own[0] : own[1];
-    const bool valid = mine && row < seq.nq;
-    const RowSpan span = row_span(p.shape, seq, row);
+    const ForwardBlock block(p);
+    const TileList all = block.all(p), mine = block.tiles(p, t);
+    const RowSpan first = block.first(p, t), last = block.last(p, t);
+    int begin, end;
+    block.share(p, all.count, begin, end);
+    const int row = block.row0 + t * block.row_step + r % block.rows;
+    const bool exists = block.exists(p, t);
+    const RowSpan span = row_span(p.shape, block.seq, row);
     const float c = p.shape.scale_log2;
     float top = -INFINITY, sum = 0.0f;
     int steps = 0;
     bool ok = true;
-    for (int i = begin; mine && i < end; ++i) {
+    for (int i = begin; exists && i < end; ++i) {
       const int j0 = all.tile(i) * kTileRows;
-      if (!sees_tile(my_tiles, all.tile(i))) continue;
+      if (!sees_tile(mine, all.tile(i))) continue;
       if (!ctl.wait(s_full(t), steps & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
         ok = false;
         break;
@@ -270,16 +297,10 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
       for (int b = 0; b < 4; ++b) tmem_ld_32x32(s_tmem + b * 32, raw[b]);
       tmem_ld_wait();
-      if (!tile_is_full(my_first, my_last, j0)) {
+      if (!tile_is_full(first, last, j0)) {
         const int low = span.low - j0, high = span.high - j0, sink = span.sink - j0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int j = b * 32 + x;
-            const bool seen = (j >= low && j <= high) || j < sink;
-            raw[b][x] = seen ? raw[b][x] : 0xff800000u;
-          }
+        for (int b = 0; b < 4; ++b) hide_scores(raw[b], span_bits(low - b * 32, high - b * 32, sink - b * 32));
       }
       float m4[4];
 #pragma unroll
@@ -344,18 +365,21 @@ __global__ void __launch_bounds__(384, 1)
     // ---- O / sum, rounded once
     if (ok) {
       tc_fence_after_sync();
-      const int64_t index = (static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + seq.q0 + row;
+      const int head = block.head0 + t * block.head_step + r / block.rows;
+      const bool valid = exists && row < block.seq.nq;
+      const int q_row = block.seq.q0 + row;
+      const int64_t index = (static_cast<int64_t>(block.batch) * p.shape.heads_q + head) * p.shape.seq_q + q_row;
       const float log2_sum = top * c + log2f(sum);
       const float scale = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
       if (valid) {
         const float lse2 = sum == 0.0f ? -INFINITY : log2_sum;
         if (p.splits > 1)
-          p.partial_lse[split * p.total_rows + index] = lse2;
+          p.partial_lse[block.split * p.total_rows + index] = lse2;
         else if (p.lse != nullptr)
           p.lse[index] = lse2 * 0.69314718055994531f;
       }
-      __nv_bfloat16* out = p.out + batch * p.out_batch + (seq.q0 + row) * p.out_seq + head * p.out_head;
-      float* partial = p.partial_out + (split * p.total_rows + index) * DP;
+      __nv_bfloat16* out = p.out + block.batch * p.out_batch + q_row * p.out_seq + head * p.out_head;
+      float* partial = p.partial_out + (block.split * p.total_rows + index) * DP;
 #pragma unroll 1
       for (int b = 0; b < DP / 32; ++b) {
         uint32_t o[32];
