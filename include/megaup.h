@@ -393,7 +393,7 @@ typedef struct mup_axial_rotary {
   int32_t device;
   int32_t batch;
   int32_t rows; /* per sequence of the batch */
-  int32_t head_dim; /* a multiple of 8, at most 512 */
+  int32_t head_dim; /* a multiple of 8, at most 256 */
   int32_t pairs; /* 2 * pairs <= head_dim; a multiple of 8 unless interleaved */
   int32_t axes;
   int32_t interleaved;

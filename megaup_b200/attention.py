@@ -267,7 +267,7 @@ class _Plan:
             # freed with this frame: the allocator hands it out again in stream order
             workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace_bytes
-        _native.call(function, ctypes.byref(a), torch.cuda.current_stream(self.device).cuda_stream)
+        _native.call(function, ctypes.byref(a), torch.cuda.current_stream(self.device.index).cuda_stream)
 
 
 _PLANS: dict[object, _Plan] = {}
@@ -317,7 +317,7 @@ def _forward(
 ) -> tuple[Tensor, Tensor | None]:
     a = plan.arguments(q, k, v)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=plan.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         a.out_strides = _stride_array(out.shape, out.stride(), plan.kind)
     a.out = out.data_ptr()
@@ -353,7 +353,7 @@ class _WindowAttention(torch.autograd.Function):
             dout = dout.clone(memory_format=torch.contiguous_format)
         elif not dout.is_contiguous():
             a.dout_strides = _stride_array(dout.shape, dout.stride(), plan.kind)
-        dq, dk, dv = grads = [torch.empty(x.shape, dtype=torch.bfloat16, device=plan.device) for x in (q, k, v)]
+        dq, dk, dv = grads = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v)]
         a.out, a.lse, a.dout = out.data_ptr(), lse.data_ptr(), dout.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         plan.launch("mup_window_attention_backward", a, plan.backward_bytes)

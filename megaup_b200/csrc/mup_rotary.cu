@@ -1,7 +1,7 @@
 // Rotary positions with several axes (include/megaup.h, mup_axial_rotary).
 //
 // Bound by memory: every element of q and k is read and written once. A warp
-// owns a row of the sequence (or a share of its heads): each lane holds the
+// owns a row of the sequence: each lane holds the
 // sines and cosines of the pairs of its 16-byte columns and walks the row's
 // heads of both tensors with them, so an angle is computed once per row and
 // not once per head, and no table of angles is read.
@@ -11,6 +11,14 @@
 // bits (position * frequency / 2 pi, error 2^-53 of the number of turns), the
 // whole turns are dropped there, and sine and cosine of the rest are taken in
 // 32 bits.
+//
+// Measured on B200 (32768 rows, 5 + 5 heads of 128, interleaved: 168 MB moved): 55 us with a warp per row and no
+// work kept between rows, 44 us with all loads of a row ahead of its angles, 35 us with resident warps and angles shared
+// between a warp's lanes, 31 us (5.4 TB/s, 82 % of the copy rate) with the heads' offsets kept as well. Two resident blocks
+// of 256 threads beat three (33 us, registers spill) and four (41 us). Rotated halves, 65536 rows of 8 + 2 heads in a fused
+// projection (335 MB): 123 us at first, 69 us (4.9 TB/s) with the two halves in two lanes.
+#include <algorithm>
+
 #include "mup_host.cuh"
 #include "mup_ptx.cuh"
 
@@ -27,16 +35,16 @@ struct RotaryParams {
   int64_t pos_axis, pos_batch, pos_row;
   const double* turns;
   const int* pair_axis;
-  int rows, head_dim, pairs, head_shares;
-  int64_t items;  // batch * rows * head_shares
+  uint32_t rows, items;  // of a sequence, of the batch
+  int head_dim, pairs, position_type;
+  int heads_each;  // heads that a group takes of a row, at most kHeads
   float sign;
 };
 
-template <int TYPE>
-__device__ __forceinline__ double load_position(const void* positions, int64_t at) {
-  if constexpr (TYPE == MUP_ROTARY_INT32) return static_cast<double>(static_cast<const int*>(positions)[at]);
-  if constexpr (TYPE == MUP_ROTARY_INT64) return static_cast<double>(static_cast<const long long*>(positions)[at]);
-  return static_cast<double>(static_cast<const float*>(positions)[at]);
+__device__ __forceinline__ double load_position(const RotaryParams& p, int64_t at) {
+  if (p.position_type == MUP_ROTARY_INT64) return static_cast<double>(static_cast<const long long*>(p.positions)[at]);
+  if (p.position_type == MUP_ROTARY_INT32) return static_cast<double>(static_cast<const int*>(p.positions)[at]);
+  return static_cast<double>(static_cast<const float*>(p.positions)[at]);
 }
 
 __device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
@@ -51,101 +59,125 @@ struct Turn {
   float cos, sin;
 };
 
-// Pairs from `pairs` on are not turned: cosine 1, sine 0 mark them.
-template <int TYPE>
-__device__ __forceinline__ Turn turn_of(const RotaryParams& p, int pair, int64_t at) {
-  const double position = load_position<TYPE>(p.positions, at + p.pair_axis[pair] * p.pos_axis);
-  const double turns = position * p.turns[pair];
-  const float rest = static_cast<float>(turns - rint(turns));
-  Turn t;
-  sincospif(2.0f * rest, &t.sin, &t.cos);
-  t.sin *= p.sign;
-  return t;
-}
+// The angles of a lane's N neighbouring pairs. Several lanes of a warp hold the same pairs (of different heads, and of
+// both halves of one): the first SHARED of them compute N / SHARED pairs each and hand them to the others. A lane keeps
+// the frequencies of those it computes and where their axes lie in `positions`.
+template <int N, int SHARED>
+struct LanePairs {
+  static constexpr int kEach = N / SHARED;
+  double turns[kEach];
+  int64_t axis[kEach];
 
-// Interleaved pairs: a lane's 16 bytes are four pairs. `lanes` lanes cover a head (a power of two up to 32), a warp's
-// 32 / lanes groups take every 32 / lanes-th head; heads wider than 256 take several passes of columns.
-template <int TYPE>
-__global__ void __launch_bounds__(256) rotary_interleaved_kernel(const RotaryParams p, int lanes) {
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  if (item >= p.items) return;
-  const int lane = threadIdx.x % 32;
-  const int share = static_cast<int>(item % p.head_shares);
-  const int64_t place = item / p.head_shares;
-  const int64_t b = place / p.rows, row = place - b * p.rows;
-  const int groups = 32 / lanes, group = lane / lanes;
-  const int64_t at = b * p.pos_batch + row * p.pos_row;
-  for (int column = (lane % lanes) * 8; column < p.head_dim; column += lanes * 8) {
-    Turn turn[4];
-    bool turned[4];
+  // `first`: the lane's first pair; `copy`: its place among the lanes with the same pairs.
+  __device__ __forceinline__ LanePairs(const RotaryParams& p, int first, int copy) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int pair = column / 2 + i;
-      turned[i] = pair < p.pairs;
-      if (turned[i]) turn[i] = turn_of<TYPE>(p, pair, at);
+    for (int i = 0; i < kEach; ++i) {
+      const int pair = first + i * SHARED + copy % SHARED;
+      const bool turned = pair < p.pairs;
+      turns[i] = turned ? p.turns[pair] : 0.0;
+      axis[i] = turned ? p.pair_axis[pair] * p.pos_axis : 0;
+    }
+  }
+  // The whole warp calls this; `lane_of(c)` is the lane that is copy c of the caller's pairs.
+  template <typename LaneOf>
+  __device__ __forceinline__ void turn(const RotaryParams& p, int64_t at, LaneOf lane_of, Turn (&t)[N]) const {
+    double position[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) position[i] = load_position(p, at + axis[i]);
+    Turn mine[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const double all = position[i] * turns[i];
+      const float rest = static_cast<float>(all - rint(all));
+      sincospif(2.0f * rest, &mine[i].sin, &mine[i].cos);
+      mine[i].sin *= p.sign;
     }
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const __nv_bfloat16* x = p.x[which] + b * p.x_batch[which] + row * p.x_row[which] + column;
-      __nv_bfloat16* y = p.y[which] + b * p.y_batch[which] + row * p.y_row[which] + column;
-#pragma unroll 4
-      for (int head = share * groups + group; head < p.heads[which]; head += p.head_shares * groups) {
-        uint4 v = *reinterpret_cast<const uint4*>(x + head * p.x_head[which]);
-        uint32_t* words = &v.x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = low_bf16(words[i]), c = high_bf16(words[i]);
-          if (turned[i]) words[i] = two_bf16(a * turn[i].cos - c * turn[i].sin, a * turn[i].sin + c * turn[i].cos);
-        }
-        *reinterpret_cast<uint4*>(y + head * p.y_head[which]) = v;
+    for (int i = 0; i < N; ++i) {
+      t[i] = mine[i / SHARED];
+      if constexpr (SHARED > 1) {
+        const int from = lane_of(i % SHARED);
+        t[i].cos = __shfl_sync(0xffffffffu, t[i].cos, from);
+        t[i].sin = __shfl_sync(0xffffffffu, t[i].sin, from);
       }
     }
   }
-}
+};
 
-// Halves: pair p is (p, p + pairs); a lane holds eight pairs as 16 bytes of each half. The columns behind 2 * pairs
-// are copied by the lanes behind the pairs'.
-template <int TYPE>
-__global__ void __launch_bounds__(256) rotary_halves_kernel(const RotaryParams p, int lanes) {
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  if (item >= p.items) return;
+// A lane holds 16 bytes of a head, `lanes` lanes (a power of two up to 32) a head, and the 32 / lanes groups of a warp take
+// every 32 / lanes-th head of a row: up to kHeads heads each, whose loads are in flight while the angles are computed.
+// Rows with more heads are cut along the grid's second dimension (and their angles computed again, a third of the
+// instructions). Interleaved, the 16 bytes are four pairs. Otherwise they are one half of eight pairs, whose other half
+// lies pairs / 8 lanes away and is exchanged by shuffles: loads and stores stay those of the interleaved form.
+constexpr int kHeads = 6;
+constexpr int kResident = 2;  // blocks per SM
+
+template <bool INTERLEAVED, int SHARED>
+__global__ void __launch_bounds__(256, kResident) rotary_kernel(const __grid_constant__ RotaryParams p, int lanes) {
+  constexpr int kPairs = INTERLEAVED ? 4 : 8;
   const int lane = threadIdx.x % 32;
-  const int share = static_cast<int>(item % p.head_shares);
-  const int64_t place = item / p.head_shares;
-  const int64_t b = place / p.rows, row = place - b * p.rows;
-  const int groups = 32 / lanes, group = lane / lanes;
-  const int64_t at = b * p.pos_batch + row * p.pos_row;
-  const int units = p.pairs / 8 + (p.head_dim - 2 * p.pairs) / 8;
-  for (int unit = lane % lanes; unit < units; unit += lanes) {
-    const bool turned = unit < p.pairs / 8;
-    const int column = turned ? unit * 8 : p.pairs + unit * 8;
-    Turn turn[8];
-    if (turned) {
+  const int groups = 32 / lanes, group = lane / lanes, place = lane % lanes;
+  const int column = place * 8;
+  const int half_lanes = p.pairs / 8;  // not interleaved: lanes of a half
+  const bool second = !INTERLEAVED && place >= half_lanes;
+  const int pair0 = INTERLEAVED ? place * 4 : (place - (second ? half_lanes : 0)) * 8;
+  const int other = lane + (second ? -half_lanes : half_lanes);
+  const int copies = INTERLEAVED ? 1 : 2;
+  const auto lane_of = [&](int copy) {
+    return INTERLEAVED ? copy * lanes + place : copy / 2 * lanes + min(pair0 / 8 + copy % 2 * half_lanes, lanes - 1);
+  };
+  const LanePairs<kPairs, SHARED> pairs(p, pair0, group * copies + (second ? 1 : 0));
+  // the group's heads of both tensors, as offsets of 16 bytes from a row's start
+  const int heads = p.heads[0] + p.heads[1];
+  uint32_t x_at[kHeads], y_at[kHeads], used = 0, second_tensor = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) turn[i] = turn_of<TYPE>(p, column + i, at);
+  for (int h = 0; h < kHeads; ++h) {
+    int head = (blockIdx.y * p.heads_each + h) * groups + group;
+    if (h >= p.heads_each || head >= heads || column >= p.head_dim) continue;
+    const int t = head >= p.heads[0];
+    head -= t ? p.heads[0] : 0;
+    used |= 1u << h;
+    second_tensor |= t << h;
+    x_at[h] = static_cast<uint32_t>((head * p.x_head[t] + column) / 8);
+    y_at[h] = static_cast<uint32_t>((head * p.y_head[t] + column) / 8);
+  }
+  for (uint32_t item = blockIdx.x * 8 + threadIdx.x / 32; item < p.items; item += gridDim.x * 8) {
+    const uint32_t b = p.rows == p.items ? 0 : item / p.rows, row = item - b * p.rows;
+    const uint4* x[2];
+    uint4* y[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t] = reinterpret_cast<const uint4*>(p.x[t] + b * p.x_batch[t] + row * p.x_row[t]);
+      y[t] = reinterpret_cast<uint4*>(p.y[t] + b * p.y_batch[t] + row * p.y_row[t]);
+    }
+    uint4 v[kHeads];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+      if (used >> h & 1) v[h] = ld_stream_v4(((second_tensor >> h & 1) ? x[1] : x[0]) + x_at[h]);
+    Turn turn[kPairs];
+    pairs.turn(p, b * p.pos_batch + row * p.pos_row, lane_of, turn);
+    if constexpr (!INTERLEAVED) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turn[i].sin = second ? turn[i].sin : -turn[i].sin;
     }
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const __nv_bfloat16* x = p.x[which] + b * p.x_batch[which] + row * p.x_row[which] + column;
-      __nv_bfloat16* y = p.y[which] + b * p.y_batch[which] + row * p.y_row[which] + column;
-#pragma unroll 2
-      for (int head = share * groups + group; head < p.heads[which]; head += p.head_shares * groups) {
-        uint4 v = *reinterpret_cast<const uint4*>(x + head * p.x_head[which]);
-        if (turned) {
-          uint4 w = *reinterpret_cast<const uint4*>(x + head * p.x_head[which] + p.pairs);
-          uint32_t *first = &v.x, *second = &w.x;
+    for (int h = 0; h < kHeads; ++h) {
+      if (h >= p.heads_each) break;
+      uint32_t* words = &v[h].x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a0 = low_bf16(first[i]), a1 = high_bf16(first[i]);
-            const float c0 = low_bf16(second[i]), c1 = high_bf16(second[i]);
-            const Turn t0 = turn[2 * i], t1 = turn[2 * i + 1];
-            first[i] = two_bf16(a0 * t0.cos - c0 * t0.sin, a1 * t1.cos - c1 * t1.sin);
-            second[i] = two_bf16(a0 * t0.sin + c0 * t0.cos, a1 * t1.sin + c1 * t1.cos);
-          }
-          *reinterpret_cast<uint4*>(y + head * p.y_head[which] + p.pairs) = w;
+      for (int i = 0; i < 4; ++i) {
+        const float lo = low_bf16(words[i]), hi = high_bf16(words[i]);
+        if constexpr (INTERLEAVED) {
+          if (pair0 + i < p.pairs)
+            words[i] = two_bf16(lo * turn[i].cos - hi * turn[i].sin, lo * turn[i].sin + hi * turn[i].cos);
+        } else {
+          const uint32_t there = __shfl_sync(0xffffffffu, words[i], other);
+          const Turn t0 = turn[2 * i], t1 = turn[2 * i + 1];
+          if (pair0 < p.pairs)
+            words[i] = two_bf16(lo * t0.cos + low_bf16(there) * t0.sin, hi * t1.cos + high_bf16(there) * t1.sin);
         }
-        *reinterpret_cast<uint4*>(y + head * p.y_head[which]) = v;
       }
+      if (used >> h & 1) ((second_tensor >> h & 1) ? y[1] : y[0])[y_at[h]] = v[h];
     }
   }
 }
@@ -160,16 +192,23 @@ int check_rows(const char* name, const void* base, const int64_t strides[3]) {
   return MUP_OK;
 }
 
-template <int TYPE>
-void launch(const RotaryParams& p, bool interleaved, cudaStream_t stream) {
-  const int units = interleaved ? p.head_dim / 8 : p.pairs / 8 + (p.head_dim - 2 * p.pairs) / 8;
+constexpr unsigned kBlocks = 148 * kResident;
+
+void launch(RotaryParams& p, bool interleaved, cudaStream_t stream) {
   int lanes = 1;
-  while (lanes < units && lanes < 32) lanes *= 2;
-  const unsigned grid = static_cast<unsigned>((p.items + 7) / 8);
+  while (lanes * 8 < p.head_dim) lanes *= 2;
+  const int per_group = (p.heads[0] + p.heads[1] + 32 / lanes - 1) / (32 / lanes);
+  const int parts = (per_group + kHeads - 1) / kHeads;
+  p.heads_each = (per_group + parts - 1) / parts;
+  const int copies = 32 / lanes * (interleaved ? 1 : 2);
+  // Warps stay for several rows: a lane's frequencies are read once, and a block's start is paid once.
+  const dim3 grid(std::min((p.items + 7) / 8, kBlocks), parts);
+  void (*kernel)(RotaryParams, int);
   if (interleaved)
-    rotary_interleaved_kernel<TYPE><<<grid, 256, 0, stream>>>(p, lanes);
+    kernel = copies >= 4 ? rotary_kernel<true, 4> : copies == 2 ? rotary_kernel<true, 2> : rotary_kernel<true, 1>;
   else
-    rotary_halves_kernel<TYPE><<<grid, 256, 0, stream>>>(p, lanes);
+    kernel = copies >= 8 ? rotary_kernel<false, 8> : copies == 4 ? rotary_kernel<false, 4> : rotary_kernel<false, 2>;
+  kernel<<<grid, 256, 0, stream>>>(p, lanes);
 }
 
 }  // namespace
@@ -177,8 +216,8 @@ void launch(const RotaryParams& p, bool interleaved, cudaStream_t stream) {
 extern "C" int mup_axial_rotary_launch(const mup_axial_rotary* args, void* stream) {
   if (args == nullptr) return host_fail(MUP_ERR_BAD_ARG, "axial rotary: null argument");
   const mup_axial_rotary& a = *args;
-  if (a.head_dim < 8 || a.head_dim > 512 || a.head_dim % 8 != 0)
-    return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: head_dim %d is not a multiple of 8 up to 512", a.head_dim);
+  if (a.head_dim < 8 || a.head_dim > 256 || a.head_dim % 8 != 0)
+    return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: head_dim %d is not a multiple of 8 up to 256", a.head_dim);
   if (a.pairs < 1 || 2 * a.pairs > a.head_dim || (!a.interleaved && a.pairs % 8 != 0))
     return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: %d pairs in heads of %d", a.pairs, a.head_dim);
   if (a.batch < 1 || a.rows < 1 || a.axes < 1 || a.heads[0] < 1 || a.heads[1] < 0)
@@ -196,24 +235,24 @@ extern "C" int mup_axial_rotary_launch(const mup_axial_rotary* args, void* strea
     p.x_batch[t] = a.x_strides[t][0], p.x_row[t] = a.x_strides[t][1], p.x_head[t] = a.x_strides[t][2];
     p.y_batch[t] = a.y_strides[t][0], p.y_row[t] = a.y_strides[t][1], p.y_head[t] = a.y_strides[t][2];
     p.heads[t] = a.heads[t];
+    // a head's place in a row is kept as 32 bits of 16-byte units
+    for (int64_t stride : {a.x_strides[t][2], a.y_strides[t][2]})
+      if (a.heads[t] > 65536 || stride / 8 * a.heads[t] > 0xffffffffll)
+        return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: %d heads at a stride of %lld", a.heads[t],
+                         static_cast<long long>(stride));
   }
   p.positions = a.positions;
   p.pos_axis = a.pos_strides[0], p.pos_batch = a.pos_strides[1], p.pos_row = a.pos_strides[2];
   p.turns = a.turns, p.pair_axis = a.pair_axis;
-  p.rows = a.rows, p.head_dim = a.head_dim, p.pairs = a.pairs;
-  p.head_shares = 1;
-  p.items = static_cast<int64_t>(a.batch) * a.rows * p.head_shares;
-  if (p.items / 8 >= 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: too many rows");
+  p.rows = a.rows, p.head_dim = a.head_dim, p.pairs = a.pairs, p.position_type = a.position_type;
+  const int64_t items = static_cast<int64_t>(a.batch) * a.rows;
+  if (items > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "axial rotary: %lld rows", static_cast<long long>(items));
+  p.items = static_cast<uint32_t>(items);
   p.sign = a.inverse ? -1.0f : 1.0f;
   DeviceScope scope(a.device);
   MUP_HOST_CUDA(scope.error());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.position_type == MUP_ROTARY_INT32)
-    launch<MUP_ROTARY_INT32>(p, a.interleaved != 0, s);
-  else if (a.position_type == MUP_ROTARY_INT64)
-    launch<MUP_ROTARY_INT64>(p, a.interleaved != 0, s);
-  else
-    launch<MUP_ROTARY_FLOAT32>(p, a.interleaved != 0, s);
+  launch(p, a.interleaved != 0, s);
   MUP_HOST_CUDA(cudaGetLastError());
   return MUP_OK;
 }

@@ -74,8 +74,8 @@ def prepare_axial_rotary(
     if not dims or min(dims) <= 0 or any(d % 2 for d in dims):
         raise ValueError(f"axis_dims must be positive even numbers, got {tuple(axis_dims)}")
     total = sum(dims)
-    if total > 512:
-        raise ValueError(f"at most 512 elements of a head can be turned, got {total}")
+    if total > 256:
+        raise ValueError(f"at most 256 elements of a head can be turned, got {total}")
     if not interleaved and total % 16:
         raise ValueError(f"rotated halves need sum(axis_dims) to be a multiple of 16, got {total}")
     theta = float(theta)
@@ -102,9 +102,9 @@ def _check(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, position
     _check_heads_tensor(q, "q", kind, None)
     batch_axis, row_axis, _ = _AXES[kind]
     head_dim = q.shape[-1]
-    if head_dim % 8 or head_dim > 512 or 2 * rotary.pairs > head_dim:
+    if head_dim % 8 or head_dim > 256 or 2 * rotary.pairs > head_dim:
         raise ValueError(
-            f"head_dim must be a multiple of 8 up to 512 and hold the {2 * rotary.pairs} turned elements, got {head_dim}"
+            f"head_dim must be a multiple of 8 up to 256 and hold the {2 * rotary.pairs} turned elements, got {head_dim}"
         )
     if k is not None:
         _check_heads_tensor(k, "k", kind, q.device)
@@ -180,11 +180,11 @@ def _turn(
     if not dense:
         a.y_strides[: 3 * len(outputs)] = [s for t in outputs for s in _row_strides(t.shape, t.stride(), kind)]
     a.positions, a.inverse = positions.data_ptr(), inverse
-    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(tensors[0].device).cuda_stream)
+    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(tensors[0].get_device()).cuda_stream)
 
 
 def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
-    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    return [torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors]
 
 
 class _AxialRotary(torch.autograd.Function):

@@ -39,7 +39,7 @@ def test_frequencies(shared) -> None:
 
 @pytest.mark.parametrize(
     "dims,settings",
-    [([], {}), ([3], {}), ([0, 4], {}), ([-2], {}), ([512, 2], {}), ([24], dict(interleaved=False)),
+    [([], {}), ([3], {}), ([0, 4], {}), ([-2], {}), ([256, 2], {}), ([24], dict(interleaved=False)),
      ([64], dict(theta=0.0)), ([64], dict(theta=float("inf"))), ([64], dict(theta=float("nan")))],
     ids=str,
 )
@@ -62,7 +62,7 @@ def _block(**changes) -> _native.MupAxialRotary:
 
 @pytest.mark.parametrize(
     "changes",
-    [dict(head_dim=4), dict(head_dim=68), dict(head_dim=520), dict(pairs=0), dict(pairs=33), dict(interleaved=0, pairs=12),
+    [dict(head_dim=4), dict(head_dim=68), dict(head_dim=264), dict(pairs=0), dict(pairs=33), dict(interleaved=0, pairs=12),
      dict(batch=0), dict(rows=0), dict(axes=0), dict(heads=(ctypes.c_int32 * 2)(0, 1)), dict(positions=0), dict(turns=0),
      dict(pair_axis=0), dict(position_type=3), dict(x=(ctypes.c_void_p * 2)(4096, 0)),
      dict(y=(ctypes.c_void_p * 2)(4104, 4096)), dict(x_strides=(ctypes.c_int64 * 6)(512, 129, 64, 512, 128, 64)),
@@ -111,8 +111,9 @@ CASES = [
     ("thd", 1, 301, 40, 8, 64, [16, 8, 8], False, False, torch.int32, False),  # 32 elements stay
     ("thd", 1, 77, 9, None, 72, [2], True, False, torch.int64, False),
     ("thd", 1, 50, 2, 2, 256, [128, 64, 64], True, False, torch.float32, False),
-    ("bshd", 2, 30, 3, 3, 512, [512], False, False, torch.int64, False),
-    ("bshd", 2, 30, 3, 3, 512, [200, 200, 112], True, False, torch.int64, True),
+    ("bshd", 2, 30, 3, 3, 256, [256], False, False, torch.int64, False),
+    ("bshd", 2, 30, 3, 3, 248, [100, 100, 48], True, False, torch.int64, True),
+    ("bshd", 2, 30, 3, 3, 248, [48, 64], False, True, torch.int64, True),
     ("bshd", 1, 64, 33, 1, 8, [6], True, False, torch.int64, False),
     ("sbhd", 1, 64, 33, 1, 24, [16], False, False, torch.int64, False),
 ]
