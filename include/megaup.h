@@ -365,8 +365,9 @@ typedef struct mup_window_attention {
   uint64_t timeout_ns; /* bound of the waits inside the kernels */
 } mup_window_attention;
 
-/* Bytes of workspace the two passes need for this problem (host arithmetic; the
- * pointers need not be set). Either output pointer may be NULL. */
+/* Bytes of workspace the two passes need for this problem (host arithmetic; of
+ * the pointers only whether kv_lengths and sequences are NULL counts). Either
+ * output pointer may be NULL. */
 int mup_window_attention_workspace(const mup_window_attention *args, uint64_t *forward_bytes,
                                    uint64_t *backward_bytes);
 int mup_window_attention_forward(const mup_window_attention *args, void *stream);

@@ -184,7 +184,7 @@ class _Plan:
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
-        scale: float | None, sequences: PackedSequences | None,
+        scale: float | None, sequences: PackedSequences | None, with_lengths: bool,
     ) -> None:
         _check_heads_tensor(q, "q", kind, None)
         _check_heads_tensor(k, "k", kind, q.device)
@@ -241,10 +241,12 @@ class _Plan:
                 setattr(a, "n_" + name, len(blocks))
             a.longest_q, a.longest_k = sequences.longest_q, sequences.longest_k
         a.timeout_ns = _KERNEL_TIMEOUT_NS
+        a.kv_lengths = 1 if with_lengths else None  # only whether there are any matters here
         forward, backward = ctypes.c_uint64(), ctypes.c_uint64()
         _native.call(
             "mup_window_attention_workspace", ctypes.byref(a), ctypes.byref(forward), ctypes.byref(backward)
         )
+        a.kv_lengths = None
         self.kind, self.block, self.device = kind, bytes(a), q.device
         # a plan that a backward pass still holds keeps the tables whose addresses it knows
         self.tables = None if sequences is None else (
@@ -276,17 +278,17 @@ _MAX_PLANS = 512
 
 def _plan(
     kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
-    sequences: PackedSequences | None,
+    sequences: PackedSequences | None, with_lengths: bool,
 ) -> _Plan:
     plans = _PLANS if sequences is None else sequences.plans
     try:
         key = (
             kind, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
-            q.device, k.device, v.device, causal, window, sinks, type(sinks), scale,
+            q.device, k.device, v.device, causal, window, sinks, type(sinks), scale, with_lengths,
         )
         return plans[key]
     except (KeyError, TypeError, AttributeError):  # new, a list as the window, not a tensor
-        plan = _Plan(kind, q, k, v, causal, window, sinks, scale, sequences)
+        plan = _Plan(kind, q, k, v, causal, window, sinks, scale, sequences, with_lengths)
     if len(plans) >= _MAX_PLANS:
         plans.clear()
     plans[(*key[:14], tuple(window), *key[15:]) if isinstance(window, list) else key] = plan
@@ -364,7 +366,7 @@ def _attend(
     kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
     kv_lengths: Tensor | None, sequences: PackedSequences | None, out: Tensor | None, return_lse: bool,
 ):
-    plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences)
+    plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences, kv_lengths is not None)
     if kv_lengths is not None:
         _check_kv_lengths(kv_lengths, q, kind)
     if out is not None:

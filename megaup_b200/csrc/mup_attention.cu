@@ -4,6 +4,7 @@
 
 #include "mup_attn_backward.cuh"
 #include "mup_attn_forward.cuh"
+#include "mup_attn_tokens.cuh"
 #include "mup_host.cuh"
 
 namespace {
@@ -99,9 +100,62 @@ ForwardPlan plan_forward(const mup_window_attention& a) {
   return f;
 }
 
-uint64_t forward_workspace(const mup_window_attention& a, const ForwardPlan& f) {
-  if (f.splits <= 1) return 0;
-  return static_cast<uint64_t>(f.splits) * total_rows(a) * (padded_dim(a) + 1) * sizeof(float);
+// Few query rows: the kernel for tokens over a cache.
+bool few_rows(const mup_window_attention& a) {
+  const int queries = a.sequences != nullptr ? a.longest_q : a.seq_q;
+  return static_cast<int64_t>(a.heads_q / a.heads_kv) * queries <= kTokenRows;
+}
+
+constexpr int kTokenShare = 2048;  // keys of a CTA (measured on 16 sequences of up to 65536 keys: 512 84 us, 1024 73, 2048 67)
+
+struct TokenPlan {
+  int splits, share;
+  bool cluster;
+};
+
+TokenPlan plan_tokens(const mup_window_attention& a) {
+  const bool packed = a.sequences != nullptr;
+  const AttnShape s = make_shape(a, nullptr);
+  const int keys = packed ? a.longest_k : a.seq_k, queries = packed ? a.longest_q : a.seq_q;
+  const int64_t window = std::min<int64_t>(static_cast<int64_t>(s.left) + s.right + queries, keys);
+  const int64_t visible = std::min<int64_t>(keys, window + s.sinks);
+  const int64_t places = static_cast<int64_t>(packed ? a.n_sequences : a.batch) * a.heads_kv;
+  const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenStep * kTokenWarps));
+  const int64_t fill = std::max<int64_t>(1, kTokenCtas * kSms / places);
+  TokenPlan t{};
+  if (most <= 2 * kTokenCluster) {  // short: the latency of a second kernel would be felt
+    t.splits = static_cast<int>(std::min<int64_t>({most, fill, kTokenCluster}));
+    t.cluster = t.splits > 1;
+    return t;
+  }
+  t.splits = static_cast<int>(std::min<int64_t>({most, fill, kMostSplits}));
+  // Sequences of different lengths, cut for the longest: shares of one size, so that no CTA has more to do than others
+  // and a short sequence leaves its last CTAs nothing.
+  if (packed || a.kv_lengths != nullptr) {
+    t.splits = static_cast<int>(std::max<int64_t>(t.splits, std::min<int64_t>(visible / kTokenShare, kMostSplits)));
+    const int64_t steps = visible / kTokenStep + 2;  // the sinks' and the window's first steps may be cut
+    t.share = ceil_div(ceil_div(steps, t.splits), kTokenWarps) * kTokenWarps;
+  }
+  return t;
+}
+
+uint64_t partial_bytes(const mup_window_attention& a, int splits) {
+  return static_cast<uint64_t>(splits) * total_rows(a) * (padded_dim(a) + 1) * sizeof(float);
+}
+
+uint64_t forward_workspace(const mup_window_attention& a) {
+  if (few_rows(a)) {
+    const TokenPlan t = plan_tokens(a);
+    return t.cluster || t.splits <= 1 ? 0 : partial_bytes(a, t.splits);
+  }
+  const ForwardPlan f = plan_forward(a);
+  return f.splits <= 1 ? 0 : partial_bytes(a, f.splits);
+}
+
+int check_workspace(const mup_window_attention& a, uint64_t needed) {
+  if (needed == 0 || (a.workspace != nullptr && a.workspace_bytes >= needed)) return MUP_OK;
+  return host_fail(MUP_ERR_BAD_ARG, "window attention: the workspace has %llu bytes, %llu are needed",
+                   static_cast<unsigned long long>(a.workspace_bytes), static_cast<unsigned long long>(needed));
 }
 
 int encode_rows(CUtensorMap* map, const mup_window_attention& a, const void* base, const int64_t strides[3], int rows,
@@ -114,12 +168,27 @@ int encode_rows(CUtensorMap* map, const mup_window_attention& a, const void* bas
 }
 
 template <int DP>
+int launch_combine(const mup_window_attention& a, const float* partial_out, const float* partial_lse, int splits,
+                   cudaStream_t stream) {
+  AttnCombine c{};
+  c.partial_out = partial_out, c.partial_lse = partial_lse, c.splits = splits;
+  c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = total_rows(a);
+  c.out = static_cast<__nv_bfloat16*>(a.out);
+  c.out_batch = a.out_strides[0], c.out_seq = a.out_strides[1], c.out_head = a.out_strides[2], c.lse = a.lse;
+  // launched while the CTAs before it run (it waits for them on the GPU)
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(c.total_rows)), config.blockDim = dim3(128), config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute, config.numAttrs = 1;
+  MUP_HOST_CUDA(cudaLaunchKernelEx(&config, attention_combine_kernel<DP>, c));
+  return MUP_OK;
+}
+
+template <int DP>
 int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
   const ForwardPlan f = plan_forward(a);
-  if (forward_workspace(a, f) > a.workspace_bytes || (f.splits > 1 && a.workspace == nullptr))
-    return host_fail(MUP_ERR_BAD_ARG, "window attention: the workspace has %llu bytes, %llu are needed",
-                     static_cast<unsigned long long>(a.workspace_bytes),
-                     static_cast<unsigned long long>(forward_workspace(a, f)));
   CUtensorMap q_map, k_map, v_map;
   int rc = encode_rows(&q_map, a, a.q, a.q_strides, a.seq_q, a.heads_q, kTileRows / f.packed_heads, f.packed_heads);
   if (rc == MUP_OK) rc = encode_rows(&k_map, a, a.k, a.k_strides, a.seq_k, a.heads_kv, kTileRows, 1);
@@ -145,14 +214,40 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
   if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many row blocks");
   attention_forward_kernel<DP><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map);
   MUP_HOST_CUDA(cudaGetLastError());
-  if (f.splits > 1) {
-    AttnCombine c{};
-    c.partial_out = p.partial_out, c.partial_lse = p.partial_lse, c.splits = f.splits;
-    c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = p.total_rows;
-    c.out = p.out, c.out_batch = p.out_batch, c.out_seq = p.out_seq, c.out_head = p.out_head, c.lse = p.lse;
-    attention_combine_kernel<DP><<<ceil_div(p.total_rows, 4), 128, 0, stream>>>(c);
-    MUP_HOST_CUDA(cudaGetLastError());
-  }
+  if (f.splits > 1) return launch_combine<DP>(a, p.partial_out, p.partial_lse, f.splits, stream);
+  return MUP_OK;
+}
+
+template <int DP>
+int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
+  const TokenPlan plan = plan_tokens(a);
+  AttnTokens p{};
+  p.shape = make_shape(a, status);
+  p.q = static_cast<const __nv_bfloat16*>(a.q), p.k = static_cast<const __nv_bfloat16*>(a.k);
+  p.v = static_cast<const __nv_bfloat16*>(a.v), p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.q_batch = a.q_strides[0], p.q_seq = a.q_strides[1], p.q_head = a.q_strides[2];
+  p.k_batch = a.k_strides[0], p.k_seq = a.k_strides[1], p.k_head = a.k_strides[2];
+  p.v_batch = a.v_strides[0], p.v_seq = a.v_strides[1], p.v_head = a.v_strides[2];
+  p.out_batch = a.out_strides[0], p.out_seq = a.out_strides[1], p.out_head = a.out_strides[2];
+  p.lse = a.lse;
+  p.splits = plan.splits, p.share = plan.share, p.cluster = plan.cluster;
+  p.total_rows = total_rows(a);
+  p.partial_out = static_cast<float*>(a.workspace);
+  p.partial_lse = p.partial_out + (plan.splits > 1 && !plan.cluster ? plan.splits * p.total_rows * DP : 0);
+  using Cfg = AttnTokensConfig<DP>;
+  const int64_t grid = static_cast<int64_t>(a.sequences != nullptr ? a.n_sequences : a.batch) * a.heads_kv * plan.splits;
+  if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many sequences");
+  static uint64_t ready = 0;
+  MUP_HOST_CUDA(allow_smem_once(attention_tokens_kernel<DP>, Cfg::kSmemBytes, a.device, &ready));
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(grid)), config.blockDim = dim3(32 * kTokenWarps);
+  config.dynamicSmemBytes = Cfg::kSmemBytes, config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(plan.splits), attribute.val.clusterDim.y = 1, attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute, config.numAttrs = plan.cluster ? 1 : 0;
+  MUP_HOST_CUDA(cudaLaunchKernelEx(&config, attention_tokens_kernel<DP>, p));
+  if (plan.splits > 1 && !plan.cluster) return launch_combine<DP>(a, p.partial_out, p.partial_lse, plan.splits, stream);
   return MUP_OK;
 }
 
@@ -203,10 +298,8 @@ uint64_t backward_workspace(const mup_window_attention& a, const BackwardPlan& b
 template <int DP>
 int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
   const BackwardPlan plan = plan_backward(a);
-  if (backward_workspace(a, plan) > a.workspace_bytes || a.workspace == nullptr)
-    return host_fail(MUP_ERR_BAD_ARG, "window attention: the workspace has %llu bytes, %llu are needed",
-                     static_cast<unsigned long long>(a.workspace_bytes),
-                     static_cast<unsigned long long>(backward_workspace(a, plan)));
+  const int checked = check_workspace(a, backward_workspace(a, plan));
+  if (checked != MUP_OK) return checked;
   CUtensorMap q_map, k_map, v_map, do_map;
   int rc = encode_rows(&q_map, a, a.q, a.q_strides, a.seq_q, a.heads_q, kTileRows, 1);
   if (rc == MUP_OK) rc = encode_rows(&do_map, a, a.dout, a.dout_strides, a.seq_q, a.heads_q, kTileRows, 1);
@@ -272,7 +365,7 @@ int mup_window_attention_workspace(const mup_window_attention* args, uint64_t* f
                                    uint64_t* backward_bytes) {
   const int rc = check_problem(args);
   if (rc != MUP_OK) return rc;
-  if (forward_bytes != nullptr) *forward_bytes = forward_workspace(*args, plan_forward(*args));
+  if (forward_bytes != nullptr) *forward_bytes = forward_workspace(*args);
   if (backward_bytes != nullptr) *backward_bytes = backward_workspace(*args, plan_backward(*args));
   return MUP_OK;
 }
@@ -283,6 +376,7 @@ int mup_window_attention_forward(const mup_window_attention* args, void* stream)
   if (rc == MUP_OK) rc = check_tensor("k", args->k, args->k_strides);
   if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
   if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
+  if (rc == MUP_OK) rc = check_workspace(*args, forward_workspace(*args));
   if (rc != MUP_OK) return rc;
   DeviceScope scope(args->device);
   MUP_HOST_CUDA(scope.error());
@@ -290,6 +384,7 @@ int mup_window_attention_forward(const mup_window_attention* args, void* stream)
   rc = device_status_word(args->device, &status);
   if (rc != MUP_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (few_rows(*args)) return args->head_dim <= 64 ? launch_tokens<64>(*args, s, status) : launch_tokens<128>(*args, s, status);
   return args->head_dim <= 64 ? launch_forward<64>(*args, s, status) : launch_forward<128>(*args, s, status);
 }
 

@@ -61,22 +61,22 @@ __device__ __forceinline__ RowSpan row_span(const AttnShape& p, const AttnSeq& s
   return r;
 }
 
-// The key tiles that the rows [first, last] see, in ascending order.
+// The key tiles (of kTileRows keys, or another size) that the rows [first, last] see, in ascending order.
 struct TileList {
   int split, second, count;  // entries [0, split) are tiles 0.., the rest start at tile `second`
   int sink_end, low, high;   // the rows' union of keys
   __device__ __forceinline__ int tile(int i) const { return i < split ? i : second + (i - split); }
 };
 
-__device__ __forceinline__ TileList make_tile_list(const RowSpan& first, const RowSpan& last) {
+__device__ __forceinline__ TileList make_tile_list(const RowSpan& first, const RowSpan& last, int size = kTileRows) {
   TileList t;
   t.sink_end = last.sink, t.low = first.low, t.high = last.high;
-  const int sink_tiles = (last.sink + kTileRows - 1) / kTileRows;
+  const int sink_tiles = (last.sink + size - 1) / size;
   if (last.high < first.low) {
     t.split = 0, t.second = 0, t.count = sink_tiles;
     return t;
   }
-  const int w0 = first.low / kTileRows, w1 = last.high / kTileRows;
+  const int w0 = first.low / size, w1 = last.high / size;
   if (sink_tiles == 0) {
     t.split = 0, t.second = w0, t.count = w1 - w0 + 1;
   } else if (w0 <= sink_tiles) {
@@ -94,8 +94,8 @@ __device__ __forceinline__ bool sees_tile(const TileList& t, int kt) {
 }
 
 // Whether every key of the tile is seen by every row between `first` and `last`.
-__device__ __forceinline__ bool tile_is_full(const RowSpan& first, const RowSpan& last, int j0) {
-  return (j0 >= last.low && j0 + kTileRows - 1 <= first.high) || j0 + kTileRows <= first.sink;
+__device__ __forceinline__ bool tile_is_full(const RowSpan& first, const RowSpan& last, int j0, int size = kTileRows) {
+  return (j0 >= last.low && j0 + size - 1 <= first.high) || j0 + size <= first.sink;
 }
 
 // Bit x of the result: x < n (n may be anything).

@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(384, 1)
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
+  grid_dep_launch();
   if (threadIdx.x == 0) {
     *abort_flag = 0u;
     mbar_init(q_full(0), 1);
@@ -421,48 +422,75 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
-// Joins the partial results of `splits` CTAs per row, always in the same order: one warp per row.
+// Joins the partial results of `splits` CTAs per row, always in the same order: a block per row, 128 / (DP / 4) threads
+// per four columns, each with every so-many-th split.
 struct AttnCombine {
   const float* partial_out;
   const float* partial_lse;
-  int splits, row_floats, head_dim, heads_q, seq_q;
+  int splits, head_dim, heads_q, seq_q;
   int64_t total_rows;
   __nv_bfloat16* out;
   int64_t out_batch, out_seq, out_head;
   float* lse;
 };
+constexpr int kMostSplits = 512;
 
 template <int DP>
-__global__ void __launch_bounds__(128) attention_combine_kernel(const AttnCombine p) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (row >= p.total_rows) return;
+__global__ void __launch_bounds__(128) attention_combine_kernel(const __grid_constant__ AttnCombine p) {
+  constexpr int kQuads = DP / 4, kLanes = 128 / kQuads;
+  __shared__ float weight[kMostSplits];
+  __shared__ float warp_top[4], warp_sum[4];
+  __shared__ float4 shared_acc[kLanes][kQuads];
+  const int64_t row = blockIdx.x;
+  const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32;
+  grid_dep_wait();  // the partial results are there
   float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.partial_lse[s * p.total_rows + row]);
+  for (int s = thread; s < p.splits; s += 128) {
+    const float l = p.partial_lse[s * p.total_rows + row];
+    weight[s] = l;
+    top = fmaxf(top, l);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  constexpr int kEach = DP / 32;
-  float acc[kEach] = {}, sum = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float l = p.partial_lse[s * p.total_rows + row];
-    const float weight = l == -INFINITY ? 0.0f : exp2_sfu(l - top);
-    if (l == -INFINITY) continue;
-    sum += weight;
-    const float* src = p.partial_out + (s * p.total_rows + row) * DP + lane * kEach;
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+  float sum = 0.0f;
+  for (int s = thread; s < p.splits; s += 128) {
+    const float l = weight[s];
+    weight[s] = l == -INFINITY ? 0.0f : exp2_sfu(l - top);
+    sum += weight[s];
+  }
 #pragma unroll
-    for (int x = 0; x < kEach; ++x) acc[x] += weight * src[x];
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) warp_sum[warp] = sum;
+  __syncthreads();
+  sum = (warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]);
+  const int quad = thread % kQuads, part = thread / kQuads;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const float4* src = reinterpret_cast<const float4*>(p.partial_out + row * DP) + quad;
+#pragma unroll 4
+  for (int s = part; s < p.splits; s += kLanes) {
+    const float w = weight[s];
+    if (w == 0.0f) continue;  // such a split may have written nothing
+    const float4 v = src[s * p.total_rows * kQuads];
+    acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+  }
+  shared_acc[part][quad] = acc;
+  __syncthreads();
+  if (part != 0 || quad * 4 >= p.head_dim) return;
+#pragma unroll
+  for (int i = 1; i < kLanes; ++i) {
+    const float4 v = shared_acc[i][quad];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
   }
   const int seq = static_cast<int>(row % p.seq_q);
   const int64_t bh = row / p.seq_q;
-  if (lane == 0 && p.lse != nullptr)
-    p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
   __nv_bfloat16* out = p.out + (bh / p.heads_q) * p.out_batch + seq * p.out_seq + (bh % p.heads_q) * p.out_head;
-#pragma unroll
-  for (int x = 0; x < kEach; x += 2) {
-    const int d = lane * kEach + x;
-    if (d < p.head_dim) *reinterpret_cast<uint32_t*>(out + d) = pack_bf16(acc[x] * scale, acc[x + 1] * scale);
-  }
+  *reinterpret_cast<uint2*>(out + quad * 4) =
+      make_uint2(pack_bf16(acc.x * scale, acc.y * scale), pack_bf16(acc.z * scale, acc.w * scale));
+  if (quad == 0 && p.lse != nullptr) p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace mup
