@@ -123,7 +123,7 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenStep * kTokenWarps));
   const int64_t fill = std::max<int64_t>(1, kTokenCtas * kSms / places);
   TokenPlan t{};
-  if (most <= 2 * kTokenCluster) {  // short: the latency of a second kernel would be felt
+  if (most <= 4 * kTokenCluster) {  // short: a second launch would cost more than it gains
     t.splits = static_cast<int>(std::min<int64_t>({most, fill, kTokenCluster}));
     t.cluster = t.splits > 1;
     return t;

@@ -173,6 +173,25 @@ __device__ __forceinline__ float exp2_sfu(float x) {
   return y;
 }
 
+// The largest of three (a NaN only where all are).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// The largest of 32 scores, in four chains.
+__device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
+  float m[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    m[b] = max3(__uint_as_float(v[b * 8]), __uint_as_float(v[b * 8 + 1]), __uint_as_float(v[b * 8 + 2]));
+    m[b] = max3(m[b], __uint_as_float(v[b * 8 + 3]), __uint_as_float(v[b * 8 + 4]));
+    m[b] = max3(m[b], __uint_as_float(v[b * 8 + 5]), __uint_as_float(v[b * 8 + 6]));
+    m[b] = fmaxf(m[b], __uint_as_float(v[b * 8 + 7]));
+  }
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
 // Two FP32 lanes in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -242,13 +261,13 @@ __device__ __forceinline__ void umma_rows_by_rows(uint32_t d_tmem, uint32_t a_sm
 
 // D[128 x DP] (+)= A[128 x 128, TMEM] B[128 x DP], B's rows being the summed index. The A columns of K step kk start
 // at kk / 4 * half_stride + kk % 4 * 8 (half_stride 32: packed without a gap).
-template <int DP>
+template <int DP, int BEGIN = 0, int END = 8>
 __device__ __forceinline__ void umma_tmem_by_cols(uint32_t d_tmem, uint32_t a_tmem, int half_stride, uint32_t b_smem,
                                                   bool accumulate) {
   constexpr uint32_t idesc = make_idesc_bf16(kTileRows, DP) | kIdescTransposeB;
   const uint64_t b = make_mnmajor_sw128_desc(b_smem, kPanelBytes);
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
+  for (int kk = BEGIN; kk < END; ++kk)
     umma_bf16_ts(d_tmem, a_tmem + (kk >> 2) * half_stride + (kk & 3) * 8, b + static_cast<uint64_t>((kk * 2048) >> 4),
                  idesc, accumulate || kk != 0);
 }

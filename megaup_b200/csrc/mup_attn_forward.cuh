@@ -36,8 +36,8 @@ struct AttnForwardConfig {
   static constexpr int kOffQ = 0;
   static constexpr int kOffStages = 2 * kTileBytes;
   static constexpr int kOffBars = kOffStages + kStages * kTileBytes;
-  // q full [2], stage full, stage empty, s full [2], p full [2], o done [2], drain
-  static constexpr int kBars = 2 + 2 * kStages + 6 + 1;
+  // q full [2], stage full, stage empty, s full [2], half of p full [2][2], done [2], drain [2]
+  static constexpr int kBars = 2 + 2 * kStages + 8 + 2;
   static constexpr int kOffWords = kOffBars + kBars * 8;
   static constexpr int kSmemBytes = kOffWords + 16;
   static constexpr int kThreads = 384;
@@ -114,9 +114,9 @@ __global__ void __launch_bounds__(384, 1)
   const auto full = [&](int s) { return bar(2 + s); };
   const auto empty = [&](int s) { return bar(2 + Cfg::kStages + s); };
   const auto s_full = [&](int t) { return bar(2 + 2 * Cfg::kStages + t); };
-  const auto p_full = [&](int t) { return bar(4 + 2 * Cfg::kStages + t); };
-  const auto o_done = [&](int t) { return bar(6 + 2 * Cfg::kStages + t); };
-  const uint32_t drain = bar(8 + 2 * Cfg::kStages);
+  const auto p_full = [&](int t, int half) { return bar(4 + 2 * Cfg::kStages + 2 * t + half); };
+  const auto done = [&](int t) { return bar(8 + 2 * Cfg::kStages + t); };
+  const auto drain = [&](int t) { return bar(10 + 2 * Cfg::kStages + t); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
@@ -124,18 +124,20 @@ __global__ void __launch_bounds__(384, 1)
   grid_dep_launch();
   if (threadIdx.x == 0) {
     *abort_flag = 0u;
+    const int users = ForwardBlock(p).exists(p, 1) ? 2 : 1;  // warps that read a stage
     mbar_init(q_full(0), 1);
     mbar_init(q_full(1), 1);
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), users);
     }
     for (int t = 0; t < 2; ++t) {
+      mbar_init(drain(t), 1);
       mbar_init(s_full(t), 1);
-      mbar_init(p_full(t), 128);
-      mbar_init(o_done(t), 1);
+      mbar_init(p_full(t, 0), 128);
+      mbar_init(p_full(t, 1), 128);
+      mbar_init(done(t), 1);
     }
-    mbar_init(drain, 1);
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -196,73 +198,73 @@ __global__ void __launch_bounds__(384, 1)
         for (int n = max(0, loads - Cfg::kStages); n < loads; ++n)
           drain_barrier(full(n % Cfg::kStages), (n / Cfg::kStages) & 1);
       }
-    } else if (warp == 9) {
+    } else if (warp == 9 || (warp == 10 && ForwardBlock(p).exists(p, 1))) {
       // ------------------------------------------------------------ products
+      // One warp per sub-tile: the issue of a product waits for room in the tensor pipe's short queue, so with one
+      // warp for both every barrier between two issues left the pipe empty.
+      const int t = warp - 9;
       const bool leader = elect_one_sync();
       const ForwardBlock block(p);
-      const TileList all = block.all(p);
-      const TileList own[2] = {block.tiles(p, 0), block.tiles(p, 1)};
-      const bool exists[2] = {block.exists(p, 0), block.exists(p, 1)};
+      const TileList all = block.all(p), mine = block.tiles(p, t);
+      const bool exists = block.exists(p, t);
       int begin, end;
       block.share(p, all.count, begin, end);
-      int loads = 0, steps[2] = {0, 0};
-      bool ok = true, pending[2] = {false, false};
-      for (int i = begin; ok && begin < end && i <= end; ++i) {
+      const uint32_t s_tmem = tmem + t * kTileRows, o_tmem = tmem + Cfg::kTmemO + t * DP;
+      const uint32_t q_tile = base + Cfg::kOffQ + t * Cfg::kTileBytes;
+      int loads = 0, steps = 0;
+      bool ok = true, pending = false;
+      for (int i = begin; begin < end && i <= end; ++i) {
+        // the copies of step i: K of tile i, then V of the tile before it
         const int k_load = loads, v_load = i < end ? loads + 1 : loads;
         const int ks = k_load % Cfg::kStages, vs = v_load % Cfg::kStages;
-        const uint32_t k_tile = base + Cfg::kOffStages + ks * Cfg::kTileBytes;
-        const uint32_t v_tile = base + Cfg::kOffStages + vs * Cfg::kTileBytes;
-        bool k_there = false, v_there = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t s_tmem = tmem + t * kTileRows;
-          if (i > begin && pending[t]) {
-            ok = ok && ctl.wait(p_full(t), (steps[t] - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
-            if (ok && !v_there) {
-              ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
-              v_there = true;
-              if (ok)
-                zero_unseen_rows<DP>(smem + Cfg::kOffStages + vs * Cfg::kTileBytes, all, all.tile(i - 1) * kTileRows,
-                                     lane);
-            }
+        loads += (i < end) + (i > begin);
+        if (i > begin) {
+          const uint32_t v_tile = base + Cfg::kOffStages + vs * Cfg::kTileBytes;
+          ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+          if (ok && pending) {
+            // (both warps clear the same rows: whichever comes second writes the zeros that are there)
+            zero_unseen_rows<DP>(smem + Cfg::kOffStages + vs * Cfg::kTileBytes, all, all.tile(i - 1) * kTileRows, lane);
+            ok = ctl.wait(p_full(t, 0), (steps - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
+            if (!ok) break;
+            tc_fence_after_sync();
+            // the first 64 keys while the softmax warps are at the others
+            if (leader) umma_tmem_by_cols<DP, 0, 4>(o_tmem, s_tmem, 32, v_tile, steps > 1);
+            ok = ctl.wait(p_full(t, 1), (steps - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
             if (!ok) break;
             tc_fence_after_sync();
             if (leader) {
-              umma_tmem_by_cols<DP>(tmem + Cfg::kTmemO + t * DP, s_tmem, 32, v_tile, steps[t] > 1);
-              umma_commit_1(o_done(t));
+              umma_tmem_by_cols<DP, 4, 8>(o_tmem, s_tmem, 32, v_tile, true);
+              umma_commit_1(done(t));
+              umma_commit_1(empty(vs));
             }
-            pending[t] = false;
+            pending = false;
+          } else if (ok && leader) {
+            mbar_arrive(empty(vs));
           }
-          if (i < end && exists[t] && sees_tile(own[t], all.tile(i))) {
-            if (steps[t] == 0) ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
-            if (ok && !k_there) {
-              ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
-              k_there = true;
-            }
+        }
+        if (ok && i < end) {
+          ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+          if (ok && exists && sees_tile(mine, all.tile(i))) {
+            if (steps == 0) ok = ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
             if (!ok) break;
             tc_fence_after_sync();
             if (leader) {
-              umma_rows_by_rows<DP>(s_tmem, base + Cfg::kOffQ + t * Cfg::kTileBytes, k_tile);
+              umma_rows_by_rows<DP>(s_tmem, q_tile, base + Cfg::kOffStages + ks * Cfg::kTileBytes);
               umma_commit_1(s_full(t));
+              umma_commit_1(empty(ks));
             }
-            pending[t] = true;
-            ++steps[t];
+            pending = true;
+            ++steps;
+          } else if (ok && leader) {
+            mbar_arrive(empty(ks));
           }
         }
         if (!ok) break;
-        // tiles that neither sub-tile used are waited for all the same: their stage is refilled next
-        if (i < end && !k_there) ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
-        if (ok && i > begin && !v_there) ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
-        if (ok && leader) {
-          if (i < end) umma_commit_1(empty(ks));
-          if (i > begin) umma_commit_1(empty(vs));
-        }
-        loads += (i < end) + (i > begin);
       }
       if (!ok) {
-        if (leader) umma_commit_1(drain);
+        if (leader) umma_commit_1(drain(t));
         __syncwarp();
-        drain_barrier(drain, 0);
+        drain_barrier(drain(t), 0);
       }
     }
   } else {
@@ -303,15 +305,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int b = 0; b < 4; ++b) hide_scores(raw[b], span_bits(low - b * 32, high - b * 32, sink - b * 32));
       }
-      float m4[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float m = __uint_as_float(raw[b][0]);
-#pragma unroll
-        for (int x = 1; x < 32; ++x) m = fmaxf(m, __uint_as_float(raw[b][x]));
-        m4[b] = m;
-      }
-      const float seen_top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      const float seen_top = fmaxf(max3(max32(raw[0]), max32(raw[1]), max32(raw[2])), max32(raw[3]));
       // the reference of the exponents: kept while the maximum grows little
       float factor = 1.0f;
       bool rescale = false;
@@ -323,12 +317,7 @@ __global__ void __launch_bounds__(384, 1)
         rescale = true;
       }
       if (__any_sync(0xffffffffu, rescale)) {
-        // all products into O so far have ended
-        if (!ctl.wait(o_done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
+        // S of this step was issued behind the last product into O: that has ended as well
         sum *= factor;
 #pragma unroll 1
         for (int b = 0; b < DP / 16; ++b) {
@@ -355,14 +344,17 @@ __global__ void __launch_bounds__(384, 1)
           packed[x] = pack_bf16(e.x, e.y);
         }
         tmem_st_32x16(s_tmem + b * 16, packed);
+        if (b & 1) {
+          tmem_st_wait();
+          tc_fence_before_sync();
+          mbar_arrive(p_full(t, b >> 1));
+        }
       }
       sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-      tmem_st_wait();
-      tc_fence_before_sync();
-      mbar_arrive(p_full(t));
       ++steps;
     }
-    if (ok && steps > 0) ok = ctl.wait(o_done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT);
+    // (the phases before the last one have ended with their successors' S)
+    if (ok && steps > 0) ok = ctl.wait(done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT);
     // ---- O / sum, rounded once
     if (ok) {
       tc_fence_after_sync();
