@@ -211,25 +211,39 @@ __global__ void __launch_bounds__(384, 1)
       block.share(p, all.count, begin, end);
       const uint32_t s_tmem = tmem + t * kTileRows, o_tmem = tmem + Cfg::kTmemO + t * DP;
       const uint32_t q_tile = base + Cfg::kOffQ + t * Cfg::kTileBytes;
-      int loads = 0, steps = 0;
+      int stage = 0, steps = 0;  // the ring's next stage and its phase
+      uint32_t phase = 0;
+      const auto advance = [&] {
+        if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+      };
       bool ok = true, pending = false;
       for (int i = begin; begin < end && i <= end; ++i) {
-        // the copies of step i: K of tile i, then V of the tile before it
-        const int k_load = loads, v_load = i < end ? loads + 1 : loads;
-        const int ks = k_load % Cfg::kStages, vs = v_load % Cfg::kStages;
-        loads += (i < end) + (i > begin);
-        if (i > begin) {
+        // Step i: K of tile i arrives, then V of the tile before it. Everything that does not depend on the softmax
+        // warps comes before the waits for them, so that the products follow each other without a pause.
+        bool active = false;
+        int ks = 0;
+        if (i < end) {
+          ks = stage;
+          ok = ctl.wait(full(ks), phase, MUP_ST_MMA_FULL_TIMEOUT);
+          advance();
+          active = exists && sees_tile(mine, all.tile(i));
+          if (active && steps == 0) ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
+        }
+        if (ok && i > begin) {
+          const int vs = stage;
           const uint32_t v_tile = base + Cfg::kOffStages + vs * Cfg::kTileBytes;
-          ok = ctl.wait(full(vs), (v_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
+          ok = ctl.wait(full(vs), phase, MUP_ST_MMA_FULL_TIMEOUT);
+          advance();
           if (ok && pending) {
             // (both warps clear the same rows: whichever comes second writes the zeros that are there)
             zero_unseen_rows<DP>(smem + Cfg::kOffStages + vs * Cfg::kTileBytes, all, all.tile(i - 1) * kTileRows, lane);
-            ok = ctl.wait(p_full(t, 0), (steps - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
+            const uint32_t parity = (steps - 1) & 1;
+            ok = ctl.wait(p_full(t, 0), parity, MUP_ST_MMA_ACC_TIMEOUT);
             if (!ok) break;
             tc_fence_after_sync();
             // the first 64 keys while the softmax warps are at the others
             if (leader) umma_tmem_by_cols<DP, 0, 4>(o_tmem, s_tmem, 32, v_tile, steps > 1);
-            ok = ctl.wait(p_full(t, 1), (steps - 1) & 1, MUP_ST_MMA_ACC_TIMEOUT);
+            ok = ctl.wait(p_full(t, 1), parity, MUP_ST_MMA_ACC_TIMEOUT);
             if (!ok) break;
             tc_fence_after_sync();
             if (leader) {
@@ -237,29 +251,23 @@ __global__ void __launch_bounds__(384, 1)
               umma_commit_1(done(t));
               umma_commit_1(empty(vs));
             }
-            pending = false;
           } else if (ok && leader) {
             mbar_arrive(empty(vs));
           }
         }
-        if (ok && i < end) {
-          ok = ctl.wait(full(ks), (k_load / Cfg::kStages) & 1, MUP_ST_MMA_FULL_TIMEOUT);
-          if (ok && exists && sees_tile(mine, all.tile(i))) {
-            if (steps == 0) ok = ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
-            if (!ok) break;
-            tc_fence_after_sync();
-            if (leader) {
-              umma_rows_by_rows<DP>(s_tmem, q_tile, base + Cfg::kOffStages + ks * Cfg::kTileBytes);
-              umma_commit_1(s_full(t));
-              umma_commit_1(empty(ks));
-            }
-            pending = true;
-            ++steps;
-          } else if (ok && leader) {
-            mbar_arrive(empty(ks));
-          }
-        }
         if (!ok) break;
+        pending = active;
+        if (active) {
+          tc_fence_after_sync();
+          if (leader) {
+            umma_rows_by_rows<DP>(s_tmem, q_tile, base + Cfg::kOffStages + ks * Cfg::kTileBytes);
+            umma_commit_1(s_full(t));
+            umma_commit_1(empty(ks));
+          }
+          ++steps;
+        } else if (i < end && leader) {
+          mbar_arrive(empty(ks));
+        }
       }
       if (!ok) {
         if (leader) umma_commit_1(drain(t));
