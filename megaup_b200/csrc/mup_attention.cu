@@ -29,6 +29,8 @@ int check_problem(const mup_window_attention* args) {
     return host_fail(MUP_ERR_BAD_ARG, "window attention: batch %d, heads %d / %d", a.batch, a.heads_q, a.heads_kv);
   if (a.seq_q < 1 || a.seq_k < 1 || a.seq_q > kMaxLength || a.seq_k > kMaxLength)
     return host_fail(MUP_ERR_BAD_ARG, "window attention: %d queries and %d keys (1 .. %d)", a.seq_q, a.seq_k, kMaxLength);
+  if (total_rows(a) > 0x7fffffff)
+    return host_fail(MUP_ERR_UNSUPPORTED, "window attention: %d x %d x %d rows", a.batch, a.heads_q, a.seq_q);
   if (a.sinks < 0 || !(a.scale > 0.0f) || a.scale > 1e30f)
     return host_fail(MUP_ERR_BAD_ARG, "window attention: sinks %d, scale %g", a.sinks, static_cast<double>(a.scale));
   if (a.sequences != nullptr) {
@@ -167,6 +169,21 @@ int encode_rows(CUtensorMap* map, const mup_window_attention& a, const void* bas
   return encode_map_4d(map, base, dims, order, box);
 }
 
+// A launch that may begin while the CTAs of the kernel before it run; the kernel waits for that one's end itself
+// (grid_dep_wait) before it touches its results.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), int64_t blocks, int threads, int smem, cudaStream_t stream,
+                         const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks)), config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem), config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute, config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 template <int DP>
 int launch_combine(const mup_window_attention& a, const float* partial_out, const float* partial_lse, int splits,
                    cudaStream_t stream) {
@@ -175,14 +192,7 @@ int launch_combine(const mup_window_attention& a, const float* partial_out, cons
   c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = total_rows(a);
   c.out = static_cast<__nv_bfloat16*>(a.out);
   c.out_batch = a.out_strides[0], c.out_seq = a.out_strides[1], c.out_head = a.out_strides[2], c.lse = a.lse;
-  // launched while the CTAs before it run (it waits for them on the GPU)
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(c.total_rows)), config.blockDim = dim3(128), config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute, config.numAttrs = 1;
-  MUP_HOST_CUDA(cudaLaunchKernelEx(&config, attention_combine_kernel<DP>, c));
+  MUP_HOST_CUDA(launch_early(attention_combine_kernel<DP>, c.total_rows, 128, 0, stream, c));
   return MUP_OK;
 }
 
@@ -334,25 +344,18 @@ int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t
   const int64_t shared_jobs = static_cast<int64_t>(p.n_sequences) * a.heads_kv * plan.shared_tiles * plan.shares;
   const int64_t k_grid = shared_jobs + static_cast<int64_t>(a.heads_kv) *
                                            (packed ? p.n_k_blocks : a.batch * (p.n_k_blocks - plan.shared_tiles));
-  if (std::max(q_grid, k_grid) > 0x7fffffff || total_rows(a) / 16 > 0x7fffffff)
+  if (q_grid + k_grid > 0x7fffffff)
     return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many row blocks");
-  using DqCfg = AttnDqConfig<DP>;
-  using DkvCfg = AttnDkvConfig<DP>;
-  static uint64_t dq_ready = 0, dkv_ready = 0;
-  MUP_HOST_CUDA(allow_smem_once(attention_dq_kernel<DP>, DqCfg::kSmemBytes, a.device, &dq_ready));
-  MUP_HOST_CUDA(allow_smem_once(attention_dkv_kernel<DP>, DkvCfg::kSmemBytes, a.device, &dkv_ready));
-  attention_delta_kernel<<<ceil_div(total_rows(a), 16), 256, 0, stream>>>(d);
+  const int smem = AttnBackwardConfig<DP>::kSmemBytes;
+  static uint64_t ready = 0;
+  MUP_HOST_CUDA(allow_smem_once(attention_backward_kernel<DP>, smem, a.device, &ready));
+  p.dkv_jobs = static_cast<int>(k_grid);
+  attention_delta_kernel<<<ceil_div(total_rows(a), 16 * kDeltaRows), 256, 0, stream>>>(d);
   MUP_HOST_CUDA(cudaGetLastError());
-  attention_dq_kernel<DP><<<static_cast<unsigned>(q_grid), 384, DqCfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map, do_map);
-  MUP_HOST_CUDA(cudaGetLastError());
-  if (k_grid > 0) {
-    attention_dkv_kernel<DP><<<static_cast<unsigned>(k_grid), 384, DkvCfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map, do_map);
-    MUP_HOST_CUDA(cudaGetLastError());
-  }
+  MUP_HOST_CUDA(launch_early(attention_backward_kernel<DP>, k_grid + q_grid, 384, smem, stream, p, q_map, k_map, v_map, do_map));
   if (plan.shared_tiles > 0) {
     const int64_t quads = static_cast<int64_t>(p.n_sequences) * a.heads_kv * plan.shared_tiles * 2 * kTileRows * (DP / 4);
-    attention_dkv_join_kernel<DP><<<ceil_div(quads, 256), 256, 0, stream>>>(p);
-    MUP_HOST_CUDA(cudaGetLastError());
+    MUP_HOST_CUDA(launch_early(attention_dkv_join_kernel<DP>, ceil_div(quads, 256), 256, 0, stream, p));
   }
   return MUP_OK;
 }

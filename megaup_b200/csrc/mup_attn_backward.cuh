@@ -17,6 +17,7 @@ struct AttnBackward {
   const int2* k_blocks;  // packed: the same of the key rows
   int n_q_blocks, n_k_blocks;  // packed: of the lists; dense: per sequence
   int n_sequences;
+  int dkv_jobs;  // CTAs of dK and dV
   // The first `shared_tiles` key tiles of every sequence are each computed by `shares` CTAs.
   int shared_tiles, shares;
   const float* lse2;   // [batch, heads, rows], base 2; +inf where a row sees nothing
@@ -44,31 +45,39 @@ __device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float sum) {
   return fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), sum);
 }
 
-__global__ void __launch_bounds__(256) attention_delta_kernel(const AttnDelta p) {
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 16;
-  const int part = threadIdx.x % 16;
-  // neighbouring half-warps take the heads of one row: their rows lie next to each other
-  const int64_t per_batch = static_cast<int64_t>(p.heads_q) * p.seq_q;
-  const int64_t b = item / per_batch;
-  const int64_t rest = item - b * per_batch;
-  const int64_t row = rest / p.heads_q;
-  const int head = static_cast<int>(rest - row * p.heads_q);
-  float sum = 0.0f;
-  if (item < p.total_rows && part * 8 < p.head_dim) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p.out + b * p.out_batch + row * p.out_seq + head * p.out_head + part * 8);
-    const uint4 y = *reinterpret_cast<const uint4*>(p.dout + b * p.dout_batch + row * p.dout_seq + head * p.dout_head + part * 8);
-    sum = dot_bf16x2(x.x, y.x, sum);
-    sum = dot_bf16x2(x.y, y.y, sum);
-    sum = dot_bf16x2(x.z, y.z, sum);
-    sum = dot_bf16x2(x.w, y.w, sum);
-  }
+constexpr int kDeltaRows = 4;  // of 16 lanes: all their loads are in flight at once; a warp's 8 rows follow each other
+
+__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ AttnDelta p) {
+  grid_dep_launch();
+  const int lane = threadIdx.x % 32, part = lane % 16;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * 2 * kDeltaRows;
+  uint4 x[kDeltaRows], y[kDeltaRows];
 #pragma unroll
-  for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (item < p.total_rows && part == 0) {
-    const int64_t index = (b * p.heads_q + head) * p.seq_q + row;
-    const float l = p.lse[index];
-    p.delta[index] = sum;
-    p.lse2[index] = l == -INFINITY ? INFINITY : l * kLog2e;
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const int64_t item = first + i * 2 + lane / 16;
+    x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    if (item >= p.total_rows || part * 8 >= p.head_dim) continue;
+    const uint32_t bh = static_cast<uint32_t>(item) / p.seq_q, row = static_cast<uint32_t>(item) - bh * p.seq_q;
+    const uint32_t b = bh / p.heads_q, head = bh - b * p.heads_q;
+    x[i] = ld_stream_v4(p.out + b * p.out_batch + row * p.out_seq + head * p.out_head + part * 8);
+    y[i] = ld_stream_v4(p.dout + b * p.dout_batch + row * p.dout_seq + head * p.dout_head + part * 8);
+  }
+  float mine = 0.0f;  // of row `first + lane`, in the first eight lanes
+#pragma unroll
+  for (int i = 0; i < kDeltaRows; ++i) {
+    float sum = dot_bf16x2(x[i].x, y[i].x, 0.0f);
+    sum = dot_bf16x2(x[i].y, y[i].y, sum);
+    sum = dot_bf16x2(x[i].z, y[i].z, sum);
+    sum = dot_bf16x2(x[i].w, y[i].w, sum);
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float there = __shfl_sync(0xffffffffu, sum, lane % 2 * 16);
+    if (lane / 2 == i) mine = there;
+  }
+  if (lane < 2 * kDeltaRows && first + lane < p.total_rows) {
+    const float l = p.lse[first + lane];
+    p.delta[first + lane] = mine;
+    p.lse2[first + lane] = l == -INFINITY ? INFINITY : l * kLog2e;
   }
 }
 
@@ -92,12 +101,10 @@ struct AttnDqConfig {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(384, 1)
-    attention_dq_kernel(const __grid_constant__ AttnBackward p, const __grid_constant__ CUtensorMap q_map,
-                        const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                        const __grid_constant__ CUtensorMap do_map) {
+__device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtensorMap& q_map, const CUtensorMap& k_map,
+                                             const CUtensorMap& v_map, const CUtensorMap& do_map, uint8_t* smem,
+                                             int job) {
   using Cfg = AttnDqConfig<DP>;
-  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   auto bar = [&](int i) { return base + Cfg::kOffBars + i * 8; };
@@ -114,8 +121,8 @@ __global__ void __launch_bounds__(384, 1)
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
-  const int head = blockIdx.x % p.shape.heads_q;
-  const int w = blockIdx.x / p.shape.heads_q;
+  const int head = job % p.shape.heads_q;
+  const int w = job / p.shape.heads_q;
   int sequence, row0;
   if (p.q_blocks != nullptr) {
     const int2 block = p.q_blocks[w];
@@ -240,6 +247,7 @@ __global__ void __launch_bounds__(384, 1)
     const RowSpan span = row_span(p.shape, seq, row);
     const int64_t index = (static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + seq.q0 + row;
     const float c = p.shape.scale_log2;
+    grid_dep_wait();
     const float shift = valid ? -p.lse2[index] : -INFINITY;
     const float delta = valid ? p.delta[index] : 0.0f;
     const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift), delta2 = make_float2(-delta, -delta);
@@ -300,30 +308,27 @@ __global__ void __launch_bounds__(384, 1)
     if (ok && n > 0) ok = ctl.wait(done, 0, MUP_ST_EPILOGUE_TIMEOUT);
     if (ok) {
       tc_fence_after_sync();
-      __nv_bfloat16* dst = p.dq + batch * p.dq_batch + (seq.q0 + row) * p.dq_seq + head * p.dq_head;
+      // both warpgroups' columns of a row are written in halves of a row, through Q's place (no product reads it now)
+      uint8_t* staged = smem + Cfg::kOffQ + half * (kTileRows * DP);
+      const int r = quarter * 32 + lane;
 #pragma unroll 1
       for (int b = 0; b < DP / 64; ++b) {
-        const int col = half * (DP / 2) + b * 32;
         uint32_t g[32];
         if (n > 0) {
-          tmem_ld_32x32(tmem + Cfg::kTmemDq + col + lane_base, g);
+          tmem_ld_32x32(tmem + Cfg::kTmemDq + half * (DP / 2) + b * 32 + lane_base, g);
           tmem_ld_wait();
         } else {
 #pragma unroll
           for (int x = 0; x < 32; ++x) g[x] = 0u;
         }
-        if (!valid) continue;
 #pragma unroll
-        for (int x = 0; x < 32; x += 8) {
-          if (col + x >= p.shape.head_dim) break;
-          uint4 v;
-          uint32_t* words = &v.x;
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            words[y] = pack_bf16(__uint_as_float(g[x + 2 * y]) * p.shape.scale, __uint_as_float(g[x + 2 * y + 1]) * p.shape.scale);
-          *reinterpret_cast<uint4*>(dst + col + x) = v;
-        }
+        for (int x = 0; x < 32; x += 8) *staged_piece<DP>(staged, r, b * 4 + x / 8) = pack_bf16x8(g + x, p.shape.scale);
       }
+      write_staged_rows<DP>(staged, quarter * 32, lane, p.shape.head_dim * 2 - half * DP, [&](int x) {
+        return row0 + x >= seq.nq ? nullptr
+                                  : reinterpret_cast<uint8_t*>(p.dq + batch * p.dq_batch + (seq.q0 + row0 + x) * p.dq_seq +
+                                                               head * p.dq_head + half * (DP / 2));
+      });
     }
     tc_fence_before_sync();
   }
@@ -355,12 +360,10 @@ struct AttnDkvConfig {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(384, 1)
-    attention_dkv_kernel(const __grid_constant__ AttnBackward p, const __grid_constant__ CUtensorMap q_map,
-                         const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                         const __grid_constant__ CUtensorMap do_map) {
+__device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUtensorMap& q_map, const CUtensorMap& k_map,
+                                              const CUtensorMap& v_map, const CUtensorMap& do_map, uint8_t* smem,
+                                              int job) {
   using Cfg = AttnDkvConfig<DP>;
-  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   auto bar = [&](int i) { return base + Cfg::kOffBars + i * 8; };
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(384, 1)
   // ---- the key tile, and this CTA's share of the query tiles that see it
   const int heads_kv = p.shape.heads_kv, group = p.shape.heads_q / heads_kv;
   const int shared_jobs = p.n_sequences * heads_kv * p.shared_tiles * p.shares;
-  int job = blockIdx.x, sequence, tile, kv_head, share = 0, shares = 1;
+  int sequence, tile, kv_head, share = 0, shares = 1;
   if (job < shared_jobs) {
     share = job % p.shares, shares = p.shares;
     job /= p.shares;
@@ -477,6 +480,7 @@ __global__ void __launch_bounds__(384, 1)
       }
     } else if (warp == 10) {
       // ------------------------------------------- lse and delta of the query rows
+      grid_dep_wait();
       for (int i = 0; i < n; ++i) {
         const int st = i % Cfg::kStatStages;
         const int head = kv_head * group + (begin + i) / q_tiles;
@@ -652,13 +656,12 @@ __global__ void __launch_bounds__(384, 1)
       // one warpgroup writes dV, the other dK
       const float scale = half == 0 ? 1.0f : p.shape.scale;
       const uint32_t src = tmem + (half == 0 ? Cfg::kTmemDv : Cfg::kTmemDk) + lane_base;
-      __nv_bfloat16* dst = half == 0 ? p.dv + batch * p.dv_batch + (seq.k0 + j) * p.dv_seq + kv_head * p.dv_head
-                                     : p.dk + batch * p.dk_batch + (seq.k0 + j) * p.dk_seq + kv_head * p.dk_head;
       const int64_t slot = ((static_cast<int64_t>(sequence) * heads_kv + kv_head) * p.shared_tiles + tile) * shares + share;
-      float* partial = p.partial + ((slot * 2 + half) * kTileRows + quarter * 32 + lane) * DP;
-#pragma unroll 1
-      for (int b = 0; b < DP / 32; ++b) {
-        uint32_t g[32];
+      // through V's and K's places: no product reads them now
+      uint8_t* staged = smem + (half == 0 ? Cfg::kOffV : Cfg::kOffK);
+      constexpr int kRowBytes = DP * 2;
+      const int r = quarter * 32 + lane;
+      const auto load_sum = [&](int b, uint32_t(&g)[32]) {
         if (n > 0) {
           tmem_ld_32x32(src + b * 32, g);
           tmem_ld_wait();
@@ -666,23 +669,36 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int x = 0; x < 32; ++x) g[x] = 0u;
         }
-        if (j >= seq.nk) continue;
+      };
+      if (shares > 1) {  // half of the FP32 columns at a time
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+#pragma unroll 1
+          for (int b = 0; b < DP / 64; ++b) {
+            uint32_t g[32];
+            load_sum(part * (DP / 64) + b, g);
 #pragma unroll
-        for (int x = 0; x < 32; x += 8) {
-          if (b * 32 + x >= p.shape.head_dim) break;
-          if (shares > 1) {
-            uint4* to = reinterpret_cast<uint4*>(partial + b * 32 + x);
-            to[0] = make_uint4(g[x], g[x + 1], g[x + 2], g[x + 3]);
-            to[1] = make_uint4(g[x + 4], g[x + 5], g[x + 6], g[x + 7]);
-          } else {
-            uint4 v;
-            uint32_t* words = &v.x;
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              words[y] = pack_bf16(__uint_as_float(g[x + 2 * y]) * scale, __uint_as_float(g[x + 2 * y + 1]) * scale);
-            *reinterpret_cast<uint4*>(dst + b * 32 + x) = v;
+            for (int x = 0; x < 32; x += 4)
+              *staged_piece<kRowBytes>(staged, r, b * 8 + x / 4) = make_uint4(g[x], g[x + 1], g[x + 2], g[x + 3]);
           }
+          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, kRowBytes, [&](int x) {
+            return reinterpret_cast<uint8_t*>(p.partial + ((slot * 2 + half) * kTileRows + x) * DP + part * (DP / 2));
+          });
         }
+      } else {
+#pragma unroll 1
+        for (int b = 0; b < DP / 32; ++b) {
+          uint32_t g[32];
+          load_sum(b, g);
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) *staged_piece<kRowBytes>(staged, r, b * 4 + x / 8) = pack_bf16x8(g + x, scale);
+        }
+        write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
+          if (j0 + x >= seq.nk) return static_cast<uint8_t*>(nullptr);
+          return reinterpret_cast<uint8_t*>(
+              half == 0 ? p.dv + batch * p.dv_batch + (seq.k0 + j0 + x) * p.dv_seq + kv_head * p.dv_head
+                        : p.dk + batch * p.dk_batch + (seq.k0 + j0 + x) * p.dk_seq + kv_head * p.dk_head);
+        });
       }
     }
     tc_fence_before_sync();
@@ -694,10 +710,34 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
+// Both in one launch, the CTAs of dK and dV (the longer ones) first: neither needs the other, and small problems fill the
+// GPU better together. Launched while the delta kernel runs; the warps that read its results wait for it.
+template <int DP>
+struct AttnBackwardConfig {
+  static constexpr int kSmemBytes = AttnDqConfig<DP>::kSmemBytes > AttnDkvConfig<DP>::kSmemBytes
+                                        ? AttnDqConfig<DP>::kSmemBytes
+                                        : AttnDkvConfig<DP>::kSmemBytes;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(384, 1)
+    attention_backward_kernel(const __grid_constant__ AttnBackward p, const __grid_constant__ CUtensorMap q_map,
+                              const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                              const __grid_constant__ CUtensorMap do_map) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  grid_dep_launch();
+  const int job = blockIdx.x;
+  if (job < p.dkv_jobs)
+    attention_dkv<DP>(p, q_map, k_map, v_map, do_map, smem, job);
+  else
+    attention_dq<DP>(p, q_map, k_map, v_map, do_map, smem, job - p.dkv_jobs);
+}
+
 // Sums the shares of the shared key tiles, always in the same order: one thread per four columns of dV or dK.
 template <int DP>
 __global__ void __launch_bounds__(256) attention_dkv_join_kernel(const __grid_constant__ AttnBackward p) {
   constexpr int kQuads = DP / 4;
+  grid_dep_wait();
   int64_t item = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
   const int quad = static_cast<int>(item % kQuads);
   item /= kQuads;

@@ -319,6 +319,37 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, 
   }
 }
 
+// Results leave through shared memory: a thread holds a row, and rows written by their threads would touch 32 lines per
+// instruction. Piece `chunk` (16 bytes) of row r of a tile with RB bytes per row, its place permuted so that neither
+// side has bank conflicts.
+template <int RB>
+__device__ __forceinline__ uint4* staged_piece(uint8_t* tile, int r, int chunk) {
+  constexpr int kMask = RB >= 128 ? 7 : RB / 16 - 1;
+  return reinterpret_cast<uint4*>(tile + r * RB + ((chunk ^ (r & kMask)) * 16));
+}
+// The warp's 32 rows, from `first`, whole rows at a time to where dst(r) points (null: nowhere), `bytes` of each.
+template <int RB, typename Dst>
+__device__ __forceinline__ void write_staged_rows(uint8_t* tile, int first, int lane, int bytes, Dst dst) {
+  constexpr int kLanes = RB / 16;
+  __syncwarp();
+#pragma unroll 4
+  for (int k = 0; k < kLanes; ++k) {
+    const int r = first + k * (32 / kLanes) + lane / kLanes, chunk = lane % kLanes;
+    const uint4 v = *staged_piece<RB>(tile, r, chunk);
+    uint8_t* to = dst(r);
+    if (to != nullptr && chunk * 16 < bytes) *reinterpret_cast<uint4*>(to + chunk * 16) = v;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ uint4 pack_bf16x8(const uint32_t* v, float scale) {
+  uint4 p;
+  p.x = pack_bf16(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale);
+  p.y = pack_bf16(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale);
+  p.z = pack_bf16(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale);
+  p.w = pack_bf16(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale);
+  return p;
+}
+
 // A row of a key or value tile that none of the block's rows sees (another sequence's, one behind the filled part of a
 // cache, one between the sinks and the window) has to be finite where its weight is 0: it becomes 0. The whole warp
 // calls this between the tile's arrival and its first product.

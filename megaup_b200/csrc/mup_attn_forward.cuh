@@ -361,56 +361,73 @@ __global__ void __launch_bounds__(384, 1)
       sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
       ++steps;
     }
-    // (the phases before the last one have ended with their successors' S)
-    if (ok && steps > 0) ok = ctl.wait(done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT);
+    // (the phases before the last one have ended with their successors' S; a sub-tile that saw nothing has no product
+    // that waited for its Q, whose place is used again below)
+    if (ok && steps > 0)
+      ok = ctl.wait(done(t), (steps - 1) & 1, MUP_ST_EPILOGUE_TIMEOUT);
+    else if (ok && exists && begin < end)
+      ok = ctl.wait(q_full(t), 0, MUP_ST_EPILOGUE_TIMEOUT);
     // ---- O / sum, rounded once
-    if (ok) {
+    if (ok && exists) {
       tc_fence_after_sync();
-      const int head = block.head0 + t * block.head_step + r / block.rows;
-      const bool valid = exists && row < block.seq.nq;
-      const int q_row = block.seq.q0 + row;
-      const int64_t index = (static_cast<int64_t>(block.batch) * p.shape.heads_q + head) * p.shape.seq_q + q_row;
-      const float log2_sum = top * c + log2f(sum);
-      const float scale = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-      if (valid) {
-        const float lse2 = sum == 0.0f ? -INFINITY : log2_sum;
+      const int head0 = block.head0 + t * block.head_step, tile_row0 = block.row0 + t * block.row_step;
+      const auto index_of = [&](int x) {  // of row x of the sub-tile
+        return (static_cast<int64_t>(block.batch) * p.shape.heads_q + head0 + x / block.rows) * p.shape.seq_q + block.seq.q0 +
+               tile_row0 + x % block.rows;
+      };
+      const auto is_row = [&](int x) { return tile_row0 + x % block.rows < block.seq.nq; };
+      const bool empty_row = sum == 0.0f;
+      if (is_row(r)) {
+        const float lse2 = empty_row ? -INFINITY : top * c + log2f(sum);
         if (p.splits > 1)
-          p.partial_lse[block.split * p.total_rows + index] = lse2;
+          p.partial_lse[block.split * p.total_rows + index_of(r)] = lse2;
         else if (p.lse != nullptr)
-          p.lse[index] = lse2 * 0.69314718055994531f;
+          p.lse[index_of(r)] = lse2 * 0.69314718055994531f;
       }
-      __nv_bfloat16* out = p.out + block.batch * p.out_batch + q_row * p.out_seq + head * p.out_head;
-      float* partial = p.partial_out + (block.split * p.total_rows + index) * DP;
-#pragma unroll 1
-      for (int b = 0; b < DP / 32; ++b) {
-        uint32_t o[32];
+      const float scale = empty_row ? 0.0f : 1.0f / sum;
+      uint8_t* staged = smem + Cfg::kOffQ + t * Cfg::kTileBytes;
+      constexpr int kRowBytes = DP * 2;
+      const auto load_o = [&](int b, uint32_t(&o)[32]) {
         if (steps > 0) {
           tmem_ld_32x32(o_tmem + b * 32, o);
           tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0u;
         }
-        if (!valid) continue;
 #pragma unroll
-        for (int x = 0; x < 32; x += 8) {
-          if (b * 32 + x >= p.shape.head_dim) break;
-          float v[8];
+        for (int x = 0; x < 32; ++x) o[x] = steps > 0 && !empty_row ? o[x] : 0u;
+      };
+      if (p.splits > 1) {  // half of the FP32 columns at a time
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+          for (int b = 0; b < DP / 64; ++b) {
+            uint32_t o[32];
+            load_o(half * (DP / 64) + b, o);
 #pragma unroll
-          for (int y = 0; y < 8; ++y) v[y] = sum == 0.0f ? 0.0f : __uint_as_float(o[x + y]) * scale;
-          if (p.splits > 1) {
-            float4* dst = reinterpret_cast<float4*>(partial + b * 32 + x);
-            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            uint4 packed;
-            packed.x = pack_bf16(v[0], v[1]);
-            packed.y = pack_bf16(v[2], v[3]);
-            packed.z = pack_bf16(v[4], v[5]);
-            packed.w = pack_bf16(v[6], v[7]);
-            *reinterpret_cast<uint4*>(out + b * 32 + x) = packed;
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(staged_piece<kRowBytes>(staged, r, b * 8 + x / 4)) =
+                  make_float4(__uint_as_float(o[x]) * scale, __uint_as_float(o[x + 1]) * scale,
+                              __uint_as_float(o[x + 2]) * scale, __uint_as_float(o[x + 3]) * scale);
           }
+          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, kRowBytes, [&](int x) {
+            return !is_row(x) ? nullptr
+                              : reinterpret_cast<uint8_t*>(p.partial_out + (block.split * p.total_rows + index_of(x)) * DP +
+                                                           half * (DP / 2));
+          });
         }
+      } else {
+#pragma unroll 1
+        for (int b = 0; b < DP / 32; ++b) {
+          uint32_t o[32];
+          load_o(b, o);
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) *staged_piece<kRowBytes>(staged, r, b * 4 + x / 8) = pack_bf16x8(o + x, scale);
+        }
+        write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
+          return !is_row(x) ? nullptr
+                            : reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
+                                                         (block.seq.q0 + tile_row0 + x % block.rows) * p.out_seq +
+                                                         (head0 + x / block.rows) * p.out_head);
+        });
       }
     }
     tc_fence_before_sync();
