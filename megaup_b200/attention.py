@@ -67,11 +67,13 @@ class PackedSequences:
         return self.sequences.device
 
 
-def _blocks(lengths: list[int], rows: int) -> list[tuple[int, int]]:
-    """(sequence, first row) of every block of ``rows`` rows, the last rows first:
-    under a causal mask they have the most keys."""
+def _blocks(table: list[tuple[int, int, int, int]], lengths: list[int], rows: int) -> list[tuple[int, ...]]:
+    """(sequence, first row, the sequence's entry of ``table``) of every block of
+    ``rows`` rows, the last rows first: under a causal mask they have the most keys."""
 
-    blocks = [(s, r) for s, length in enumerate(lengths) for r in range(0, length, rows)]
+    blocks = [
+        (s, r, *entry, 0, 0) for s, (entry, length) in enumerate(zip(table, lengths)) for r in range(0, length, rows)
+    ]
     return sorted(blocks, key=lambda block: -block[1])
 
 
@@ -105,9 +107,9 @@ def prepare_packed_sequences(
         cu_seqlens_q=cu_q,
         cu_seqlens_k=cu_k,
         sequences=on_device(table),
-        q_blocks_256=on_device(_blocks(queries, 256)),
-        q_blocks_128=on_device(_blocks(queries, 128)),
-        k_blocks_128=on_device(_blocks(keys, 128)[::-1]),
+        q_blocks_256=on_device(_blocks(table, queries, 256)),
+        q_blocks_128=on_device(_blocks(table, queries, 128)),
+        k_blocks_128=on_device(_blocks(table, keys, 128)[::-1]),
         longest_q=max(queries),
         longest_k=max(keys),
     )

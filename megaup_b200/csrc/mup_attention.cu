@@ -207,9 +207,11 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
   AttnForward p{};
   p.shape = make_shape(a, status);
   if (a.sequences != nullptr)
-    p.tiles = reinterpret_cast<const int2*>(f.small_blocks ? a.q_blocks_128 : a.q_blocks_256);
+    p.tiles = reinterpret_cast<const AttnPackedBlock*>(f.small_blocks ? a.q_blocks_128 : a.q_blocks_256);
   p.blocks_per_sequence = f.blocks / a.batch;
-  p.head_sets = f.head_sets, p.packed_heads = f.packed_heads, p.pair_heads = f.pair_heads;
+  p.head_sets = f.head_sets, p.packed_heads = f.packed_heads, p.rows_log2 = 7;
+  for (int h = f.packed_heads; h > 1; h /= 2) --p.rows_log2;
+  p.pair_heads = f.pair_heads;
   p.splits = f.splits, p.single = f.single;
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.out_batch = a.out_strides[0], p.out_seq = a.out_strides[1], p.out_head = a.out_strides[2];
@@ -328,8 +330,8 @@ int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t
   AttnBackward p{};
   p.shape = make_shape(a, status);
   const bool packed = a.sequences != nullptr;
-  p.q_blocks = reinterpret_cast<const int2*>(packed ? a.q_blocks_128 : nullptr);
-  p.k_blocks = reinterpret_cast<const int2*>(packed ? a.k_blocks_128 : nullptr);
+  p.q_blocks = reinterpret_cast<const AttnPackedBlock*>(packed ? a.q_blocks_128 : nullptr);
+  p.k_blocks = reinterpret_cast<const AttnPackedBlock*>(packed ? a.k_blocks_128 : nullptr);
   p.n_q_blocks = packed ? a.n_q_blocks_128 : ceil_div(a.seq_q, kTileRows);
   p.n_k_blocks = packed ? a.n_k_blocks_128 : ceil_div(a.seq_k, kTileRows);
   p.n_sequences = packed ? a.n_sequences : a.batch;

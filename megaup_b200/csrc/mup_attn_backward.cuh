@@ -13,8 +13,8 @@ namespace mup {
 
 struct AttnBackward {
   AttnShape shape;
-  const int2* q_blocks;  // packed: {sequence, first row} per 128 query rows
-  const int2* k_blocks;  // packed: the same of the key rows
+  const AttnPackedBlock* q_blocks;  // packed: blocks of 128 query rows; null when dense
+  const AttnPackedBlock* k_blocks;  // packed: blocks of 128 key rows
   int n_q_blocks, n_k_blocks;  // packed: of the lists; dense: per sequence
   int n_sequences;
   int dkv_jobs;  // CTAs of dK and dV
@@ -124,13 +124,13 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
   const int head = job % p.shape.heads_q;
   const int w = job / p.shape.heads_q;
   int sequence, row0;
+  AttnSeq seq;
   if (p.q_blocks != nullptr) {
-    const int2 block = p.q_blocks[w];
-    sequence = block.x, row0 = block.y;
+    seq = load_block(p.q_blocks, w, sequence, row0);
   } else {
     sequence = w % p.shape.batch, row0 = (p.n_q_blocks - 1 - w / p.shape.batch) * kTileRows;
+    seq = load_sequence(p.shape, sequence);
   }
-  const AttnSeq seq = load_sequence(p.shape, sequence);
   const int batch = p.shape.sequences != nullptr ? 0 : sequence;
   const int kv_head = head / (p.shape.heads_q / p.shape.heads_kv);
   const RowSpan first = row_span(p.shape, seq, row0);
@@ -387,25 +387,28 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
   const int heads_kv = p.shape.heads_kv, group = p.shape.heads_q / heads_kv;
   const int shared_jobs = p.n_sequences * heads_kv * p.shared_tiles * p.shares;
   int sequence, tile, kv_head, share = 0, shares = 1;
+  AttnSeq seq;
   if (job < shared_jobs) {
     share = job % p.shares, shares = p.shares;
     job /= p.shares;
     tile = job % p.shared_tiles;
     kv_head = job / p.shared_tiles % heads_kv;
     sequence = job / p.shared_tiles / heads_kv;
+    seq = load_sequence(p.shape, sequence);
   } else {
     job -= shared_jobs;
     kv_head = job % heads_kv;
     job /= heads_kv;
     if (p.k_blocks != nullptr) {
-      const int2 block = p.k_blocks[job];
-      sequence = block.x, tile = block.y / kTileRows;
+      int row0;
+      seq = load_block(p.k_blocks, job, sequence, row0);
+      tile = row0 / kTileRows;
       if (tile < p.shared_tiles) return;
     } else {
       sequence = job % p.shape.batch, tile = p.shared_tiles + job / p.shape.batch;
+      seq = load_sequence(p.shape, sequence);
     }
   }
-  const AttnSeq seq = load_sequence(p.shape, sequence);
   const int batch = p.shape.sequences != nullptr ? 0 : sequence;
   const int j0 = tile * kTileRows;
   if (j0 >= seq.nk) return;  // packed: a shared tile that this sequence does not have

@@ -47,6 +47,19 @@ __device__ __forceinline__ AttnSeq load_sequence(const AttnShape& p, int sequenc
   return s;
 }
 
+// An entry of a packed block list: a block of rows and the sequence it belongs to, read at once.
+struct alignas(32) AttnPackedBlock {
+  int sequence, row0, q0, nq, k0, nk, unused[2];
+};
+__device__ __forceinline__ AttnSeq load_block(const AttnPackedBlock* list, int i, int& sequence, int& row0) {
+  const int4 a = reinterpret_cast<const int4*>(list + i)[0], b = reinterpret_cast<const int4*>(list + i)[1];
+  sequence = a.x, row0 = a.y;
+  AttnSeq s;
+  s.q0 = a.z, s.nq = a.w, s.k0 = b.x, s.nk = b.y;
+  s.off = s.nk - s.nq;
+  return s;
+}
+
 struct RowSpan {
   int sink, low, high;  // [0, sink) and [low, high]
 };

@@ -13,10 +13,11 @@ namespace mup {
 
 struct AttnForward {
   AttnShape shape;
-  const int2* tiles;        // packed: {sequence, first row} per row block; null when dense
+  const AttnPackedBlock* tiles;  // packed: the row blocks; null when dense
   int blocks_per_sequence;  // dense: row blocks per sequence
   int head_sets;            // heads_q / heads per CTA
-  int packed_heads;         // heads per sub-tile (a power of two): rows of a sub-tile = heads x rows_per_head
+  int packed_heads;         // heads per sub-tile, a power of two: its 128 rows are heads x rows of a head
+  int rows_log2;            // of a head in a sub-tile
   int pair_heads;           // sub-tile 1 holds the next heads (1) or the next rows (0)
   int splits;               // CTAs that share one block's key tiles
   int single;               // only sub-tile 0 exists
@@ -47,7 +48,7 @@ struct AttnForwardConfig {
 // What a CTA computes: decoded by each role for itself, so that no role holds what only another needs.
 struct ForwardBlock {
   AttnSeq seq;
-  int batch, head0, kv_head, rows, row0, row_step, head_step, split;
+  int batch, head0, kv_head, rows, rows_log2, row0, row_step, head_step, split;
 
   __device__ __forceinline__ explicit ForwardBlock(const AttnForward& p) {
     int w = blockIdx.x;
@@ -56,18 +57,18 @@ struct ForwardBlock {
     const int head_set = w % p.head_sets;
     w /= p.head_sets;
     int sequence;
-    rows = kTileRows / p.packed_heads;  // rows of a head in a sub-tile
+    rows_log2 = p.rows_log2;
+    rows = 1 << rows_log2;
     row_step = p.pair_heads ? 0 : rows;
     head_step = p.pair_heads ? p.packed_heads : 0;
     if (p.tiles != nullptr) {
-      const int2 tile = p.tiles[w];
-      sequence = tile.x, row0 = tile.y;
+      seq = load_block(p.tiles, w, sequence, row0);
     } else {
       // the last rows first: under a causal mask they have the most keys
       sequence = w % p.shape.batch;
       row0 = (p.blocks_per_sequence - 1 - w / p.shape.batch) * (p.single || p.pair_heads ? rows : 2 * rows);
+      seq = load_sequence(p.shape, sequence);
     }
-    seq = load_sequence(p.shape, sequence);
     batch = p.shape.sequences != nullptr ? 0 : sequence;
     head0 = head_set * p.packed_heads * (p.pair_heads ? 2 : 1);
     kv_head = head0 / (p.shape.heads_q / p.shape.heads_kv);
@@ -122,16 +123,29 @@ __global__ void __launch_bounds__(384, 1)
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
   grid_dep_launch();
-  if (threadIdx.x == 0) {
+  // The copies of this CTA, in the order of the products: for step i K of tile i, then V of the tile before it.
+  const auto load_tile = [&](const ForwardBlock& block, const CUtensorMap& map, int kt, int s) {
+    mbar_arrive_expect_tx(full(s), Cfg::kTileBytes);
+    const uint32_t dst = base + Cfg::kOffStages + s * Cfg::kTileBytes;
+#pragma unroll
+    for (int panel = 0; panel < Cfg::kPanels; ++panel)
+      tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, block.seq.k0 + kt * kTileRows, block.kv_head, block.batch,
+                  full(s));
+  };
+  const bool loads_here = warp == 8 && elect_one_sync();
+  if (loads_here) {
+    const ForwardBlock block(p);
+    const TileList all = block.all(p);
+    int begin, end;
+    block.share(p, all.count, begin, end);
     *abort_flag = 0u;
-    const int users = ForwardBlock(p).exists(p, 1) ? 2 : 1;  // warps that read a stage
-    mbar_init(q_full(0), 1);
-    mbar_init(q_full(1), 1);
+    const int users = block.exists(p, 1) ? 2 : 1;  // warps that read a stage
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), users);
     }
     for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full(t), 1);
       mbar_init(drain(t), 1);
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t, 0), 128);
@@ -140,6 +154,20 @@ __global__ void __launch_bounds__(384, 1)
     }
     fence_mbar_init();
     fence_proxy_async_smem();
+    // the first copies do not wait for the other warps
+    if (begin < end) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!block.exists(p, t)) continue;
+        mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
+#pragma unroll
+        for (int panel = 0; panel < Cfg::kPanels; ++panel)
+          tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
+                      block.seq.q0 + block.row0 + t * block.row_step, block.head0 + t * block.head_step, block.batch,
+                      q_full(t));
+        if (t == 0) load_tile(block, k_map, all.tile(begin), 0);
+      }
+    }
   }
   if (warp == 9) {
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
@@ -152,44 +180,24 @@ __global__ void __launch_bounds__(384, 1)
 
   if (warp >= 8) {
     fewer_registers<72>();
-    if (warp == 8 && elect_one_sync()) {
+    if (loads_here) {
+      // ------------------------------------------------------------ TMA loads
       const ForwardBlock block(p);
       const TileList all = block.all(p);
       int begin, end;
       block.share(p, all.count, begin, end);
-      // ------------------------------------------------------------ TMA loads
-      tma_prefetch_desc(&k_map);
-      tma_prefetch_desc(&v_map);
-      int loads = 0;
+      int loads = 1;
       bool ok = true;
-      auto load_tile = [&](const CUtensorMap& map, int kt) {
+      const auto load = [&](const CUtensorMap& map, int kt) {
         const int s = loads % Cfg::kStages, use = loads / Cfg::kStages;
         if (use > 0 && !ctl.wait(empty(s), (use - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) return false;
-        mbar_arrive_expect_tx(full(s), Cfg::kTileBytes);
-        const uint32_t dst = base + Cfg::kOffStages + s * Cfg::kTileBytes;
-#pragma unroll
-        for (int panel = 0; panel < Cfg::kPanels; ++panel)
-          tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, block.seq.k0 + kt * kTileRows, block.kv_head, block.batch,
-                      full(s));
+        load_tile(block, map, kt, s);
         ++loads;
         return true;
       };
-      if (begin < end) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!block.exists(p, t)) continue;
-          mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
-#pragma unroll
-          for (int panel = 0; panel < Cfg::kPanels; ++panel)
-            tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
-                        block.seq.q0 + block.row0 + t * block.row_step, block.head0 + t * block.head_step, block.batch,
-                        q_full(t));
-          if (t == 0) ok = load_tile(k_map, all.tile(begin));
-        }
-        for (int i = begin + 1; ok && i <= end; ++i) {
-          if (i < end) ok = load_tile(k_map, all.tile(i));
-          if (ok) ok = load_tile(v_map, all.tile(i - 1));
-        }
+      for (int i = begin + 1; ok && i <= end; ++i) {
+        if (i < end) ok = load(k_map, all.tile(i));
+        if (ok) ok = load(v_map, all.tile(i - 1));
       }
       if (!ok) {  // the copies in flight end before this CTA's shared memory is given up
 #pragma unroll
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(384, 1)
     const RowSpan first = block.first(p, t), last = block.last(p, t);
     int begin, end;
     block.share(p, all.count, begin, end);
-    const int row = block.row0 + t * block.row_step + r % block.rows;
+    const int row = block.row0 + t * block.row_step + (r & (block.rows - 1));
     const bool exists = block.exists(p, t);
     const RowSpan span = row_span(p.shape, block.seq, row);
     const float c = p.shape.scale_log2;
@@ -372,10 +380,10 @@ __global__ void __launch_bounds__(384, 1)
       tc_fence_after_sync();
       const int head0 = block.head0 + t * block.head_step, tile_row0 = block.row0 + t * block.row_step;
       const auto index_of = [&](int x) {  // of row x of the sub-tile
-        return (static_cast<int64_t>(block.batch) * p.shape.heads_q + head0 + x / block.rows) * p.shape.seq_q + block.seq.q0 +
-               tile_row0 + x % block.rows;
+        return (static_cast<int64_t>(block.batch) * p.shape.heads_q + head0 + (x >> block.rows_log2)) * p.shape.seq_q +
+               block.seq.q0 + tile_row0 + (x & (block.rows - 1));
       };
-      const auto is_row = [&](int x) { return tile_row0 + x % block.rows < block.seq.nq; };
+      const auto is_row = [&](int x) { return tile_row0 + (x & (block.rows - 1)) < block.seq.nq; };
       const bool empty_row = sum == 0.0f;
       if (is_row(r)) {
         const float lse2 = empty_row ? -INFINITY : top * c + log2f(sum);
@@ -425,8 +433,8 @@ __global__ void __launch_bounds__(384, 1)
         write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
           return !is_row(x) ? nullptr
                             : reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
-                                                         (block.seq.q0 + tile_row0 + x % block.rows) * p.out_seq +
-                                                         (head0 + x / block.rows) * p.out_head);
+                                                         (block.seq.q0 + tile_row0 + (x & (block.rows - 1))) * p.out_seq +
+                                                         (head0 + (x >> block.rows_log2)) * p.out_head);
         });
       }
     }

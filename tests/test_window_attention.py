@@ -97,9 +97,14 @@ def test_window_sides() -> None:
 def test_packed_sequences_on_the_host() -> None:
     s = mega_up.prepare_packed_sequences([0, 300, 300, 301], [0, 0, 5, 140], device="cpu")
     assert s.sequences.tolist() == [[0, 300, 0, 0], [300, 0, 0, 5], [300, 1, 5, 135]]
-    assert s.q_blocks_256.tolist() == [[0, 256], [0, 0], [2, 0]]
-    assert s.q_blocks_128.tolist() == [[0, 256], [0, 128], [0, 0], [2, 0]]
-    assert sorted(map(tuple, s.k_blocks_128.tolist())) == [(1, 0), (2, 0), (2, 128)]
+    table = s.sequences.tolist()
+
+    def blocks(*pairs):
+        return [[sequence, row, *table[sequence], 0, 0] for sequence, row in pairs]
+
+    assert s.q_blocks_256.tolist() == blocks((0, 256), (0, 0), (2, 0))
+    assert s.q_blocks_128.tolist() == blocks((0, 256), (0, 128), (0, 0), (2, 0))
+    assert sorted(s.k_blocks_128.tolist()) == blocks((1, 0), (2, 0), (2, 128))
     assert (s.longest_q, s.longest_k, s.num_sequences) == (300, 135, 3)
     layout = mega_up.prepare_packed_sequences(torch.tensor([0, 4], dtype=torch.int32), device="cpu")
     assert layout.cu_seqlens_k == (0, 4)
