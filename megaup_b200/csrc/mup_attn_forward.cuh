@@ -235,7 +235,14 @@ __global__ void __launch_bounds__(384, 1)
           ok = ctl.wait(full(ks), phase, MUP_ST_MMA_FULL_TIMEOUT);
           advance();
           active = exists && sees_tile(mine, all.tile(i));
-          if (active && steps == 0) ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
+          if (active && steps == 0) {
+            ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
+            // Behind the first sub-tile's first product: the one's exponentials then run beside the other's products, and
+            // both stay so (3030 cycles a step). Started together they stay together for ten steps and more, at 4700 to
+            // 5800 cycles a step.
+            if (t == 1 && i == begin && block.exists(p, 0) && sees_tile(block.tiles(p, 0), all.tile(i)))
+              ok = ok && ctl.wait(s_full(0), 0, MUP_ST_MMA_ACC_TIMEOUT);
+          }
         }
         if (ok && i > begin) {
           const int vs = stage;
