@@ -354,6 +354,22 @@ __device__ __forceinline__ void write_staged_rows(uint8_t* tile, int first, int 
   }
   __syncwarp();
 }
+// The same where row r goes to `to` + r * stride, rows from `end` on nowhere.
+template <int RB>
+__device__ __forceinline__ void write_staged_rows(uint8_t* tile, int first, int lane, int bytes, uint8_t* to,
+                                                  int64_t stride, int end) {
+  constexpr int kLanes = RB / 16, kRows = 32 / kLanes;
+  __syncwarp();
+  const int chunk = lane % kLanes, r0 = first + lane / kLanes;
+  uint8_t* dst = to + r0 * stride + chunk * 16;
+  if (chunk * 16 >= bytes) end = 0;
+#pragma unroll 8
+  for (int k = 0; k < kLanes; ++k, dst += kRows * stride) {
+    const uint4 v = *staged_piece<RB>(tile, r0 + k * kRows, chunk);
+    if (r0 + k * kRows < end) *reinterpret_cast<uint4*>(dst) = v;
+  }
+  __syncwarp();
+}
 __device__ __forceinline__ uint4 pack_bf16x8(const uint32_t* v, float scale) {
   uint4 p;
   p.x = pack_bf16(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale);

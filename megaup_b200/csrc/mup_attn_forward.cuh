@@ -132,57 +132,56 @@ __global__ void __launch_bounds__(384, 1)
       tma_load_4d(dst + panel * kPanelBytes, &map, panel * 64, block.seq.k0 + kt * kTileRows, block.kv_head, block.batch,
                   full(s));
   };
-  const bool loads_here = warp == 8 && elect_one_sync();
-  if (loads_here) {
-    const ForwardBlock block(p);
-    const TileList all = block.all(p);
-    int begin, end;
-    block.share(p, all.count, begin, end);
-    *abort_flag = 0u;
-    const int users = block.exists(p, 1) ? 2 : 1;  // warps that read a stage
-    for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), users);
-    }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(q_full(t), 1);
-      mbar_init(drain(t), 1);
-      mbar_init(s_full(t), 1);
-      mbar_init(p_full(t, 0), 128);
-      mbar_init(p_full(t, 1), 128);
-      mbar_init(done(t), 1);
-    }
-    fence_mbar_init();
-    fence_proxy_async_smem();
-    // the first copies do not wait for the other warps
-    if (begin < end) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (!block.exists(p, t)) continue;
-        mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
-#pragma unroll
-        for (int panel = 0; panel < Cfg::kPanels; ++panel)
-          tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
-                      block.seq.q0 + block.row0 + t * block.row_step, block.head0 + t * block.head_step, block.batch,
-                      q_full(t));
-        if (t == 0) load_tile(block, k_map, all.tile(begin), 0);
-      }
-    }
-  }
-  if (warp == 9) {
-    tmem_alloc<1>(smem_u32(tmem_slot), 512);
-    tmem_relinquish<1>();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-
+  // Both kinds of warps change their registers first and meet when barriers and TMEM are there.
   if (warp >= 8) {
     fewer_registers<72>();
+    const bool loads_here = warp == 8 && elect_one_sync();
+    const ForwardBlock block(p);
+    if (loads_here) {
+      const TileList all = block.all(p);
+      int begin, end;
+      block.share(p, all.count, begin, end);
+      *abort_flag = 0u;
+      const int users = block.exists(p, 1) ? 2 : 1;  // warps that read a stage
+      for (int s = 0; s < Cfg::kStages; ++s) {
+        mbar_init(full(s), 1);
+        mbar_init(empty(s), users);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(q_full(t), 1);
+        mbar_init(drain(t), 1);
+        mbar_init(s_full(t), 1);
+        mbar_init(p_full(t, 0), 128);
+        mbar_init(p_full(t, 1), 128);
+        mbar_init(done(t), 1);
+      }
+      fence_mbar_init();
+      fence_proxy_async_smem();
+      // the first copies do not wait for the other warps
+      if (begin < end) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!block.exists(p, t)) continue;
+          mbar_arrive_expect_tx(q_full(t), Cfg::kTileBytes);
+#pragma unroll
+          for (int panel = 0; panel < Cfg::kPanels; ++panel)
+            tma_load_4d(base + Cfg::kOffQ + t * Cfg::kTileBytes + panel * kPanelBytes, &q_map, panel * 64,
+                        block.seq.q0 + block.row0 + t * block.row_step, block.head0 + t * block.head_step, block.batch,
+                        q_full(t));
+          if (t == 0) load_tile(block, k_map, all.tile(begin), 0);
+        }
+      }
+    }
+    if (warp == 9) {
+      tmem_alloc<1>(smem_u32(tmem_slot), 512);
+      tmem_relinquish<1>();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
     if (loads_here) {
       // ------------------------------------------------------------ TMA loads
-      const ForwardBlock block(p);
       const TileList all = block.all(p);
       int begin, end;
       block.share(p, all.count, begin, end);
@@ -206,13 +205,12 @@ __global__ void __launch_bounds__(384, 1)
         for (int n = max(0, loads - Cfg::kStages); n < loads; ++n)
           drain_barrier(full(n % Cfg::kStages), (n / Cfg::kStages) & 1);
       }
-    } else if (warp == 9 || (warp == 10 && ForwardBlock(p).exists(p, 1))) {
+    } else if (warp == 9 || (warp == 10 && block.exists(p, 1))) {
       // ------------------------------------------------------------ products
       // One warp per sub-tile: the issue of a product waits for room in the tensor pipe's short queue, so with one
       // warp for both every barrier between two issues left the pipe empty.
       const int t = warp - 9;
       const bool leader = elect_one_sync();
-      const ForwardBlock block(p);
       const TileList all = block.all(p), mine = block.tiles(p, t);
       const bool exists = block.exists(p, t);
       int begin, end;
@@ -296,9 +294,6 @@ __global__ void __launch_bounds__(384, 1)
     const int t = warp / 4;
     const int quarter = warp % 4;
     const int r = quarter * 32 + lane;
-    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_tmem = tmem + t * kTileRows + lane_base;
-    const uint32_t o_tmem = tmem + Cfg::kTmemO + t * DP + lane_base;
     const ForwardBlock block(p);
     const TileList all = block.all(p), mine = block.tiles(p, t);
     const RowSpan first = block.first(p, t), last = block.last(p, t);
@@ -308,6 +303,13 @@ __global__ void __launch_bounds__(384, 1)
     const bool exists = block.exists(p, t);
     const RowSpan span = row_span(p.shape, block.seq, row);
     const float c = p.shape.scale_log2;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_tmem = tmem + t * kTileRows + lane_base;
+    const uint32_t o_tmem = tmem + Cfg::kTmemO + t * DP + lane_base;
     float top = -INFINITY, sum = 0.0f;
     int steps = 0;
     bool ok = true;
@@ -423,7 +425,13 @@ __global__ void __launch_bounds__(384, 1)
                   make_float4(__uint_as_float(o[x]) * scale, __uint_as_float(o[x + 1]) * scale,
                               __uint_as_float(o[x + 2]) * scale, __uint_as_float(o[x + 3]) * scale);
           }
-          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, kRowBytes, [&](int x) {
+          if (p.packed_heads == 1)
+            write_staged_rows<kRowBytes>(staged, quarter * 32, lane, kRowBytes,
+                                         reinterpret_cast<uint8_t*>(p.partial_out + (block.split * p.total_rows + index_of(0)) * DP +
+                                                                    half * (DP / 2)),
+                                         DP * 4, block.seq.nq - tile_row0);
+          else
+            write_staged_rows<kRowBytes>(staged, quarter * 32, lane, kRowBytes, [&](int x) {
             return !is_row(x) ? nullptr
                               : reinterpret_cast<uint8_t*>(p.partial_out + (block.split * p.total_rows + index_of(x)) * DP +
                                                            half * (DP / 2));
@@ -437,7 +445,13 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int x = 0; x < 32; x += 8) *staged_piece<kRowBytes>(staged, r, b * 4 + x / 8) = pack_bf16x8(o + x, scale);
         }
-        write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
+        if (p.packed_heads == 1)
+          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2,
+                                       reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
+                                                                  (block.seq.q0 + tile_row0) * p.out_seq + head0 * p.out_head),
+                                       p.out_seq * 2, block.seq.nq - tile_row0);
+        else
+          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
           return !is_row(x) ? nullptr
                             : reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
                                                          (block.seq.q0 + tile_row0 + (x & (block.rows - 1))) * p.out_seq +
@@ -450,7 +464,7 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   if (warp == 9) {
     tc_fence_after_sync();
-    tmem_dealloc<1>(tmem, 512);
+    tmem_dealloc<1>(*tmem_slot, 512);
   }
 }
 
