@@ -400,11 +400,13 @@ typedef struct mup_axial_rotary {
   int32_t axes;
   int32_t interleaved;
   int32_t inverse;
-  int32_t heads[2]; /* heads[1] == 0: one tensor */
-  const void *x[2];
-  void *y[2];
-  int64_t x_strides[2][3];
-  int64_t y_strides[2][3];
+  int32_t heads[2]; /* of q and k; heads[1] == 0: q alone */
+  const void *q;
+  const void *k;
+  void *q_out;
+  void *k_out;
+  int64_t x_strides[2][3]; /* of q and k */
+  int64_t y_strides[2][3]; /* of their outputs */
   const void *positions; /* element of axis a, sequence b, row r at a * pos_strides[0] + b * [1] + r * [2] */
   int64_t pos_strides[3];
   int32_t position_type; /* MUP_ROTARY_* */

@@ -81,8 +81,7 @@ class MupAxialRotary(ctypes.Structure):
             "device", "batch", "rows", "head_dim", "pairs", "axes", "interleaved", "inverse",
         )),
         ("heads", c_int32 * 2),
-        ("x", c_void_p * 2),
-        ("y", c_void_p * 2),
+        *((name, c_void_p) for name in ("q", "k", "q_out", "k_out")),
         ("x_strides", c_int64 * 6),
         ("y_strides", c_int64 * 6),
         ("positions", c_void_p),

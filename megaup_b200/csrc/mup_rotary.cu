@@ -228,10 +228,12 @@ extern "C" int mup_axial_rotary_launch(const mup_axial_rotary* args, void* strea
   RotaryParams p{};
   for (int t = 0; t < 2; ++t) {
     if (a.heads[t] == 0) continue;
-    int rc = check_rows(t == 0 ? "q" : "k", a.x[t], a.x_strides[t]);
-    if (rc == MUP_OK) rc = check_rows(t == 0 ? "q's output" : "k's output", a.y[t], a.y_strides[t]);
+    const void* x = t == 0 ? a.q : a.k;
+    void* y = t == 0 ? a.q_out : a.k_out;
+    int rc = check_rows(t == 0 ? "q" : "k", x, a.x_strides[t]);
+    if (rc == MUP_OK) rc = check_rows(t == 0 ? "q's output" : "k's output", y, a.y_strides[t]);
     if (rc != MUP_OK) return rc;
-    p.x[t] = static_cast<const __nv_bfloat16*>(a.x[t]), p.y[t] = static_cast<__nv_bfloat16*>(a.y[t]);
+    p.x[t] = static_cast<const __nv_bfloat16*>(x), p.y[t] = static_cast<__nv_bfloat16*>(y);
     p.x_batch[t] = a.x_strides[t][0], p.x_row[t] = a.x_strides[t][1], p.x_head[t] = a.x_strides[t][2];
     p.y_batch[t] = a.y_strides[t][0], p.y_row[t] = a.y_strides[t][1], p.y_head[t] = a.y_strides[t][2];
     p.heads[t] = a.heads[t];

@@ -173,14 +173,17 @@ def _turn(
     *, dense: bool = True,
 ) -> None:
     a = _native.MupAxialRotary.from_buffer_copy(block)
-    for i, (x, y) in enumerate(zip(tensors, outputs)):
-        a.x[i], a.y[i] = source, _ = x.data_ptr(), y.data_ptr()
-        if source % 16:
-            raise ValueError(f"q and k must be 16-byte aligned, got address {source:#x}")
+    x = tensors[0]
+    a.q, a.q_out = address, _ = x.data_ptr(), outputs[0].data_ptr()
+    if len(tensors) == 2:
+        a.k, a.k_out = other, _ = tensors[1].data_ptr(), outputs[1].data_ptr()
+        address |= other
+    if address % 16:
+        raise ValueError("q and k must be 16-byte aligned, got addresses " + ", ".join(hex(t.data_ptr()) for t in tensors))
     if not dense:
         a.y_strides[: 3 * len(outputs)] = [s for t in outputs for s in _row_strides(t.shape, t.stride(), kind)]
     a.positions, a.inverse = positions.data_ptr(), inverse
-    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(tensors[0].get_device()).cuda_stream)
+    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(x.get_device()).cuda_stream)
 
 
 def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
@@ -214,10 +217,12 @@ def _plan(kind: str, tensors: Sequence[Tensor | None], rotary: AxialRotary, posi
     """The checked argument block of a call, kept per set of shapes and strides."""
 
     try:
-        key = (
-            kind, positions.shape, positions.stride(), positions.dtype, positions.device,
-            *((t.shape, t.stride(), t.dtype, t.device) for t in tensors),
-        )
+        q = tensors[0]
+        key = (kind, positions.shape, positions.stride(), positions.dtype, positions.device,
+               q.shape, q.stride(), q.dtype, q.device)
+        if len(tensors) == 2:
+            k = tensors[1]
+            key += (k.shape, k.stride(), k.dtype, k.device)
         return rotary.plans[key]
     except (KeyError, AttributeError):  # new, not a tensor
         _check(kind, tensors[0], tensors[1] if len(tensors) > 1 else None, rotary, positions)
@@ -232,7 +237,7 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
         raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
     tensors = (q,) if k is None else (q, k)
     block = _plan(kind, tensors, rotary, positions)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
         outputs = _AxialRotary.apply(block, kind, rotary, positions, *tensors)

@@ -52,7 +52,8 @@ def _block(**changes) -> _native.MupAxialRotary:
     a = _native.MupAxialRotary()
     a.batch, a.rows, a.head_dim, a.pairs, a.axes, a.interleaved = 1, 4, 64, 32, 1, 1
     a.heads[:] = (2, 1)
-    a.x[:] = a.y[:] = (4096, 8192)
+    a.q = a.q_out = 4096
+    a.k = a.k_out = 8192
     a.x_strides[:] = a.y_strides[:] = (512, 128, 64, 512, 128, 64)
     a.positions = a.turns = a.pair_axis = 4096
     for name, value in changes.items():
@@ -64,8 +65,8 @@ def _block(**changes) -> _native.MupAxialRotary:
     "changes",
     [dict(head_dim=4), dict(head_dim=68), dict(head_dim=264), dict(pairs=0), dict(pairs=33), dict(interleaved=0, pairs=12),
      dict(batch=0), dict(rows=0), dict(axes=0), dict(heads=(ctypes.c_int32 * 2)(0, 1)), dict(positions=0), dict(turns=0),
-     dict(pair_axis=0), dict(position_type=3), dict(x=(ctypes.c_void_p * 2)(4096, 0)),
-     dict(y=(ctypes.c_void_p * 2)(4104, 4096)), dict(x_strides=(ctypes.c_int64 * 6)(512, 129, 64, 512, 128, 64)),
+     dict(pair_axis=0), dict(position_type=3), dict(k=0),
+     dict(q_out=4104), dict(x_strides=(ctypes.c_int64 * 6)(512, 129, 64, 512, 128, 64)),
      dict(y_strides=(ctypes.c_int64 * 6)(512, 128, 64, 512, 128, -64))],
     ids=str,
 )
