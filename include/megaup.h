@@ -346,6 +346,10 @@ typedef struct mup_window_attention {
   const void *v;
   void *out;
   float *lse; /* [batch, heads_q, seq_q]; optional in the forward pass */
+  /* What out's rounding to BF16 left, itself BF16, in out's strides; optional. The
+   * forward pass writes it for the backward pass, whose row sums of dout * out would
+   * else carry that rounding into every element of a row's score gradient. */
+  void *out_rest;
   const void *dout;
   void *dq;
   void *dk;

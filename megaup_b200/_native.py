@@ -61,7 +61,7 @@ class MupWindowAttention(ctypes.Structure):
         ("scale", ctypes.c_float),
         *((name + "_strides", c_int64 * 3) for name in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")),
         *((name, c_void_p) for name in (
-            "q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "kv_lengths", "sequences", "q_blocks_256",
+            "q", "k", "v", "out", "lse", "out_rest", "dout", "dq", "dk", "dv", "kv_lengths", "sequences", "q_blocks_256",
             "q_blocks_128", "k_blocks_128",
         )),
         *((name, c_int32) for name in (

@@ -24,6 +24,7 @@ The gradient is deterministic. Kernels: ``csrc/mup_attn_*.cuh``.
 
 from __future__ import annotations
 
+import array
 import ctypes
 from collections.abc import Sequence
 from dataclasses import dataclass, field
@@ -74,7 +75,8 @@ def _blocks(table: list[tuple[int, int, int, int]], lengths: list[int], rows: in
     blocks = [
         (s, r, *entry, 0, 0) for s, (entry, length) in enumerate(zip(table, lengths)) for r in range(0, length, rows)
     ]
-    return sorted(blocks, key=lambda block: -block[1])
+    blocks.sort(key=lambda block: -block[1])
+    return blocks
 
 
 def prepare_packed_sequences(
@@ -100,18 +102,22 @@ def prepare_packed_sequences(
     keys = [b - a for a, b in zip(cu_k, cu_k[1:])]
     table = [(a, n, b, m) for a, n, b, m in zip(cu_q, queries, cu_k, keys)]
 
-    def on_device(rows):
-        return torch.tensor(rows, dtype=torch.int32).to(device)
-
+    # one copy to the device; entries of 8 numbers start at multiples of 32 bytes
+    parts = {
+        "q_blocks_256": _blocks(table, queries, 256),
+        "q_blocks_128": _blocks(table, queries, 128),
+        "k_blocks_128": _blocks(table, keys, 128)[::-1],
+        "sequences": table,
+    }
+    flat = array.array("i", (v for rows in parts.values() for row in rows for v in row))
+    everything = torch.frombuffer(flat, dtype=torch.int32).to(device, copy=True)
+    tables, start = {}, 0
+    for name, rows in parts.items():
+        width = 4 if name == "sequences" else 8
+        tables[name] = everything[start : start + len(rows) * width].view(len(rows), width)
+        start += len(rows) * width
     return PackedSequences(
-        cu_seqlens_q=cu_q,
-        cu_seqlens_k=cu_k,
-        sequences=on_device(table),
-        q_blocks_256=on_device(_blocks(table, queries, 256)),
-        q_blocks_128=on_device(_blocks(table, queries, 128)),
-        k_blocks_128=on_device(_blocks(table, keys, 128)[::-1]),
-        longest_q=max(queries),
-        longest_k=max(keys),
+        cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, longest_q=max(queries), longest_k=max(keys), **tables
     )
 
 
@@ -317,7 +323,8 @@ def _check_out(out: object, q: Tensor) -> None:
 
 
 def _forward(
-    plan: _Plan, q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, need_lse: bool, kv_lengths: Tensor | None
+    plan: _Plan, q: Tensor, k: Tensor, v: Tensor, out: Tensor | None, need_lse: bool, kv_lengths: Tensor | None,
+    rest: Tensor | None = None,
 ) -> tuple[Tensor, Tensor | None]:
     a = plan.arguments(q, k, v)
     if out is None:
@@ -331,6 +338,8 @@ def _forward(
         a.lse = lse.data_ptr()
     if kv_lengths is not None:
         a.kv_lengths = kv_lengths.data_ptr()
+    if rest is not None:
+        a.out_rest = rest.data_ptr()
     plan.launch("mup_window_attention_forward", a, plan.forward_bytes)
     return out, lse
 
@@ -339,8 +348,10 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan):
         ctx.set_materialize_grads(False)
-        out, lse = _forward(plan, q, k, v, None, True, None)
-        ctx.save_for_backward(q, k, v, out, lse)
+        # what the result's rounding leaves: the backward pass sums result * gradient per row
+        rest = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out, lse = _forward(plan, q, k, v, None, True, None, rest)
+        ctx.save_for_backward(q, k, v, out, lse, rest)
         ctx.plan = plan
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -350,7 +361,7 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return None, None, None, None
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, rest = ctx.saved_tensors
         plan: _Plan = ctx.plan
         a = plan.arguments(q, k, v)
         if not _rows_are_loadable(dout):  # a broadcast or transposed gradient
@@ -358,7 +369,7 @@ class _WindowAttention(torch.autograd.Function):
         elif not dout.is_contiguous():
             a.dout_strides = _stride_array(dout.shape, dout.stride(), plan.kind)
         dq, dk, dv = grads = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v)]
-        a.out, a.lse, a.dout = out.data_ptr(), lse.data_ptr(), dout.data_ptr()
+        a.out, a.out_rest, a.lse, a.dout = out.data_ptr(), rest.data_ptr(), lse.data_ptr(), dout.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         plan.launch("mup_window_attention_backward", a, plan.backward_bytes)
         return (*grads, None)

@@ -190,7 +190,7 @@ int launch_combine(const mup_window_attention& a, const float* partial_out, cons
   AttnCombine c{};
   c.partial_out = partial_out, c.partial_lse = partial_lse, c.splits = splits;
   c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = total_rows(a);
-  c.out = static_cast<__nv_bfloat16*>(a.out);
+  c.out = static_cast<__nv_bfloat16*>(a.out), c.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   c.out_batch = a.out_strides[0], c.out_seq = a.out_strides[1], c.out_head = a.out_strides[2], c.lse = a.lse;
   MUP_HOST_CUDA(launch_early(attention_combine_kernel<DP>, c.total_rows, 128, 0, stream, c));
   return MUP_OK;
@@ -213,7 +213,7 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
   for (int h = f.packed_heads; h > 1; h /= 2) --p.rows_log2;
   p.pair_heads = f.pair_heads;
   p.splits = f.splits, p.single = f.single;
-  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out = static_cast<__nv_bfloat16*>(a.out), p.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   p.out_batch = a.out_strides[0], p.out_seq = a.out_strides[1], p.out_head = a.out_strides[2];
   p.lse = a.lse;
   p.total_rows = total_rows(a);
@@ -236,7 +236,8 @@ int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* 
   AttnTokens p{};
   p.shape = make_shape(a, status);
   p.q = static_cast<const __nv_bfloat16*>(a.q), p.k = static_cast<const __nv_bfloat16*>(a.k);
-  p.v = static_cast<const __nv_bfloat16*>(a.v), p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.v = static_cast<const __nv_bfloat16*>(a.v);
+  p.out = static_cast<__nv_bfloat16*>(a.out), p.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   p.q_batch = a.q_strides[0], p.q_seq = a.q_strides[1], p.q_head = a.q_strides[2];
   p.k_batch = a.k_strides[0], p.k_seq = a.k_strides[1], p.k_head = a.k_strides[2];
   p.v_batch = a.v_strides[0], p.v_seq = a.v_strides[1], p.v_head = a.v_strides[2];
@@ -321,6 +322,7 @@ int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t
   float* workspace = static_cast<float*>(a.workspace);
 
   AttnDelta d{};
+  d.out_rest = static_cast<const __nv_bfloat16*>(a.out_rest);
   d.out = static_cast<const __nv_bfloat16*>(a.out), d.dout = static_cast<const __nv_bfloat16*>(a.dout);
   d.out_batch = a.out_strides[0], d.out_seq = a.out_strides[1], d.out_head = a.out_strides[2];
   d.dout_batch = a.dout_strides[0], d.dout_seq = a.dout_strides[1], d.dout_head = a.dout_strides[2];
@@ -381,6 +383,7 @@ int mup_window_attention_forward(const mup_window_attention* args, void* stream)
   if (rc == MUP_OK) rc = check_tensor("k", args->k, args->k_strides);
   if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
   if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
+  if (rc == MUP_OK && args->out_rest != nullptr) rc = check_tensor("out_rest", args->out_rest, args->out_strides);
   if (rc == MUP_OK) rc = check_workspace(*args, forward_workspace(*args));
   if (rc != MUP_OK) return rc;
   DeviceScope scope(args->device);
@@ -402,6 +405,7 @@ int mup_window_attention_backward(const mup_window_attention* args, void* stream
   if (rc == MUP_OK) rc = check_tensor("k", args->k, args->k_strides);
   if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
   if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
+  if (rc == MUP_OK && args->out_rest != nullptr) rc = check_tensor("out_rest", args->out_rest, args->out_strides);
   if (rc == MUP_OK) rc = check_tensor("dout", args->dout, args->dout_strides);
   if (rc == MUP_OK) rc = check_tensor("dq", args->dq, args->dq_strides);
   if (rc == MUP_OK) rc = check_tensor("dk", args->dk, args->dk_strides);

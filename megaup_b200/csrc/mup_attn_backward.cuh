@@ -32,7 +32,7 @@ struct AttnBackward {
 // ---------------------------------------------------------------------------
 
 struct AttnDelta {
-  const __nv_bfloat16 *out, *dout;
+  const __nv_bfloat16 *out, *out_rest, *dout;  // out_rest may be null
   int64_t out_batch, out_seq, out_head, dout_batch, dout_seq, dout_head;
   const float* lse;
   float *lse2, *delta;
@@ -51,16 +51,18 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   grid_dep_launch();
   const int lane = threadIdx.x % 32, part = lane % 16;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * 2 * kDeltaRows;
-  uint4 x[kDeltaRows], y[kDeltaRows];
+  uint4 x[kDeltaRows], y[kDeltaRows], z[kDeltaRows];
 #pragma unroll
   for (int i = 0; i < kDeltaRows; ++i) {
     const int64_t item = first + i * 2 + lane / 16;
-    x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    x[i] = y[i] = z[i] = make_uint4(0, 0, 0, 0);
     if (item >= p.total_rows || part * 8 >= p.head_dim) continue;
     const uint32_t bh = static_cast<uint32_t>(item) / p.seq_q, row = static_cast<uint32_t>(item) - bh * p.seq_q;
     const uint32_t b = bh / p.heads_q, head = bh - b * p.heads_q;
     x[i] = ld_stream_v4(p.out + b * p.out_batch + row * p.out_seq + head * p.out_head + part * 8);
     y[i] = ld_stream_v4(p.dout + b * p.dout_batch + row * p.dout_seq + head * p.dout_head + part * 8);
+    if (p.out_rest != nullptr)
+      z[i] = ld_stream_v4(p.out_rest + b * p.out_batch + row * p.out_seq + head * p.out_head + part * 8);
   }
   float mine = 0.0f;  // of row `first + lane`, in the first eight lanes
 #pragma unroll
@@ -69,6 +71,10 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
     sum = dot_bf16x2(x[i].y, y[i].y, sum);
     sum = dot_bf16x2(x[i].z, y[i].z, sum);
     sum = dot_bf16x2(x[i].w, y[i].w, sum);
+    float rest = dot_bf16x2(z[i].x, y[i].x, 0.0f);
+    rest = dot_bf16x2(z[i].y, y[i].y, rest);
+    rest = dot_bf16x2(z[i].z, y[i].z, rest);
+    sum += dot_bf16x2(z[i].w, y[i].w, rest);
 #pragma unroll
     for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const float there = __shfl_sync(0xffffffffu, sum, lane % 2 * 16);

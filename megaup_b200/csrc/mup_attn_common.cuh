@@ -379,6 +379,20 @@ __device__ __forceinline__ uint4 pack_bf16x8(const uint32_t* v, float scale) {
   return p;
 }
 
+// What the rounding of pack_bf16x8 leaves.
+__device__ __forceinline__ uint32_t pack_bf16_rest(float lo, float hi) {
+  const uint32_t p = pack_bf16(lo, hi);
+  return pack_bf16(lo - __uint_as_float(p << 16), hi - __uint_as_float(p & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 pack_bf16x8_rest(const uint32_t* v, float scale) {
+  uint4 p;
+  p.x = pack_bf16_rest(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale);
+  p.y = pack_bf16_rest(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale);
+  p.z = pack_bf16_rest(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale);
+  p.w = pack_bf16_rest(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale);
+  return p;
+}
+
 // A row of a key or value tile that none of the block's rows sees (another sequence's, one behind the filled part of a
 // cache, one between the sinks and the window) has to be finite where its weight is 0: it becomes 0. The whole warp
 // calls this between the tile's arrival and its first product.

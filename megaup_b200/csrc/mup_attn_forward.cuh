@@ -21,7 +21,7 @@ struct AttnForward {
   int pair_heads;           // sub-tile 1 holds the next heads (1) or the next rows (0)
   int splits;               // CTAs that share one block's key tiles
   int single;               // only sub-tile 0 exists
-  __nv_bfloat16* out;
+  __nv_bfloat16 *out, *out_rest;  // out_rest: what out's rounding leaves, or null
   int64_t out_batch, out_seq, out_head;
   float* lse;               // [batch, heads, rows] or null
   float* partial_out;       // [splits, total rows, DP], splits > 1
@@ -438,25 +438,29 @@ __global__ void __launch_bounds__(384, 1)
           });
         }
       } else {
+        const auto write = [&](__nv_bfloat16* out, bool rest) {
 #pragma unroll 1
-        for (int b = 0; b < DP / 32; ++b) {
-          uint32_t o[32];
-          load_o(b, o);
+          for (int b = 0; b < DP / 32; ++b) {
+            uint32_t o[32];
+            load_o(b, o);
 #pragma unroll
-          for (int x = 0; x < 32; x += 8) *staged_piece<kRowBytes>(staged, r, b * 4 + x / 8) = pack_bf16x8(o + x, scale);
-        }
-        if (p.packed_heads == 1)
-          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2,
-                                       reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
-                                                                  (block.seq.q0 + tile_row0) * p.out_seq + head0 * p.out_head),
-                                       p.out_seq * 2, block.seq.nq - tile_row0);
-        else
-          write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
-          return !is_row(x) ? nullptr
-                            : reinterpret_cast<uint8_t*>(p.out + block.batch * p.out_batch +
-                                                         (block.seq.q0 + tile_row0 + (x & (block.rows - 1))) * p.out_seq +
-                                                         (head0 + (x >> block.rows_log2)) * p.out_head);
-        });
+            for (int x = 0; x < 32; x += 8)
+              *staged_piece<kRowBytes>(staged, r, b * 4 + x / 8) =
+                  rest ? pack_bf16x8_rest(o + x, scale) : pack_bf16x8(o + x, scale);
+          }
+          __nv_bfloat16* to = out + block.batch * p.out_batch + (block.seq.q0 + tile_row0) * p.out_seq + head0 * p.out_head;
+          if (p.packed_heads == 1)
+            write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, reinterpret_cast<uint8_t*>(to),
+                                         p.out_seq * 2, block.seq.nq - tile_row0);
+          else
+            write_staged_rows<kRowBytes>(staged, quarter * 32, lane, p.shape.head_dim * 2, [&](int x) {
+              return !is_row(x) ? nullptr
+                                : reinterpret_cast<uint8_t*>(to + (x & (block.rows - 1)) * p.out_seq +
+                                                             (x >> block.rows_log2) * p.out_head);
+            });
+        };
+        write(p.out, false);
+        if (p.out_rest != nullptr) write(p.out_rest, true);
       }
     }
     tc_fence_before_sync();
@@ -475,7 +479,7 @@ struct AttnCombine {
   const float* partial_lse;
   int splits, head_dim, heads_q, seq_q;
   int64_t total_rows;
-  __nv_bfloat16* out;
+  __nv_bfloat16 *out, *out_rest;
   int64_t out_batch, out_seq, out_head;
   float* lse;
 };
@@ -533,9 +537,12 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const __grid_con
   const int seq = static_cast<int>(row % p.seq_q);
   const int64_t bh = row / p.seq_q;
   const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-  __nv_bfloat16* out = p.out + (bh / p.heads_q) * p.out_batch + seq * p.out_seq + (bh % p.heads_q) * p.out_head;
-  *reinterpret_cast<uint2*>(out + quad * 4) =
+  const int64_t at = (bh / p.heads_q) * p.out_batch + seq * p.out_seq + (bh % p.heads_q) * p.out_head + quad * 4;
+  *reinterpret_cast<uint2*>(p.out + at) =
       make_uint2(pack_bf16(acc.x * scale, acc.y * scale), pack_bf16(acc.z * scale, acc.w * scale));
+  if (p.out_rest != nullptr)
+    *reinterpret_cast<uint2*>(p.out_rest + at) =
+        make_uint2(pack_bf16_rest(acc.x * scale, acc.y * scale), pack_bf16_rest(acc.z * scale, acc.w * scale));
   if (quad == 0 && p.lse != nullptr) p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 

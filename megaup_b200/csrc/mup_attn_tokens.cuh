@@ -33,7 +33,7 @@ struct AttnTokens {
   int splits;   // CTAs per sequence and key/value head
   int share;    // steps of a CTA, or 0: a splits-th of its sequence's
   int cluster;  // they are one cluster
-  __nv_bfloat16* out;
+  __nv_bfloat16 *out, *out_rest;  // out_rest: what out's rounding leaves, or null
   int64_t out_batch, out_seq, out_head;
   float* lse;          // [batch, heads, rows] or null
   float* partial_out;  // [splits, total rows, DP] and
@@ -313,10 +313,14 @@ __global__ void __launch_bounds__(32 * kTokenWarps, kTokenCtas) attention_tokens
       }
       const int head = kv_head * group + row / seq.nq, query = seq.q0 + row % seq.nq;
       const float scale = all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
-      __nv_bfloat16* out = p.out + batch * p.out_batch + query * p.out_seq + head * p.out_head + lane * (DP / 32);
+      const int64_t at = batch * p.out_batch + query * p.out_seq + head * p.out_head + lane * (DP / 32);
 #pragma unroll
-      for (int x = 0; x < DP / 32; x += 2)
-        if (lane * (DP / 32) + x < dim) *reinterpret_cast<uint32_t*>(out + x) = pack_bf16(acc[x] * scale, acc[x + 1] * scale);
+      for (int x = 0; x < DP / 32; x += 2) {
+        if (lane * (DP / 32) + x >= dim) continue;
+        *reinterpret_cast<uint32_t*>(p.out + at + x) = pack_bf16(acc[x] * scale, acc[x + 1] * scale);
+        if (p.out_rest != nullptr)
+          *reinterpret_cast<uint32_t*>(p.out_rest + at + x) = pack_bf16_rest(acc[x] * scale, acc[x + 1] * scale);
+      }
       if (p.lse != nullptr && lane == 0)
         p.lse[(static_cast<int64_t>(batch) * p.shape.heads_q + head) * p.shape.seq_q + query] =
             all_sum == 0.0f ? -INFINITY : (all_top + log2f(all_sum)) * 0.69314718055994531f;
@@ -337,10 +341,15 @@ __global__ void __launch_bounds__(32 * kTokenWarps, kTokenCtas) attention_tokens
     for (int x = 0; x < DP / kEach; ++x) dst[x * kEach + column] = joined[x] * scale;
     if (column == 0) p.partial_lse[split * p.total_rows + index] = lse2;
   } else {
-    __nv_bfloat16* out = p.out + batch * p.out_batch + query * p.out_seq + head * p.out_head;
+    const int64_t at = batch * p.out_batch + query * p.out_seq + head * p.out_head + column;
 #pragma unroll
-    for (int x = 0; x < DP / kEach; ++x)
-      if (x * kEach + column < dim) out[x * kEach + column] = __float2bfloat16_rn(joined[x] * scale);
+    for (int x = 0; x < DP / kEach; ++x) {
+      if (x * kEach + column >= dim) continue;
+      const float v = joined[x] * scale;
+      const __nv_bfloat16 rounded = __float2bfloat16_rn(v);
+      p.out[at + x * kEach] = rounded;
+      if (p.out_rest != nullptr) p.out_rest[at + x * kEach] = __float2bfloat16_rn(v - __bfloat162float(rounded));
+    }
     if (column == 0 && p.lse != nullptr) p.lse[index] = lse2 * 0.69314718055994531f;
   }
 }

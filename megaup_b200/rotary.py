@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from collections.abc import Sequence
 from dataclasses import dataclass, field
 
@@ -88,13 +89,16 @@ def prepare_axial_rotary(
     )
     turns = [theta**-e / (2.0 * math.pi) for e in exponents]
     axis = [a for a, d in enumerate(dims) for _ in range(d // 2)]
+    # one copy to the device
+    packed = struct.pack(f"={len(turns)}d{len(axis)}i", *turns, *axis)
+    both = torch.frombuffer(bytearray(packed), dtype=torch.uint8).to(device, copy=True)
     return AxialRotary(
         axis_dims=dims,
         theta=theta,
         interleaved=bool(interleaved),
         shared_frequencies=bool(shared_frequencies),
-        turns=torch.tensor(turns, dtype=torch.float64).to(device),
-        pair_axis=torch.tensor(axis, dtype=torch.int32).to(device),
+        turns=both[: 8 * len(turns)].view(torch.float64),
+        pair_axis=both[8 * len(turns) :].view(torch.int32),
     )
 
 
