@@ -338,6 +338,10 @@ bool pdl_enabled() {
   return cached == 1;
 }
 
+}  // namespace
+bool mup::early_launches() { return pdl_enabled(); }
+namespace {
+
 template <int G, int MODE>
 int launch_kernel(const mup::GemmParams& params, int grid, cudaStream_t stream) {
   // lists without two-accumulator items run the instantiation without their code

@@ -169,21 +169,6 @@ int encode_rows(CUtensorMap* map, const mup_window_attention& a, const void* bas
   return encode_map_4d(map, base, dims, order, box);
 }
 
-// A launch that may begin while the CTAs of the kernel before it run; the kernel waits for that one's end itself
-// (grid_dep_wait) before it touches its results.
-template <typename... Params, typename... Args>
-cudaError_t launch_early(void (*kernel)(Params...), int64_t blocks, int threads, int smem, cudaStream_t stream,
-                         const Args&... args) {
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks)), config.blockDim = dim3(static_cast<unsigned>(threads));
-  config.dynamicSmemBytes = static_cast<size_t>(smem), config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute, config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 template <int DP>
 int launch_combine(const mup_window_attention& a, const float* partial_out, const float* partial_lse, int splits,
                    cudaStream_t stream) {
@@ -192,7 +177,7 @@ int launch_combine(const mup_window_attention& a, const float* partial_out, cons
   c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = total_rows(a);
   c.out = static_cast<__nv_bfloat16*>(a.out), c.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   c.out_batch = a.out_strides[0], c.out_seq = a.out_strides[1], c.out_head = a.out_strides[2], c.lse = a.lse;
-  MUP_HOST_CUDA(launch_early(attention_combine_kernel<DP>, c.total_rows, 128, 0, stream, c));
+  MUP_HOST_CUDA(launch_early(attention_combine_kernel<DP>, dim3(static_cast<unsigned>(c.total_rows)), 128, 0, 1, stream, c));
   return MUP_OK;
 }
 
@@ -224,8 +209,8 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
   MUP_HOST_CUDA(allow_smem_once(attention_forward_kernel<DP>, Cfg::kSmemBytes, a.device, &ready));
   const int64_t grid = static_cast<int64_t>(f.blocks) * f.head_sets * f.splits;
   if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many row blocks");
-  attention_forward_kernel<DP><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p, q_map, k_map, v_map);
-  MUP_HOST_CUDA(cudaGetLastError());
+  MUP_HOST_CUDA(launch_early(attention_forward_kernel<DP>, dim3(static_cast<unsigned>(grid)), Cfg::kThreads, Cfg::kSmemBytes, 1,
+                             stream, p, q_map, k_map, v_map));
   if (f.splits > 1) return launch_combine<DP>(a, p.partial_out, p.partial_lse, f.splits, stream);
   return MUP_OK;
 }
@@ -252,14 +237,8 @@ int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* 
   if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many sequences");
   static uint64_t ready = 0;
   MUP_HOST_CUDA(allow_smem_once(attention_tokens_kernel<DP>, Cfg::kSmemBytes, a.device, &ready));
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(grid)), config.blockDim = dim3(32 * kTokenWarps);
-  config.dynamicSmemBytes = Cfg::kSmemBytes, config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(plan.splits), attribute.val.clusterDim.y = 1, attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute, config.numAttrs = plan.cluster ? 1 : 0;
-  MUP_HOST_CUDA(cudaLaunchKernelEx(&config, attention_tokens_kernel<DP>, p));
+  MUP_HOST_CUDA(launch_early(attention_tokens_kernel<DP>, dim3(static_cast<unsigned>(grid)), 32 * kTokenWarps, Cfg::kSmemBytes,
+                             plan.cluster ? plan.splits : 1, stream, p));
   if (plan.splits > 1 && !plan.cluster) return launch_combine<DP>(a, p.partial_out, p.partial_lse, plan.splits, stream);
   return MUP_OK;
 }
@@ -354,12 +333,11 @@ int launch_backward(const mup_window_attention& a, cudaStream_t stream, uint32_t
   static uint64_t ready = 0;
   MUP_HOST_CUDA(allow_smem_once(attention_backward_kernel<DP>, smem, a.device, &ready));
   p.dkv_jobs = static_cast<int>(k_grid);
-  attention_delta_kernel<<<ceil_div(total_rows(a), 16 * kDeltaRows), 256, 0, stream>>>(d);
-  MUP_HOST_CUDA(cudaGetLastError());
-  MUP_HOST_CUDA(launch_early(attention_backward_kernel<DP>, k_grid + q_grid, 384, smem, stream, p, q_map, k_map, v_map, do_map));
+  MUP_HOST_CUDA(launch_early(attention_delta_kernel, ceil_div(total_rows(a), 16 * kDeltaRows), 256, 0, 1, stream, d));
+  MUP_HOST_CUDA(launch_early(attention_backward_kernel<DP>, dim3(static_cast<unsigned>(k_grid + q_grid)), 384, smem, 1, stream, p, q_map, k_map, v_map, do_map));
   if (plan.shared_tiles > 0) {
     const int64_t quads = static_cast<int64_t>(p.n_sequences) * a.heads_kv * plan.shared_tiles * 2 * kTileRows * (DP / 4);
-    MUP_HOST_CUDA(launch_early(attention_dkv_join_kernel<DP>, ceil_div(quads, 256), 256, 0, stream, p));
+    MUP_HOST_CUDA(launch_early(attention_dkv_join_kernel<DP>, ceil_div(quads, 256), 256, 0, 1, stream, p));
   }
   return MUP_OK;
 }

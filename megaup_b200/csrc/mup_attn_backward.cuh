@@ -48,6 +48,8 @@ __device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float sum) {
 constexpr int kDeltaRows = 4;  // of 16 lanes: all their loads are in flight at once; a warp's 8 rows follow each other
 
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ AttnDelta p) {
+  // the kernel after this one reads what the ones before it wrote as well: it may begin once those have ended
+  grid_dep_wait();
   grid_dep_launch();
   const int lane = threadIdx.x % 32, part = lane % 16;
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * 2 * kDeltaRows;

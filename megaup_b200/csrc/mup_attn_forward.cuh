@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(384, 1)
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
   grid_dep_launch();
+  grid_dep_wait();
   // The copies of this CTA, in the order of the products: for step i K of tile i, then V of the tile before it.
   const auto load_tile = [&](const ForwardBlock& block, const CUtensorMap& map, int kt, int s) {
     mbar_arrive_expect_tx(full(s), Cfg::kTileBytes);

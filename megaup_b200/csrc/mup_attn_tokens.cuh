@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps, kTokenCtas) attention_tokens
   w /= p.splits;
   const int kv_head = w % p.shape.heads_kv, sequence = w / p.shape.heads_kv;
   grid_dep_launch();
+  grid_dep_wait();
   const AttnSeq seq = load_sequence(p.shape, sequence);
   const int batch = p.shape.sequences != nullptr ? 0 : sequence;
   const int group = p.shape.heads_q / p.shape.heads_kv;

@@ -53,6 +53,32 @@ class DeviceScope {
   cudaError_t error_ = cudaSuccess;
 };
 
+// Whether kernels are launched so that they may begin while the kernel before them runs (MEGA_UP_PDL).
+bool early_launches();
+
+// A launch of that kind (`cluster` > 1: in clusters of so many CTAs). The kernel waits for the end of the one before
+// itself (grid_dep_wait) before it touches global memory that is not constant.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster,
+                                cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid, config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem), config.stream = stream;
+  cudaLaunchAttribute attributes[2]{};
+  config.attrs = attributes;
+  if (early_launches()) {
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    config.numAttrs = 1;
+  }
+  if (cluster > 1) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = static_cast<unsigned>(cluster), a.val.clusterDim.y = 1, a.val.clusterDim.z = 1;
+  }
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // Launch attributes of a kernel are set once per device; `mask` is the static
 // word of one kernel.
 template <typename Kernel>

@@ -115,6 +115,8 @@ constexpr int kResident = 2;  // blocks per SM
 template <bool INTERLEAVED, int SHARED>
 __global__ void __launch_bounds__(256, kResident) rotary_kernel(const __grid_constant__ RotaryParams p, int lanes) {
   constexpr int kPairs = INTERLEAVED ? 4 : 8;
+  grid_dep_launch();
+  grid_dep_wait();
   const int lane = threadIdx.x % 32;
   const int groups = 32 / lanes, group = lane / lanes, place = lane % lanes;
   const int column = place * 8;
@@ -194,7 +196,7 @@ int check_rows(const char* name, const void* base, const int64_t strides[3]) {
 
 constexpr unsigned kBlocks = 148 * kResident;
 
-void launch(RotaryParams& p, bool interleaved, cudaStream_t stream) {
+cudaError_t launch(RotaryParams& p, bool interleaved, cudaStream_t stream) {
   int lanes = 1;
   while (lanes * 8 < p.head_dim) lanes *= 2;
   const int per_group = (p.heads[0] + p.heads[1] + 32 / lanes - 1) / (32 / lanes);
@@ -208,7 +210,7 @@ void launch(RotaryParams& p, bool interleaved, cudaStream_t stream) {
     kernel = copies >= 4 ? rotary_kernel<true, 4> : copies == 2 ? rotary_kernel<true, 2> : rotary_kernel<true, 1>;
   else
     kernel = copies >= 8 ? rotary_kernel<false, 8> : copies == 4 ? rotary_kernel<false, 4> : rotary_kernel<false, 2>;
-  kernel<<<grid, 256, 0, stream>>>(p, lanes);
+  return launch_early(kernel, grid, 256, 0, 1, stream, p, lanes);
 }
 
 }  // namespace
@@ -254,7 +256,6 @@ extern "C" int mup_axial_rotary_launch(const mup_axial_rotary* args, void* strea
   DeviceScope scope(a.device);
   MUP_HOST_CUDA(scope.error());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  launch(p, a.interleaved != 0, s);
-  MUP_HOST_CUDA(cudaGetLastError());
+  MUP_HOST_CUDA(launch(p, a.interleaved != 0, s));
   return MUP_OK;
 }
