@@ -419,7 +419,8 @@ def window_attention_bshd(
     outside ``[0, Sk]`` counts as the nearer end. Slices of a fused projection may
     be passed as they are; ``D`` is a multiple of 8 up to 128. ``return_lse`` adds
     the FP32 ``[B,H,Sq]`` log-sum-exp of every row (no gradient flows through it).
-    Differentiable in ``q``, ``k`` and ``v``.
+    ``out`` is written instead of a new tensor; it may be ``q`` itself and overlaps
+    no other input. Differentiable in ``q``, ``k`` and ``v``.
     """
 
     return _attend("bshd", q, k, v, causal, window, sinks, scale, kv_lengths, None, out, return_lse)

@@ -110,6 +110,8 @@ bool few_rows(const mup_window_attention& a) {
 
 constexpr int kTokenShare = 2048;  // keys of a CTA (measured on 16 sequences of up to 65536 keys: 512 84 us, 1024 73, 2048 67)
 
+constexpr int kMostTokenCtas = 4096;  // bounds the workspace: 8 KB of a CTA
+
 struct TokenPlan {
   int splits, share;
   bool cluster;
@@ -134,7 +136,8 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   // Sequences of different lengths, cut for the longest: shares of one size, so that no CTA has more to do than others
   // and a short sequence leaves its last CTAs nothing.
   if (packed || a.kv_lengths != nullptr) {
-    t.splits = static_cast<int>(std::max<int64_t>(t.splits, std::min<int64_t>(visible / kTokenShare, kMostSplits)));
+    const int64_t bound = std::min<int64_t>(kMostSplits, kMostTokenCtas / places);
+    t.splits = static_cast<int>(std::max<int64_t>(t.splits, std::min<int64_t>(visible / kTokenShare, bound)));
     const int64_t steps = visible / kTokenStep + 2;  // the sinks' and the window's first steps may be cut
     t.share = ceil_div(ceil_div(steps, t.splits), kTokenWarps) * kTokenWarps;
   }
@@ -247,6 +250,7 @@ int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* 
 struct BackwardPlan {
   int shared_tiles, shares;
 };
+constexpr int64_t kMostSharedJobs = 1024;
 
 BackwardPlan plan_backward(const mup_window_attention& a) {
   const bool packed = a.sequences != nullptr;
@@ -260,16 +264,22 @@ BackwardPlan plan_backward(const mup_window_attention& a) {
   const int64_t window_rows =
       std::min(all_rows, static_cast<int64_t>(group) * (ceil_div(std::min<int64_t>(window, queries), kTileRows) + 1));
   // A sink's tile is seen by every later row, other tiles by a window's rows: it is cut into shares of about as many
-  // query tiles. Too few key tiles for the GPU: all of them are cut.
+  // query tiles. Too few key tiles for the GPU: all of them are cut. (Packed sequences that are shorter than the longest
+  // leave shares unused; their number is bounded, and with it the workspace: 128 KB a share.)
   const int64_t ctas = std::max<int64_t>(1, tiles * a.heads_kv);
+  const int64_t sequences = packed ? a.n_sequences : a.batch;
+  const auto bounded = [&](int64_t shares, int shared_tiles) {
+    return std::min(shares, kMostSharedJobs / std::max<int64_t>(1, sequences * a.heads_kv * shared_tiles));
+  };
   BackwardPlan b{};
   if (2 * ctas <= kSms) {
     b.shared_tiles = key_tiles;
-    b.shares = static_cast<int>(std::min<int64_t>(kSms / ctas, ceil_div(all_rows, 2)));
-  } else if (s.sinks > 0 && keys > 0) {
+    b.shares = static_cast<int>(bounded(std::min<int64_t>(kSms / ctas, ceil_div(all_rows, 2)), b.shared_tiles));
+  }
+  if (b.shares <= 1 && s.sinks > 0 && keys > 0) {
     const int64_t per_cta = std::max(window_rows, ctas * window_rows / (4 * kSms));
     b.shared_tiles = ceil_div(std::min(s.sinks, keys), kTileRows);
-    b.shares = static_cast<int>(std::min<int64_t>(64, ceil_div(all_rows, per_cta)));
+    b.shares = static_cast<int>(bounded(std::min<int64_t>(64, ceil_div(all_rows, per_cta)), b.shared_tiles));
   }
   if (b.shares <= 1 || keys == 0) b.shared_tiles = 0, b.shares = 1;
   return b;

@@ -351,6 +351,26 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
 // dK, dV
 // ---------------------------------------------------------------------------
 
+// The query tiles that see something of a key tile, times the heads of the group, and how they are cut into shares.
+struct KeyTileSteps {
+  int q_tile0, q_tiles, steps;
+  __device__ __forceinline__ KeyTileSteps(const AttnShape& p, const AttnSeq& seq, int tile) {
+    const int j0 = tile * kTileRows, j1 = min(j0 + kTileRows, seq.nk) - 1;
+    const bool has_sinks = j0 < p.sinks;
+    const int low = has_sinks ? (p.causal ? max(0, j0 - seq.off) : 0) : max(0, j0 - p.right - seq.off);
+    const int high = has_sinks ? seq.nq - 1 : min(seq.nq - 1, j1 + p.left - seq.off);
+    q_tile0 = low / kTileRows;
+    q_tiles = high < low ? 0 : high / kTileRows - q_tile0 + 1;
+    steps = q_tiles * (p.heads_q / p.heads_kv);
+  }
+  __device__ __forceinline__ int per_share(int shares) const { return (steps + shares - 1) / shares; }
+  // shares that have steps (the first one counts as such: it writes zeros where nothing sees the tile)
+  __device__ __forceinline__ int used(int shares) const {
+    const int each = per_share(shares);
+    return each == 0 ? 1 : (steps + each - 1) / each;
+  }
+};
+
 template <int DP>
 struct AttnDkvConfig {
   static constexpr int kPanels = DP / 64;
@@ -420,17 +440,12 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
   const int batch = p.shape.sequences != nullptr ? 0 : sequence;
   const int j0 = tile * kTileRows;
   if (j0 >= seq.nk) return;  // packed: a shared tile that this sequence does not have
-  // rows at `at` with at_low <= at <= at_high see something of the tile
   const bool has_sinks = j0 < p.shape.sinks;
-  int i_low = (has_sinks && !p.shape.causal ? 0 : max(0, j0 - p.shape.right - seq.off));
-  if (has_sinks && p.shape.causal) i_low = max(0, j0 - seq.off);
-  const int j1 = min(j0 + kTileRows, seq.nk) - 1;
-  const int i_high = has_sinks ? seq.nq - 1 : min(seq.nq - 1, j1 + p.shape.left - seq.off);
-  const int q_tile0 = i_low / kTileRows;
-  const int q_tiles = i_high < i_low ? 0 : i_high / kTileRows - q_tile0 + 1;
-  const int steps = q_tiles * group;
-  const int per_share = (steps + shares - 1) / shares;
-  const int begin = min(share * per_share, steps), n = min(begin + per_share, steps) - begin;
+  const KeyTileSteps work(p.shape, seq, tile);
+  const int q_tile0 = work.q_tile0, q_tiles = work.q_tiles;
+  const int per_share = work.per_share(shares);
+  const int begin = min(share * per_share, work.steps), n = min(begin + per_share, work.steps) - begin;
+  if (share > 0 && n == 0) return;  // (the joining kernel knows)
 
   if (threadIdx.x == 0) {
     *abort_flag = 0u;
@@ -766,7 +781,8 @@ __global__ void __launch_bounds__(256) attention_dkv_join_kernel(const __grid_co
   if (j >= seq.nk) return;
   const int64_t slot = ((static_cast<int64_t>(sequence) * p.shape.heads_kv + kv_head) * p.shared_tiles + tile) * p.shares;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = 0; s < p.shares; ++s) {
+  const int used = KeyTileSteps(p.shape, seq, tile).used(p.shares);
+  for (int s = 0; s < used; ++s) {
     const float4 v = *reinterpret_cast<const float4*>(p.partial + (((slot + s) * 2 + which) * kTileRows + r) * DP + quad * 4);
     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }

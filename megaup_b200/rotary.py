@@ -268,7 +268,7 @@ def axial_rotary_bshd(
 
     ``positions`` (int32, int64 or float32 on the device) are ``[axes,S]``, shared
     by the batch, or ``[axes,B,S]``. ``out``: tensors of the same shapes to write,
-    which may be the inputs themselves. Differentiable in ``q`` and ``k``.
+    which may be the inputs themselves (but not overlap them shifted). Differentiable in ``q`` and ``k``.
     """
 
     return _rotate("bshd", q, k, rotary, positions, out)

@@ -80,6 +80,23 @@ def test_workspace_sizes(library) -> None:
     assert few > 0 and few % (4 * (64 + 1)) == 0
 
 
+def test_the_workspace_is_bounded(library) -> None:
+    """Sequences of very different lengths are cut for the longest one: that may not cost memory for every short one."""
+
+    forward, backward = ctypes.c_uint64(), ctypes.c_uint64()
+    sequences, longest = 4000, 1 << 20
+    rows = sequences + longest
+    for sinks, left, longest_q in ((4, 127, longest), (4, 127, 1), (0, -1, 1), (300, 1023, 16)):
+        a = _block(
+            batch=1, seq_q=rows if longest_q > 16 else longest_q * sequences, seq_k=rows, left=left, sinks=sinks,
+            sequences=4096, n_sequences=sequences, n_q_blocks_256=sequences, n_q_blocks_128=2 * sequences + 8192,
+            n_k_blocks_128=sequences + 8192, longest_q=longest_q, longest_k=longest,
+        )
+        assert library.mup_window_attention_workspace(ctypes.byref(a), ctypes.byref(forward), ctypes.byref(backward)) == 0
+        per_row = 4 * 2 * 4 * a.seq_q
+        assert forward.value <= 1 << 28 and backward.value - per_row <= 1 << 28, (sinks, left, longest_q)
+
+
 def test_window_sides() -> None:
     assert module._window_sides(None, True) == (-1, 0)
     assert module._window_sides(None, False) == (-1, -1)
@@ -267,6 +284,74 @@ def test_packed_sequences(lengths_q, lengths_k, heads, kv_heads, dim, causal, le
         assert_within(grads[1][ks], e.dk, e.dk_error, "dk")
         assert_within(grads[2][ks], e.dv, e.dv_error, "dv")
         a, c = a + n, c + m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sinks", [4, 200])
+def test_one_long_sequence_among_many_short_ones(sinks) -> None:
+    lengths = [1 + i % 3 for i in range(300)] + [1500] + [1 + i % 5 for i in range(200)]
+    q, k, v, dout, sequences = _packed(lengths, lengths, 4, 2, 64, seed=11)
+    for x in (q, k, v):
+        x.requires_grad_()
+    out = mega_up.window_attention_thd(q, k, v, sequences, window=60, sinks=sinks)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    a = 0
+    for n in lengths:
+        rows = slice(a, a + n)
+        e = attention(q[rows], k[rows], v[rows], visible(n, n, causal=True, left=60, right=0, sinks=sinks), dout=dout[rows])
+        assert_within(out[rows], e.out, e.out_error, "out")
+        for got, want, error in zip(grads, (e.dq, e.dk, e.dv), (e.dq_error, e.dk_error, e.dv_error)):
+            assert_within(got[rows], want, error, "gradient")
+        a += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks,capacity", [(None, 0, 9000), (300, 4, 9000), (None, 0, 700)])
+def test_a_captured_token_over_a_growing_cache(window, sinks, capacity) -> None:
+    """One graph, replayed while the cache fills: the lengths and the new rows are read at every replay."""
+
+    batch, heads, kv_heads, dim = 3, 8, 2, 128
+    q = _normal((batch, 1, heads, dim), 1)
+    k, v = (torch.full((batch, capacity, kv_heads, dim), float("nan"), dtype=BF16, device=DEVICE) for _ in range(2))
+    lengths = torch.tensor([capacity - 400, 5, 300], dtype=torch.int32, device=DEVICE)
+    rows = [_normal((batch, capacity, kv_heads, dim), s) for s in (2, 3)]
+    for b, n in enumerate(lengths.tolist()):
+        k[b, :n], v[b, :n] = rows[0][b, :n], rows[1][b, :n]
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = mega_up.window_attention_bshd(q, k, v, window=window, sinks=sinks, kv_lengths=lengths)
+    for step in range(3):
+        for b, n in enumerate(lengths.tolist()):
+            k[b, n : n + 130], v[b, n : n + 130] = rows[0][b, n : n + 130], rows[1][b, n : n + 130]
+        lengths.add_(130)
+        q.copy_(_normal(q.shape, 20 + step))
+        graph.replay()
+        torch.cuda.synchronize()
+        for b, n in enumerate(lengths.tolist()):
+            e = attention(q[b], k[b, :n], v[b, :n], visible(1, n, causal=True, left=window, right=0, sinks=sinks))
+            assert_within(out[b], e.out, e.out_error, f"step {step}, length {n}")
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_and_out_in_place_of_q() -> None:
+    calls = []
+    for s, (queries, keys) in enumerate(((1, 5000), (200, 5000), (2000, 2000), (7, 640))):
+        q, k, v = _normal((1, queries, 4, 128), s), _normal((1, keys, 2, 128), 10 + s), _normal((1, keys, 2, 128), 20 + s)
+        calls.append((q, k, v, mega_up.window_attention_bshd(q, k, v, window=1000, sinks=2)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    results = [[] for _ in calls]
+    for _ in range(10):
+        for (q, k, v, _), stream, kept in zip(calls, streams, results):
+            with torch.cuda.stream(stream):
+                kept.append(mega_up.window_attention_bshd(q, k, v, window=1000, sinks=2))
+    torch.cuda.synchronize()
+    for (q, k, v, want), kept in zip(calls, results):
+        assert all(torch.equal(want, x) for x in kept)
+        own = q.clone()
+        assert torch.equal(mega_up.window_attention_bshd(own, k, v, window=1000, sinks=2, out=own), want)
 
 
 @pytest.mark.gpu
