@@ -181,6 +181,9 @@ CASES = [
     ("bshd", 1, 640, 640, 2, 1, 72, True, 127, 0, 1000),  # more sinks than keys
     ("bshd", 1, 1000, 1000, 4, 2, 128, True, 1 << 40, 0, 0),
     ("sbhd", 2, 700, 700, 2, 1, 120, False, 130, 5, 129),
+    ("bshd", 2, 1, 300, 128, 1, 64, True, None, 0, 0),  # a group as large as a tile
+    ("sbhd", 1, 3, 400, 48, 2, 128, True, 150, 0, 9),  # 24 heads of a group, packed by eight
+    ("bshd", 1, 20, 2500, 6, 2, 128, False, 700, 0, 1),
 ]
 
 
