@@ -28,6 +28,8 @@ import array
 import ctypes
 from collections.abc import Sequence
 from dataclasses import dataclass, field
+from itertools import chain
+from operator import itemgetter
 
 import torch
 from torch import Tensor
@@ -68,14 +70,14 @@ class PackedSequences:
         return self.sequences.device
 
 
-def _blocks(table: list[tuple[int, int, int, int]], lengths: list[int], rows: int) -> list[tuple[int, ...]]:
-    """(sequence, first row, the sequence's entry of ``table``) of every block of
-    ``rows`` rows, the last rows first: under a causal mask they have the most keys."""
+def _blocks(table: list[tuple[int, int, int, int]], lengths: list[int]) -> list[tuple[int, ...]]:
+    """(sequence, first row, the sequence's entry of ``table``, 0, 0) of every block of
+    128 rows, the last rows first: under a causal mask they have the most keys."""
 
     blocks = [
-        (s, r, *entry, 0, 0) for s, (entry, length) in enumerate(zip(table, lengths)) for r in range(0, length, rows)
+        (s, r, *entry, 0, 0) for s, (entry, length) in enumerate(zip(table, lengths)) for r in range(0, length, 128)
     ]
-    blocks.sort(key=lambda block: -block[1])
+    blocks.sort(key=itemgetter(1), reverse=True)
     return blocks
 
 
@@ -103,13 +105,14 @@ def prepare_packed_sequences(
     table = [(a, n, b, m) for a, n, b, m in zip(cu_q, queries, cu_k, keys)]
 
     # one copy to the device; entries of 8 numbers start at multiples of 32 bytes
+    q_blocks = _blocks(table, queries)
     parts = {
-        "q_blocks_256": _blocks(table, queries, 256),
-        "q_blocks_128": _blocks(table, queries, 128),
-        "k_blocks_128": _blocks(table, keys, 128)[::-1],
+        "q_blocks_256": [block for block in q_blocks if block[1] % 256 == 0],
+        "q_blocks_128": q_blocks,
+        "k_blocks_128": (q_blocks if keys == queries else _blocks(table, keys))[::-1],
         "sequences": table,
     }
-    flat = array.array("i", (v for rows in parts.values() for row in rows for v in row))
+    flat = array.array("i", chain.from_iterable(chain.from_iterable(parts.values())))
     everything = torch.frombuffer(flat, dtype=torch.int32).to(device, copy=True)
     tables, start = {}, 0
     for name, rows in parts.items():
