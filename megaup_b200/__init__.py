@@ -1,6 +1,6 @@
 """B200-native fused GEMM + Ulysses all-to-all operators behind the ``mega_up`` API.
 
-Two operators, forward only, BF16 in / FP32 accumulate / one rounding to BF16,
+Two exchange operators, forward only, BF16 in / FP32 accumulate / one rounding to BF16,
 one node, ``UP`` in {2, 4, 8}:
 
 * peer-write GEMM - ``x @ W.T + b`` whose epilogue stores every head shard
@@ -9,6 +9,10 @@ one node, ``UP`` in {2, 4, 8}:
 * head-shard pull GEMM - pull warps gather every peer's head shard of each row
   while the MMA warps consume finished panels (replaces all_to_all + permute +
   linear).
+
+Between the two, on the tensors they exchange: rotary positions with several
+axes (``axial_rotary_*``) and sliding-window attention with sinks
+(``window_attention_*``), both with their gradients.
 
 The device code is hand-written sm_100a CUDA in ``libmegaup.so`` (C ABI in
 ``include/megaup.h``); this package is the host side.

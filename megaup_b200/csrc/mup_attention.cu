@@ -98,11 +98,13 @@ ForwardPlan plan_forward(const mup_window_attention& a) {
   const int tiles = std::max(1, std::min(ceil_div(keys, kTileRows),
                                          ceil_div(std::min<int64_t>(window, keys), kTileRows) + 1 + ceil_div(std::min(s.sinks, keys), kTileRows)));
   const int64_t ctas = static_cast<int64_t>(f.blocks) * f.head_sets;
-  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms / std::max<int64_t>(ctas, 1), ceil_div(tiles, 2))));
+  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms / std::max<int64_t>(ctas, 1), tiles)));
   return f;
 }
 
-// Few query rows: the kernel for tokens over a cache.
+// Few query rows: the kernel for tokens over a cache. Measured, few rows' kernel / 128-row kernel, 8 rows: 256 keys 5.7 /
+// 8.5 us, 4096 7.4 / 10.6, 65536 18.8 / 18.3, 16 sequences of 4096 16.0 / 16.4, 64 of them 36.4 / 34.6; 16 rows, 4096
+// keys: 7.5 / 9.7. It has one row tile: above 16 rows it would read the cache again for each.
 bool few_rows(const mup_window_attention& a) {
   const int queries = a.sequences != nullptr ? a.longest_q : a.seq_q;
   return static_cast<int64_t>(a.heads_q / a.heads_kv) * queries <= kTokenRows;
@@ -127,7 +129,9 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenStep * kTokenWarps));
   const int64_t fill = std::max<int64_t>(1, kTokenCtas * kSms / places);
   TokenPlan t{};
-  if (most <= 4 * kTokenCluster) {  // short: a second launch would cost more than it gains
+  // Short: joined within a cluster, without a workspace and a second launch. Measured with 8 heads over 256 / 1024 / 2000
+  // keys: 5.7 / 7.7 / 10.0 us on the GPU (two launches 6.2 / 6.5 / 7.8), but 11 us of host time a call instead of 15.
+  if (most <= 4 * kTokenCluster) {
     t.splits = static_cast<int>(std::min<int64_t>({most, fill, kTokenCluster}));
     t.cluster = t.splits > 1;
     return t;
@@ -180,7 +184,10 @@ int launch_combine(const mup_window_attention& a, const float* partial_out, cons
   c.head_dim = a.head_dim, c.heads_q = a.heads_q, c.seq_q = a.seq_q, c.total_rows = total_rows(a);
   c.out = static_cast<__nv_bfloat16*>(a.out), c.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   c.out_batch = a.out_strides[0], c.out_seq = a.out_strides[1], c.out_head = a.out_strides[2], c.lse = a.lse;
-  MUP_HOST_CUDA(launch_early(attention_combine_kernel<DP>, dim3(static_cast<unsigned>(c.total_rows)), 128, 0, 1, stream, c));
+  // Few rows with many parts want more threads a row (8 rows of 296 parts: 11 us with 128 threads, 3 us with 512).
+  const bool wide = splits > 48;
+  MUP_HOST_CUDA(launch_early(wide ? attention_combine_kernel<DP, 512> : attention_combine_kernel<DP, 128>,
+                             dim3(static_cast<unsigned>(c.total_rows)), wide ? 512 : 128, 0, 1, stream, c));
   return MUP_OK;
 }
 

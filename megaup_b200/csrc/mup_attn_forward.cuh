@@ -473,8 +473,8 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
-// Joins the partial results of `splits` CTAs per row, always in the same order: a block per row, 128 / (DP / 4) threads
-// per four columns, each with every so-many-th split.
+// Joins the partial results of `splits` CTAs per row, always in the same order: a block per row, THREADS / (DP / 4)
+// threads per four columns, each with every so-many-th split.
 struct AttnCombine {
   const float* partial_out;
   const float* partial_lse;
@@ -486,17 +486,17 @@ struct AttnCombine {
 };
 constexpr int kMostSplits = 512;
 
-template <int DP>
-__global__ void __launch_bounds__(128) attention_combine_kernel(const __grid_constant__ AttnCombine p) {
-  constexpr int kQuads = DP / 4, kLanes = 128 / kQuads;
+template <int DP, int THREADS>
+__global__ void __launch_bounds__(THREADS) attention_combine_kernel(const __grid_constant__ AttnCombine p) {
+  constexpr int kQuads = DP / 4, kLanes = THREADS / kQuads, kWarps = THREADS / 32;
   __shared__ float weight[kMostSplits];
-  __shared__ float warp_top[4], warp_sum[4];
+  __shared__ float warp_top[kWarps], warp_sum[kWarps];
   __shared__ float4 shared_acc[kLanes][kQuads];
   const int64_t row = blockIdx.x;
   const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32;
   grid_dep_wait();  // the partial results are there
   float top = -INFINITY;
-  for (int s = thread; s < p.splits; s += 128) {
+  for (int s = thread; s < p.splits; s += THREADS) {
     const float l = p.partial_lse[s * p.total_rows + row];
     weight[s] = l;
     top = fmaxf(top, l);
@@ -505,9 +505,10 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const __grid_con
   for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (lane == 0) warp_top[warp] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_top[w]);
   float sum = 0.0f;
-  for (int s = thread; s < p.splits; s += 128) {
+  for (int s = thread; s < p.splits; s += THREADS) {
     const float l = weight[s];
     weight[s] = l == -INFINITY ? 0.0f : exp2_sfu(l - top);
     sum += weight[s];
@@ -516,7 +517,9 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const __grid_con
   for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) warp_sum[warp] = sum;
   __syncthreads();
-  sum = (warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]);
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += warp_sum[w];
   const int quad = thread % kQuads, part = thread / kQuads;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const float4* src = reinterpret_cast<const float4*>(p.partial_out + row * DP) + quad;
