@@ -103,14 +103,16 @@ ForwardPlan plan_forward(const mup_window_attention& a) {
 }
 
 // Few query rows: the kernel for tokens over a cache. Measured, few rows' kernel / 128-row kernel, 8 rows: 256 keys 5.7 /
-// 8.5 us, 4096 7.4 / 10.6, 65536 18.8 / 18.3, 16 sequences of 4096 16.0 / 16.4, 64 of them 36.4 / 34.6; 16 rows, 4096
-// keys: 7.5 / 9.7. It has one row tile: above 16 rows it would read the cache again for each.
+// 8.5 us, 4096 6.9 / 10.6, 65536 13.4 / 18.3, 16 sequences of 4096 11.4 / 16.4, 64 of them 28.1 / 34.6; 16 rows, 4096
+// keys: 7.3 / 9.7. It has one row tile: above 16 rows it would read the cache again for each.
 bool few_rows(const mup_window_attention& a) {
   const int queries = a.sequences != nullptr ? a.longest_q : a.seq_q;
   return static_cast<int64_t>(a.heads_q / a.heads_kv) * queries <= kTokenRows;
 }
 
-constexpr int kTokenShare = 2048;  // keys of a CTA (measured on 16 sequences of up to 65536 keys: 512 84 us, 1024 73, 2048 67)
+// Keys of a CTA where lengths differ. Measured on 16 sequences of 8192 to 65536 keys (308 MB): 1024 56.9 us, 2048 67.8 (as
+// many CTAs as places, some with less to do), 4096 55.3; smaller shares spread one long sequence among short ones better.
+constexpr int kTokenShare = 1024;
 
 constexpr int kMostTokenCtas = 4096;  // bounds the workspace: 8 KB of a CTA
 
@@ -126,11 +128,11 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   const int64_t window = std::min<int64_t>(static_cast<int64_t>(s.left) + s.right + queries, keys);
   const int64_t visible = std::min<int64_t>(keys, window + s.sinks);
   const int64_t places = static_cast<int64_t>(packed ? a.n_sequences : a.batch) * a.heads_kv;
-  const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenStep * kTokenWarps));
+  const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenKeys));
   const int64_t fill = std::max<int64_t>(1, kTokenCtas * kSms / places);
   TokenPlan t{};
   // Short: joined within a cluster, without a workspace and a second launch. Measured with 8 heads over 256 / 1024 / 2000
-  // keys: 5.7 / 7.7 / 10.0 us on the GPU (two launches 6.2 / 6.5 / 7.8), but 11 us of host time a call instead of 15.
+  // keys: 5.7 / 7.2 / 8.3 us on the GPU (two launches about 6.2 / 6.5 / 7.0), but 11 us of host time a call instead of 15.
   if (most <= 4 * kTokenCluster) {
     t.splits = static_cast<int>(std::min<int64_t>({most, fill, kTokenCluster}));
     t.cluster = t.splits > 1;
@@ -142,8 +144,7 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   if (packed || a.kv_lengths != nullptr) {
     const int64_t bound = std::min<int64_t>(kMostSplits, kMostTokenCtas / places);
     t.splits = static_cast<int>(std::max<int64_t>(t.splits, std::min<int64_t>(visible / kTokenShare, bound)));
-    const int64_t steps = visible / kTokenStep + 2;  // the sinks' and the window's first steps may be cut
-    t.share = ceil_div(ceil_div(steps, t.splits), kTokenWarps) * kTokenWarps;
+    t.share = ceil_div(visible / kTokenKeys + 3, t.splits);  // the sinks' and the window's tiles may be cut at their ends
   }
   return t;
 }
@@ -228,14 +229,15 @@ int launch_forward(const mup_window_attention& a, cudaStream_t stream, uint32_t*
 template <int DP>
 int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* status) {
   const TokenPlan plan = plan_tokens(a);
+  CUtensorMap k_map, v_map;
+  int rc = encode_rows(&k_map, a, a.k, a.k_strides, a.seq_k, a.heads_kv, kTokenKeys, 1);
+  if (rc == MUP_OK) rc = encode_rows(&v_map, a, a.v, a.v_strides, a.seq_k, a.heads_kv, kTokenKeys, 1);
+  if (rc != MUP_OK) return rc;
   AttnTokens p{};
   p.shape = make_shape(a, status);
-  p.q = static_cast<const __nv_bfloat16*>(a.q), p.k = static_cast<const __nv_bfloat16*>(a.k);
-  p.v = static_cast<const __nv_bfloat16*>(a.v);
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.out = static_cast<__nv_bfloat16*>(a.out), p.out_rest = static_cast<__nv_bfloat16*>(a.out_rest);
   p.q_batch = a.q_strides[0], p.q_seq = a.q_strides[1], p.q_head = a.q_strides[2];
-  p.k_batch = a.k_strides[0], p.k_seq = a.k_strides[1], p.k_head = a.k_strides[2];
-  p.v_batch = a.v_strides[0], p.v_seq = a.v_strides[1], p.v_head = a.v_strides[2];
   p.out_batch = a.out_strides[0], p.out_seq = a.out_strides[1], p.out_head = a.out_strides[2];
   p.lse = a.lse;
   p.splits = plan.splits, p.share = plan.share, p.cluster = plan.cluster;
@@ -247,8 +249,8 @@ int launch_tokens(const mup_window_attention& a, cudaStream_t stream, uint32_t* 
   if (grid > 0x7fffffff) return host_fail(MUP_ERR_UNSUPPORTED, "window attention: too many sequences");
   static uint64_t ready = 0;
   MUP_HOST_CUDA(allow_smem_once(attention_tokens_kernel<DP>, Cfg::kSmemBytes, a.device, &ready));
-  MUP_HOST_CUDA(launch_early(attention_tokens_kernel<DP>, dim3(static_cast<unsigned>(grid)), 32 * kTokenWarps, Cfg::kSmemBytes,
-                             plan.cluster ? plan.splits : 1, stream, p));
+  MUP_HOST_CUDA(launch_early(attention_tokens_kernel<DP>, dim3(static_cast<unsigned>(grid)), Cfg::kThreads, Cfg::kSmemBytes,
+                             plan.cluster ? plan.splits : 1, stream, p, k_map, v_map));
   if (plan.splits > 1 && !plan.cluster) return launch_combine<DP>(a, p.partial_out, p.partial_lse, plan.splits, stream);
   return MUP_OK;
 }
