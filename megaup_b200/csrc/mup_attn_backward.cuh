@@ -1,10 +1,13 @@
 // Backward pass of the sliding-window attention with sinks. With P = exp(S - lse) and delta = rowsum(dO * O):
 //     dP = dO V^T,  dS = P (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
 //
-// Two kernels recompute S and dP: one walks the key tiles of a block of query rows and sums dQ, one walks the query
-// tiles of a block of key rows (over all heads of the group) and sums dK and dV. That is seven products per pair of
-// tiles where a single kernel with a shared dQ would need five, but every sum stays in one CTA's TMEM: no atomics, no
-// FP32 gradient in memory, the same bits every time.
+// One launch of two kinds of CTAs, which both recompute S and dP: one walks the key tiles of a block of query rows and sums
+// dQ, one walks the query tiles of a block of key rows (over all heads of the group) and sums dK and dV. That is seven
+// products per pair of tiles where CTAs that share dQ would need five, but every sum stays in one CTA's TMEM: no atomics,
+// no FP32 gradient in memory, the same bits every time.
+//
+// Bound by the board's power on long sequences: 65536 rows, window 4096, 4 heads of one group, 128 wide take 1632 us in
+// one launch (two launches 1770: the first one's last wave left SMs idle), seven products at 1.14 PFLOP/s.
 #pragma once
 
 #include "mup_attn_common.cuh"
@@ -28,7 +31,7 @@ struct AttnBackward {
 };
 
 // ---------------------------------------------------------------------------
-// delta and the base-2 log-sum-exp of every row: 16 lanes per row.
+// delta and the base-2 log-sum-exp of every row: 16 lanes per row. Bound by memory: O, its rest and dO are read once.
 // ---------------------------------------------------------------------------
 
 struct AttnDelta {
