@@ -33,6 +33,7 @@ from operator import itemgetter
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .ops import _INPUT_LABEL, _normalize_cu_seqlens, _tensor_signature
@@ -60,6 +61,9 @@ class PackedSequences:
     longest_q: int
     longest_k: int
     plans: dict = field(default_factory=dict, init=False, repr=False, compare=False)
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "plans": {}}  # a copy has its own tables: kept plans know these ones' addresses
 
     @property
     def num_sequences(self) -> int:
@@ -223,10 +227,10 @@ class _Plan:
                 )
         if not isinstance(sinks, int) or isinstance(sinks, bool) or sinks < 0:
             raise ValueError(f"sinks must be a non-negative int, got {sinks!r}")
-        scale = head_dim**-0.5 if scale is None else float(scale)
+        scale = head_dim**-0.5 if scale is None else scale
         if not 0.0 < scale <= 1e30:
             raise ValueError(f"scale must be positive and finite, got {scale}")
-        left, right = _window_sides(window, bool(causal))
+        left, right = _window_sides(window, causal)
         if sequences is not None:
             if sequences.device != q.device:
                 raise ValueError(f"sequences live on {sequences.device}, q on {q.device}")
@@ -334,6 +338,7 @@ def _forward(
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         a.out_strides = _stride_array(out.shape, out.stride(), plan.kind)
+        increment_version(out)  # autograd refuses a graph that had saved it
     a.out = out.data_ptr()
     lse = None
     if need_lse:
@@ -382,6 +387,8 @@ def _attend(
     kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
     kv_lengths: Tensor | None, sequences: PackedSequences | None, out: Tensor | None, return_lse: bool,
 ):
+    # plans are kept by these values: no object that can change (a tensor of one number) stands for them
+    causal, scale = bool(causal), None if scale is None else float(scale)
     plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences, kv_lengths is not None)
     if kv_lengths is not None:
         _check_kv_lengths(kv_lengths, q, kind)

@@ -23,6 +23,7 @@ from dataclasses import dataclass, field
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .attention import _AXES, _check_heads_tensor, _dense_strides, _row_strides, _rows_are_loadable, _strides_are_loadable
@@ -43,6 +44,9 @@ class AxialRotary:
     turns: Tensor
     pair_axis: Tensor
     plans: dict = field(default_factory=dict, init=False, repr=False, compare=False)
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "plans": {}}  # a copy has its own tables: kept blocks know these ones' addresses
 
     @property
     def pairs(self) -> int:
@@ -251,6 +255,7 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
         else:
             _check_outputs(out, tensors)
             outputs = out
+            increment_version(outputs)  # autograd refuses a graph that had saved them
         _turn(block, kind, tensors, outputs, positions, False, dense=out is None)
     return outputs[0], outputs[1] if k is not None else None
 
@@ -267,8 +272,8 @@ def axial_rotary_bshd(
     returns both.
 
     ``positions`` (int32, int64 or float32 on the device) are ``[axes,S]``, shared
-    by the batch, or ``[axes,B,S]``. ``out``: tensors of the same shapes to write,
-    which may be the inputs themselves (but not overlap them shifted). Differentiable in ``q`` and ``k``.
+    by the batch, or ``[axes,B,S]``. ``out``: tensors of the same shapes to write;
+    each may be its own input and overlaps no input otherwise. Differentiable in ``q`` and ``k``.
     """
 
     return _rotate("bshd", q, k, rotary, positions, out)

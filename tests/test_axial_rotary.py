@@ -2,8 +2,10 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -279,3 +281,32 @@ def test_refusals() -> None:
     leaf = q.clone().requires_grad_()
     with pytest.raises(ValueError, match="gradient"):
         call(leaf, k, rotary, positions, out=(torch.empty_like(q), torch.empty_like(k)))
+
+
+def test_copies_keep_no_plan() -> None:
+    """Plans know the addresses of the tables: a copy, which has tables of its own, must not use them."""
+
+    rotary = mega_up.prepare_axial_rotary([8, 4, 4], device="cpu")
+    rotary.plans["some call"] = object()
+    for other in (copy.copy(rotary), copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
+        assert other.plans == {} and other.axis_dims == (8, 4, 4) and other.pairs == 8
+        assert torch.equal(other.turns, rotary.turns) and torch.equal(other.pair_axis, rotary.pair_axis)
+        assert other.turns.data_ptr() % 8 == 0
+    assert rotary.plans
+
+
+@pytest.mark.gpu
+def test_a_copy_outlives_its_original() -> None:
+    rotary = mega_up.prepare_axial_rotary([32, 16, 16], device=DEVICE)
+    q = torch.randn(30, 2, 64, device=DEVICE).to(BF16)
+    positions = torch.arange(90, device=DEVICE).view(3, 30)
+    want, _ = mega_up.axial_rotary_thd(q, None, rotary, positions)
+    other = copy.deepcopy(rotary)
+    rotary.turns.zero_()  # no turn at all where it is used by mistake
+    assert torch.equal(mega_up.axial_rotary_thd(q, None, other, positions)[0], want)
+    loss = (q.float().requires_grad_() * 2).to(BF16)
+    saved = loss.square().sum()
+    with torch.no_grad():
+        mega_up.axial_rotary_thd(loss, None, other, positions, out=(loss,))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -556,3 +558,46 @@ def test_scale_is_used() -> None:
     e = attention(q[0], k[0], v[0], visible(100, 100, causal=True, left=None, right=0, sinks=0), scale=0.5)
     assert_within(out[0], e.out, e.out_error, "out")
     assert e.out_error.max() < 32 * HALF_BF16
+
+
+def test_copies_of_packed_sequences_keep_no_plan() -> None:
+    """Plans know the addresses of the tables: a copy, which has tables of its own, must not use them."""
+
+    sequences = mega_up.prepare_packed_sequences([0, 5, 300], device="cpu")
+    sequences.plans["some call"] = object()
+    for other in (copy.copy(sequences), copy.deepcopy(sequences), pickle.loads(pickle.dumps(sequences))):
+        assert other.plans == {} and other.cu_seqlens_q == (0, 5, 300) and other.longest_k == 295
+        assert torch.equal(other.q_blocks_128, sequences.q_blocks_128) and other.q_blocks_128.data_ptr() % 16 == 0
+    assert sequences.plans
+
+
+@pytest.mark.gpu
+def test_a_copied_description_outlives_its_original() -> None:
+    lengths = [130, 300]
+    q, k, v, _, sequences = _packed(lengths, lengths, 4, 2, 64, seed=3)
+    want = mega_up.window_attention_thd(q, k, v, sequences, window=40)
+    other = copy.deepcopy(sequences)
+    for table in (sequences.sequences, sequences.q_blocks_256, sequences.q_blocks_128, sequences.k_blocks_128):
+        table.zero_()  # blocks without rows or keys: harmless where they are used by mistake
+    assert torch.equal(mega_up.window_attention_thd(q, k, v, other, window=40), want)
+
+
+@pytest.mark.gpu
+def test_a_scale_that_changes_in_place() -> None:
+    q, k, v = (_normal((1, 50, 2, 64), s) for s in (1, 2, 3))
+    scale, causal = torch.tensor(0.125), torch.tensor(True)
+    for value, flag in ((0.125, True), (0.5, True), (0.5, False)):
+        scale.fill_(value), causal.fill_(flag)
+        want = mega_up.window_attention_bshd(q, k, v, scale=value, causal=flag)
+        assert torch.equal(mega_up.window_attention_bshd(q, k, v, scale=scale, causal=causal), want)
+
+
+@pytest.mark.gpu
+def test_a_result_written_over_a_saved_tensor() -> None:
+    x, k, v = (_normal((1, 20, 2, 64), s) for s in (1, 2, 3))
+    q = x.requires_grad_() * 2
+    loss = q.square().sum()
+    with torch.no_grad():
+        mega_up.window_attention_bshd(q, k, v, out=q)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
