@@ -222,7 +222,9 @@ def check(function: str, code: int) -> None:
 def call(function: str, *args: object) -> None:
     """Call an int-returning entry point and raise on a negative code."""
 
-    check(function, getattr(lib(), function)(*args))
+    code = getattr(_LIB or lib(), function)(*args)
+    if code != MUP_OK:
+        check(function, code)
 
 
 def pointer_array(addresses: list[int] | tuple[int, ...]) -> ctypes.Array:

@@ -151,7 +151,13 @@ def _strides_are_loadable(tensor: Tensor) -> bool:
 
 
 def _rows_are_loadable(tensor: Tensor) -> bool:
-    return tensor.data_ptr() % 16 == 0 and _strides_are_loadable(tensor)
+    return tensor.data_ptr() % 16 == 0 and (tensor.is_contiguous() or _strides_are_loadable(tensor))
+
+
+def _current_stream(device: int) -> int:
+    """The stream's handle. (``torch.cuda.current_stream`` makes an object of it: 1.3 us of a short call's 11.)"""
+
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _dense_strides(shape: Sequence[int]) -> list[int]:
@@ -195,7 +201,7 @@ class _Plan:
     """The checks and the host arithmetic of a call, kept per set of shapes, strides
     and settings: the argument block without addresses, and the workspace sizes."""
 
-    __slots__ = ("kind", "block", "lse_shape", "forward_bytes", "backward_bytes", "device", "tables")
+    __slots__ = ("kind", "block", "lse_shape", "forward_bytes", "backward_bytes", "tables")
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
@@ -262,7 +268,7 @@ class _Plan:
             "mup_window_attention_workspace", ctypes.byref(a), ctypes.byref(forward), ctypes.byref(backward)
         )
         a.kv_lengths = None
-        self.kind, self.block, self.device = kind, bytes(a), q.device
+        self.kind, self.block = kind, bytes(a)
         # a plan that a backward pass still holds keeps the tables whose addresses it knows
         self.tables = None if sequences is None else (
             sequences.sequences, sequences.q_blocks_256, sequences.q_blocks_128, sequences.k_blocks_128,
@@ -277,14 +283,14 @@ class _Plan:
             raise ValueError(f"q, k and v must be 16-byte aligned, got addresses {[hex(x) for x in addresses]}")
         return a
 
-    def launch(self, function: str, a: _native.MupWindowAttention, workspace_bytes: int) -> None:
-        """On the current stream of the tensors' device."""
+    def launch(self, function: str, a: _native.MupWindowAttention, workspace_bytes: int, q: Tensor) -> None:
+        """On the current stream of the device of ``q``."""
 
         if workspace_bytes:
             # freed with this frame: the allocator hands it out again in stream order
-            workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)
+            workspace = q.new_empty(workspace_bytes, dtype=torch.uint8)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace_bytes
-        _native.call(function, ctypes.byref(a), torch.cuda.current_stream(self.device.index).cuda_stream)
+        _native.call(function, ctypes.byref(a), _current_stream(a.device))
 
 
 _PLANS: dict[object, _Plan] = {}
@@ -342,13 +348,13 @@ def _forward(
     a.out = out.data_ptr()
     lse = None
     if need_lse:
-        lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=plan.device)
+        lse = q.new_empty(plan.lse_shape, dtype=torch.float32)
         a.lse = lse.data_ptr()
     if kv_lengths is not None:
         a.kv_lengths = kv_lengths.data_ptr()
     if rest is not None:
         a.out_rest = rest.data_ptr()
-    plan.launch("mup_window_attention_forward", a, plan.forward_bytes)
+    plan.launch("mup_window_attention_forward", a, plan.forward_bytes, q)
     return out, lse
 
 
@@ -379,7 +385,7 @@ class _WindowAttention(torch.autograd.Function):
         dq, dk, dv = grads = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v)]
         a.out, a.out_rest, a.lse, a.dout = out.data_ptr(), rest.data_ptr(), lse.data_ptr(), dout.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        plan.launch("mup_window_attention_backward", a, plan.backward_bytes)
+        plan.launch("mup_window_attention_backward", a, plan.backward_bytes, q)
         return (*grads, None)
 
 

@@ -26,7 +26,9 @@ from torch import Tensor
 from torch.autograd.graph import increment_version
 
 from . import _native
-from .attention import _AXES, _check_heads_tensor, _dense_strides, _row_strides, _rows_are_loadable, _strides_are_loadable
+from .attention import (
+    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _row_strides, _rows_are_loadable, _strides_are_loadable,
+)
 from .ops import _tensor_signature
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -181,8 +183,7 @@ def _turn(
     *, dense: bool = True,
 ) -> None:
     a = _native.MupAxialRotary.from_buffer_copy(block)
-    x = tensors[0]
-    a.q, a.q_out = address, _ = x.data_ptr(), outputs[0].data_ptr()
+    a.q, a.q_out = address, _ = tensors[0].data_ptr(), outputs[0].data_ptr()
     if len(tensors) == 2:
         a.k, a.k_out = other, _ = tensors[1].data_ptr(), outputs[1].data_ptr()
         address |= other
@@ -191,7 +192,7 @@ def _turn(
     if not dense:
         a.y_strides[: 3 * len(outputs)] = [s for t in outputs for s in _row_strides(t.shape, t.stride(), kind)]
     a.positions, a.inverse = positions.data_ptr(), inverse
-    _native.call("mup_axial_rotary_launch", ctypes.byref(a), torch.cuda.current_stream(x.get_device()).cuda_stream)
+    _native.call("mup_axial_rotary_launch", ctypes.byref(a), _current_stream(a.device))
 
 
 def _fresh(tensors: Sequence[Tensor]) -> list[Tensor]:
