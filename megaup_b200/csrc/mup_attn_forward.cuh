@@ -44,8 +44,8 @@ struct AttnForwardConfig {
   static constexpr int kOffQ = 0;
   static constexpr int kOffStages = 2 * kTileBytes;
   static constexpr int kOffBars = kOffStages + kStages * kTileBytes;
-  // q full [2], stage full, stage empty, s full [2], half of p full [2][2], done [2], drain [2]
-  static constexpr int kBars = 2 + 2 * kStages + 8 + 2;
+  // q full [2], stage full, stage empty, s full [2], half of p full [2][2], done [2], drain [2], started
+  static constexpr int kBars = 2 + 2 * kStages + 8 + 2 + 1;
   static constexpr int kOffWords = kOffBars + kBars * 8;
   static constexpr int kSmemBytes = kOffWords + 16;
   static constexpr int kThreads = 384;
@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(384, 1)
   const auto p_full = [&](int t, int half) { return bar(4 + 2 * Cfg::kStages + 2 * t + half); };
   const auto done = [&](int t) { return bar(8 + 2 * Cfg::kStages + t); };
   const auto drain = [&](int t) { return bar(10 + 2 * Cfg::kStages + t); };
+  const uint32_t started = bar(12 + 2 * Cfg::kStages);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(384, 1)
         mbar_init(full(s), 1);
         mbar_init(empty(s), users);
       }
+      mbar_init(started, 1);
       for (int t = 0; t < 2; ++t) {
         mbar_init(q_full(t), 1);
         mbar_init(drain(t), 1);
@@ -245,9 +247,9 @@ __global__ void __launch_bounds__(384, 1)
             ok = ok && ctl.wait(q_full(t), 0, MUP_ST_MMA_FULL_TIMEOUT);
             // Behind the first sub-tile's first product: the one's exponentials then run beside the other's products, and
             // both stay so (3030 cycles a step). Started together they stay together for ten steps and more, at 4700 to
-            // 5800 cycles a step.
+            // 5800 cycles a step. (A barrier of its own with one phase: this warp may look late, when s_full is phases on.)
             if (t == 1 && i == begin && block.exists(p, 0) && sees_tile(block.tiles(p, 0), all.tile(i)))
-              ok = ok && ctl.wait(s_full(0), 0, MUP_ST_MMA_ACC_TIMEOUT);
+              ok = ok && ctl.wait(started, 0, MUP_ST_MMA_ACC_TIMEOUT);
           }
         }
         if (ok && i > begin) {
@@ -284,6 +286,7 @@ __global__ void __launch_bounds__(384, 1)
             umma_rows_by_rows<DP>(s_tmem, q_tile, base + Cfg::kOffStages + ks * Cfg::kTileBytes);
             umma_commit_1(s_full(t));
             umma_commit_1(empty(ks));
+            if (t == 0 && i == begin) umma_commit_1(started);
           }
           ++steps;
         } else if (i < end && leader) {
