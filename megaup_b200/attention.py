@@ -13,9 +13,10 @@ Row ``i`` of a sequence with ``Lq`` queries and ``Lk`` keys stands at position
 
 ``out = softmax(scale * q k^T) v`` over the visible keys, query head ``h`` using
 key/value head ``h // (heads_q // heads_kv)``. A row that sees no key gets 0. A
-key that no query row sees has no influence, whatever it holds; an infinity or
-NaN in a key or value row that some query sees may reach the other rows of the
-same block of queries.
+key that no query row sees and a row that sees no key have no influence and the
+gradient 0, whatever they hold; an infinity or NaN in a key or value row that
+some query sees may reach the other rows of the same block of queries (backward:
+one in a row of the gradient or a query the other keys of a block of keys).
 
 BF16 in and out, FP32 sums, one rounding of the probabilities (and, backward,
 of the score gradients) to BF16 for the second product and one of the results.

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   }
   if (lane < 2 * kDeltaRows && first + lane < p.total_rows) {
     const float l = p.lse[first + lane];
-    p.delta[first + lane] = mine;
+    p.delta[first + lane] = l == -INFINITY ? 0.0f : mine;  // whatever dO is where the row sees nothing
     p.lse2[first + lane] = l == -INFINITY ? INFINITY : l * kLog2e;
   }
 }
@@ -107,7 +107,7 @@ struct AttnDqConfig {
   // q and dO full, k full/empty, v full/empty, s full [2], dp full, ds full, done, drain
   static constexpr int kBars = 1 + 2 * kKStages + 2 * kVStages + 6;
   static constexpr int kOffWords = kOffBars + kBars * 8;
-  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kSmemBytes = kOffWords + 16;  // TMEM's address, abort, copies into the two rings
   static constexpr int kTmemDp = 256, kTmemDq = 384;
 };
 
@@ -130,6 +130,7 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
   const uint32_t dp_full = bar(kS + 2), ds_full = bar(kS + 3), done = bar(kS + 4), drain = bar(kS + 5);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  volatile uint32_t* copies = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 8);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
   const int head = job % p.shape.heads_q;
@@ -150,7 +151,7 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
   const int n = tiles.count;
 
   if (threadIdx.x == 0) {
-    *abort_flag = 0u;
+    *abort_flag = 0u, copies[0] = copies[1] = 0u;
     for (int i = 0; i < Cfg::kBars; ++i) mbar_init(bar(i), bar(i) == ds_full ? 256 : 1);
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -167,8 +168,7 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
   if (warp >= 8) {
     fewer_registers<72>();
     if (warp == 8 && elect_one_sync() && n > 0) {
-      bool ok = true;
-      int i = 0;
+      int i = 0, key_copies = 0;
       auto load = [&](const CUtensorMap& map, uint32_t dst, uint32_t full, int row, int h) {
 #pragma unroll
         for (int panel = 0; panel < Cfg::kPanels; ++panel)
@@ -180,27 +180,15 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
       for (; i < n; ++i) {
         const int ks = i % Cfg::kKStages, vs = i % Cfg::kVStages;
         const int row = seq.k0 + tiles.tile(i) * kTileRows;
-        if (i >= Cfg::kKStages && !ctl.wait(k_empty(ks), (i / Cfg::kKStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
-          ok = false;
-          break;
-        }
+        if (i >= Cfg::kKStages && !ctl.wait(k_empty(ks), (i / Cfg::kKStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(k_full(ks), Cfg::kTileBytes);
         load(k_map, base + Cfg::kOffK + ks * Cfg::kTileBytes, k_full(ks), row, kv_head);
-        if (i >= Cfg::kVStages && !ctl.wait(v_empty(vs), (i / Cfg::kVStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
-          drain_barrier(k_full(ks), (i / Cfg::kKStages) & 1);
-          ok = false;
-          break;
-        }
+        ++key_copies;
+        if (i >= Cfg::kVStages && !ctl.wait(v_empty(vs), (i / Cfg::kVStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(v_full(vs), Cfg::kTileBytes);
         load(v_map, base + Cfg::kOffV + vs * Cfg::kTileBytes, v_full(vs), row, kv_head);
       }
-      if (!ok) {
-        drain_barrier(q_full, 0);
-        for (int m = max(0, i - Cfg::kKStages); m < i; ++m)
-          drain_barrier(k_full(m % Cfg::kKStages), (m / Cfg::kKStages) & 1);
-        for (int m = max(0, i - Cfg::kVStages); m < i; ++m)
-          drain_barrier(v_full(m % Cfg::kVStages), (m / Cfg::kVStages) & 1);
-      }
+      copies[0] = key_copies, copies[1] = i;
     } else if (warp == 9 && n > 0) {
       const bool leader = elect_one_sync();
       // S of tile i goes to buffer i % 2, where dS replaces it; dP has one buffer.
@@ -344,6 +332,11 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
     tc_fence_before_sync();
   }
   __syncthreads();
+  if (*abort_flag != 0u && threadIdx.x == 0 && n > 0) {  // the copies in flight end before their places are given up
+    drain_barrier(q_full, 0);
+    drain_ring(k_full(0), Cfg::kKStages, copies[0]);
+    drain_ring(v_full(0), Cfg::kVStages, copies[1]);
+  }
   if (warp == 9) {
     tc_fence_after_sync();
     tmem_dealloc<1>(tmem, 512);
@@ -386,7 +379,7 @@ struct AttnDkvConfig {
   // k and v full, q full/empty, dO full/empty, stats full/empty, s, dp, p, ds full, done, drain
   static constexpr int kBars = 1 + 2 * kQStages + 2 * kDoStages + 2 * kStatStages + 6;
   static constexpr int kOffWords = kOffBars + kBars * 8;
-  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kSmemBytes = kOffWords + 16;  // TMEM's address, abort, copies into the two rings
   static constexpr int kTmemDp = 128, kTmemDv = 256, kTmemDk = 384;
 };
 
@@ -412,6 +405,7 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
   const uint32_t done = bar(kS + 4), drain = bar(kS + 5);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  volatile uint32_t* copies = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 8);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
   // ---- the key tile, and this CTA's share of the query tiles that see it
@@ -451,7 +445,7 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
   if (share > 0 && n == 0) return;  // (the joining kernel knows)
 
   if (threadIdx.x == 0) {
-    *abort_flag = 0u;
+    *abort_flag = 0u, copies[0] = copies[1] = 0u;
     for (int i = 0; i < Cfg::kBars; ++i) {
       const uint32_t b = bar(i);
       const bool all_threads = b == p_full || b == ds_full || (b >= stat_empty(0) && b < s_full);
@@ -472,8 +466,7 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
   if (warp >= 8) {
     fewer_registers<72>();
     if (warp == 8 && elect_one_sync() && n > 0) {
-      bool ok = true;
-      int i = 0;
+      int i = 0, query_copies = 0;
       auto load = [&](const CUtensorMap& map, uint32_t dst, uint32_t full, int row, int h) {
 #pragma unroll
         for (int panel = 0; panel < Cfg::kPanels; ++panel)
@@ -486,27 +479,15 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
         const int qs = i % Cfg::kQStages, ds = i % Cfg::kDoStages;
         const int head = kv_head * group + (begin + i) / q_tiles;
         const int row = seq.q0 + (q_tile0 + (begin + i) % q_tiles) * kTileRows;
-        if (i >= Cfg::kQStages && !ctl.wait(q_empty(qs), (i / Cfg::kQStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
-          ok = false;
-          break;
-        }
+        if (i >= Cfg::kQStages && !ctl.wait(q_empty(qs), (i / Cfg::kQStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(q_full(qs), Cfg::kTileBytes);
         load(q_map, base + Cfg::kOffQ + qs * Cfg::kTileBytes, q_full(qs), row, head);
-        if (i >= Cfg::kDoStages && !ctl.wait(do_empty(ds), (i / Cfg::kDoStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) {
-          drain_barrier(q_full(qs), (i / Cfg::kQStages) & 1);
-          ok = false;
-          break;
-        }
+        ++query_copies;
+        if (i >= Cfg::kDoStages && !ctl.wait(do_empty(ds), (i / Cfg::kDoStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(do_full(ds), Cfg::kTileBytes);
         load(do_map, base + Cfg::kOffDo + ds * Cfg::kTileBytes, do_full(ds), row, head);
       }
-      if (!ok) {
-        drain_barrier(kv_full, 0);
-        for (int m = max(0, i - Cfg::kQStages); m < i; ++m)
-          drain_barrier(q_full(m % Cfg::kQStages), (m / Cfg::kQStages) & 1);
-        for (int m = max(0, i - Cfg::kDoStages); m < i; ++m)
-          drain_barrier(do_full(m % Cfg::kDoStages), (m / Cfg::kDoStages) & 1);
-      }
+      copies[0] = query_copies, copies[1] = i;
     } else if (warp == 10) {
       // ------------------------------------------- lse and delta of the query rows
       grid_dep_wait();
@@ -534,11 +515,14 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
       }
     } else if (warp == 9 && n > 0) {
       const bool leader = elect_one_sync();
-      // the rows of a query tile behind the sequence's end (packed: the next sequence's) become 0
+      // rows that see nothing, and those of a query tile behind the sequence's end (packed: the next sequence's), become 0
+      const int blind = !p.shape.causal && has_sinks ? 0 : -seq.off - p.shape.right;  // so many first ones
       auto clean = [&](int i, uint8_t* where) {
         const int row0 = (q_tile0 + (begin + i) % q_tiles) * kTileRows;
-        if (p.shape.sequences == nullptr || row0 + kTileRows <= seq.nq) return;
-        zero_tile_rows<DP>(where, seq.nq - row0, kTileRows, lane);
+        const bool ends = p.shape.sequences != nullptr && row0 + kTileRows > seq.nq;
+        if (row0 >= blind && !ends) return;
+        if (row0 < blind) zero_tile_rows<DP>(where, 0, min(blind - row0, kTileRows), lane);
+        if (ends) zero_tile_rows<DP>(where, seq.nq - row0, kTileRows, lane);
         fence_proxy_async_smem();
         __syncwarp();
       };
@@ -661,6 +645,10 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
         uint32_t g[32];
         tmem_ld_32x32(tmem + Cfg::kTmemDp + half * 64 + b * 32 + lane_base, g);
         tmem_ld_wait();
+        if (!full) {  // where P is 0 the key's value row may hold anything
+#pragma unroll
+          for (int x = 0; x < 32; ++x) g[x] = s[b][x] == 0u ? 0u : g[x];
+        }
         uint32_t packed[16];
 #pragma unroll
         for (int x = 0; x < 32; x += 4) {
@@ -733,6 +721,11 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
     tc_fence_before_sync();
   }
   __syncthreads();
+  if (*abort_flag != 0u && threadIdx.x == 0 && n > 0) {  // the copies in flight end before their places are given up
+    drain_barrier(kv_full, 0);
+    drain_ring(q_full(0), Cfg::kQStages, copies[0]);
+    drain_ring(do_full(0), Cfg::kDoStages, copies[1]);
+  }
   if (warp == 9) {
     tc_fence_after_sync();
     tmem_dealloc<1>(tmem, 512);

@@ -309,6 +309,11 @@ __device__ __forceinline__ void drain_barrier(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return;
 }
 
+// The last of `loads` copies into a ring of `stages` end: a wait ran out, and their places are about to be given up.
+__device__ __forceinline__ void drain_ring(uint32_t full, int stages, int loads) {
+  for (int n = max(0, loads - stages); n < loads; ++n) drain_barrier(full + n % stages * 8, (n / stages) & 1);
+}
+
 // Rows [from, to) of a tile that is in shared memory become zero. The whole warp calls it; the tile's next reader is
 // a product (async proxy).
 template <int DP>

@@ -47,7 +47,7 @@ struct AttnForwardConfig {
   // q full [2], stage full, stage empty, s full [2], half of p full [2][2], done [2], drain [2], started
   static constexpr int kBars = 2 + 2 * kStages + 8 + 2 + 1;
   static constexpr int kOffWords = kOffBars + kBars * 8;
-  static constexpr int kSmemBytes = kOffWords + 16;
+  static constexpr int kSmemBytes = kOffWords + 16;  // TMEM's address, abort, copies of K and V, sub-tiles with a Q
   static constexpr int kThreads = 384;
   static constexpr int kTmemO = 256;
 };
@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t started = bar(12 + 2 * Cfg::kStages);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffWords);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 4);
+  volatile uint32_t* copies = reinterpret_cast<volatile uint32_t*>(smem + Cfg::kOffWords + 8);
   const WaitControl ctl{abort_flag, p.shape.status, p.shape.timeout_ns};
 
   grid_dep_launch();
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(384, 1)
       const TileList all = block.all(p);
       int begin, end;
       block.share(p, all.count, begin, end);
-      *abort_flag = 0u;
+      *abort_flag = 0u, copies[0] = copies[1] = 0u;
       const int users = block.exists(p, 1) ? 2 : 1;  // warps that read a stage
       for (int s = 0; s < Cfg::kStages; ++s) {
         mbar_init(full(s), 1);
@@ -208,13 +209,7 @@ __global__ void __launch_bounds__(384, 1)
         if (i < end) ok = load(k_map, all.tile(i));
         if (ok) ok = load(v_map, all.tile(i - 1));
       }
-      if (!ok) {  // the copies in flight end before this CTA's shared memory is given up
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (block.exists(p, t)) drain_barrier(q_full(t), 0);
-        for (int n = max(0, loads - Cfg::kStages); n < loads; ++n)
-          drain_barrier(full(n % Cfg::kStages), (n / Cfg::kStages) & 1);
-      }
+      if (begin < end) copies[0] = loads, copies[1] = block.exists(p, 1) ? 2 : 1;
     } else if (warp == 9 || (warp == 10 && block.exists(p, 1))) {
       // ------------------------------------------------------------ products
       // One warp per sub-tile: the issue of a product waits for room in the tensor pipe's short queue, so with one
@@ -477,6 +472,10 @@ __global__ void __launch_bounds__(384, 1)
     tc_fence_before_sync();
   }
   __syncthreads();
+  if (*abort_flag != 0u && threadIdx.x == 0) {  // the copies in flight end before this CTA's shared memory is given up
+    for (int t = 0; t < static_cast<int>(copies[1]); ++t) drain_barrier(q_full(t), 0);
+    drain_ring(full(0), Cfg::kStages, copies[0]);
+  }
   if (warp == 9) {
     tc_fence_after_sync();
     tmem_dealloc<1>(*tmem_slot, 512);

@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(AttnTokensConfig<DP>::kThreads, kTokenCtas)
 
   float o[DP / 8][4] = {};
   float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  int loads = min(end - begin, Cfg::kStages);
   const float c2 = p.shape.scale_log2;
   if (warp == kTokenWarps) {
     __syncthreads();
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(AttnTokensConfig<DP>::kThreads, kTokenCtas)
         const int n = i - begin;
         if (!ctl.wait(empty(n % Cfg::kStages), (n / Cfg::kStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         load_tile(i);
+        ++loads;
       }
     }
   } else {
@@ -256,6 +258,10 @@ __global__ void __launch_bounds__(AttnTokensConfig<DP>::kThreads, kTokenCtas)
     }
   }
   __syncthreads();  // every tile has been read: the ring's place is used again
+  if (*abort_flag != 0u) {
+    if (loads_here) drain_ring(full(0), Cfg::kStages, loads);
+    __syncthreads();
+  }
 
   // ---- join the warps
   float* smem_o = reinterpret_cast<float*>(smem);  // [warps, rows, row floats]

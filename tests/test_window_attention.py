@@ -391,6 +391,57 @@ def test_unseen_keys_may_hold_anything() -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["k", "v", "both"])
+@pytest.mark.parametrize("causal, queries, dim", [(True, 300, 64), (True, 100, 128), (False, 77, 128)])
+def test_unseen_keys_have_no_gradient_whatever_they_hold(causal, queries, dim, where) -> None:
+    q, dout = _normal((1, queries, 4, dim), 1), _normal((1, queries, 4, dim), 2)
+    k, v = _normal((1, 1000, 2, dim), 3), _normal((1, 1000, 2, dim), 4)
+    low = 1000 - queries - 90  # the first key of the first row's window
+
+    def run():
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        out = mega_up.window_attention_bshd(*leaves, causal=causal, window=90, sinks=6)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    want = run()
+    for x in {"k": (k,), "v": (v,), "both": (k, v)}[where]:
+        x[:, 6:low] = float("nan")
+    for a, b in zip(want, run()):
+        assert torch.equal(a, b)
+    assert not want[2][:, 6:low].any() and not want[3][:, 6:low].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("settings, blind", [
+    (dict(window=50, sinks=3), 130), (dict(), 130), (dict(causal=False, window=(40, 20)), 110),
+])
+def test_rows_that_see_nothing_have_no_gradient_whatever_they_hold(settings, blind, packed) -> None:
+    queries, keys = 300, 170  # the first rows stand before the first key
+    rows = 2 * queries if packed else queries
+    q, dout = _normal((rows, 4, 64), 1), _normal((rows, 4, 64), 2)
+    k, v = _normal((rows // queries * keys, 2, 64), 3), _normal((rows // queries * keys, 2, 64), 4)
+    sequences = mega_up.prepare_packed_sequences([0, queries, 2 * queries], [0, keys, 2 * keys], device=DEVICE) if packed else None
+
+    def run():
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        if packed:
+            out = mega_up.window_attention_thd(*leaves, sequences, **settings)
+        else:
+            out = mega_up.window_attention_bshd(*(x[None] for x in leaves), **settings)[0]
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    want = run()
+    for start in range(0, rows, queries):
+        assert not want[0][start : start + blind].any() and not want[1][start : start + blind].any()
+        assert want[0][start + blind].any() and want[1][start + blind].any()
+        q[start : start + blind] = float("nan")
+        dout[start : start + blind] = float("inf")
+    for a, b in zip(want, run()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_slices_of_a_fused_projection_and_out() -> None:
     heads, kv_heads, dim, rows = 4, 2, 64, 333
     fused = _normal((rows, 2, heads + 2 * kv_heads, dim), 1)
