@@ -198,11 +198,15 @@ def _window_sides(window: object, causal: bool) -> tuple[int, int]:
     )
 
 
+def _layouts(*tensors: Tensor) -> list[tuple]:
+    return [(x.shape, x.stride(), x.dtype, x.device) for x in tensors]
+
+
 class _Plan:
     """The checks and the host arithmetic of a call, kept per set of shapes, strides
     and settings: the argument block without addresses, and the workspace sizes."""
 
-    __slots__ = ("kind", "block", "lse_shape", "forward_bytes", "backward_bytes", "tables")
+    __slots__ = ("kind", "block", "saved", "lse_shape", "forward_bytes", "backward_bytes", "tables")
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
@@ -275,6 +279,10 @@ class _Plan:
             sequences.sequences, sequences.q_blocks_256, sequences.q_blocks_128, sequences.k_blocks_128,
         )
         self.lse_shape = (heads, rows) if batch_axis is None else (batch, heads, rows)
+        # what a backward pass expects of q, k, v, out, lse and rest
+        dense = (q.shape, tuple(_dense_strides(q.shape)), q.dtype, q.device)
+        lse = (torch.Size(self.lse_shape), tuple(_dense_strides(self.lse_shape)), torch.float32, q.device)
+        self.saved = [*_layouts(q, k, v), dense, lse, dense]
         self.forward_bytes, self.backward_bytes = forward.value, backward.value
 
     def arguments(self, q: Tensor, k: Tensor, v: Tensor) -> _native.MupWindowAttention:
@@ -283,6 +291,31 @@ class _Plan:
         if (addresses[0] | addresses[1] | addresses[2]) % 16:
             raise ValueError(f"q, k and v must be 16-byte aligned, got addresses {[hex(x) for x in addresses]}")
         return a
+
+    def saved_arguments(self, saved: Sequence[Tensor]) -> tuple[_native.MupWindowAttention, list[Tensor]]:
+        """The block of a backward pass, and ``q, k, v, out, lse, rest`` as its copies may read them. A hook of saved
+        tensors (offloading, checkpointing) may return them with other strides or addresses than the forward pass had."""
+
+        tensors, restrided = list(saved), []
+        for i, (want, got) in enumerate(zip(self.saved, _layouts(*saved))):
+            x = tensors[i]
+            if want == got and x.data_ptr() % 16 == 0:
+                continue
+            name = ("q", "k", "v", "out", "lse", "rest")[i]
+            if (want[0], *want[2:]) != (got[0], *got[2:]):
+                raise RuntimeError(
+                    f"the saved {name} was {want[2]} {tuple(want[0])} on {want[3]}, a hook of saved tensors returned "
+                    f"{got[2]} {tuple(got[0])} on {got[3]}"
+                )
+            if not (_rows_are_loadable(x) if i < 3 else x.is_contiguous() and x.data_ptr() % 16 == 0):
+                x = tensors[i] = x.clone(memory_format=torch.contiguous_format)
+            if i < 3:
+                restrided.append((name, x))
+        a = self.arguments(*tensors[:3])
+        for name, x in restrided:
+            setattr(a, name + "_strides", _stride_array(x.shape, x.stride(), self.kind))
+        a.out, a.lse, a.out_rest = (x.data_ptr() for x in tensors[3:])
+        return a, tensors
 
     def launch(self, function: str, a: _native.MupWindowAttention, workspace_bytes: int, q: Tensor) -> None:
         """On the current stream of the device of ``q``."""
@@ -376,15 +409,14 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return None, None, None, None
-        q, k, v, out, lse, rest = ctx.saved_tensors
         plan: _Plan = ctx.plan
-        a = plan.arguments(q, k, v)
+        a, (q, k, v, *_) = plan.saved_arguments(ctx.saved_tensors)
         if not _rows_are_loadable(dout):  # a broadcast or transposed gradient
             dout = dout.clone(memory_format=torch.contiguous_format)
         elif not dout.is_contiguous():
             a.dout_strides = _stride_array(dout.shape, dout.stride(), plan.kind)
         dq, dk, dv = grads = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v)]
-        a.out, a.out_rest, a.lse, a.dout = out.data_ptr(), rest.data_ptr(), lse.data_ptr(), dout.data_ptr()
+        a.dout = dout.data_ptr()
         a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         plan.launch("mup_window_attention_backward", a, plan.backward_bytes, q)
         return (*grads, None)
