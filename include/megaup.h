@@ -104,6 +104,16 @@ int mup_set_max_active_ctas(int max_ctas);
 int mup_status_create(uint32_t **host_ptr, void **device_ptr);
 int mup_status_destroy(uint32_t *host_ptr);
 
+/* Kernels that are given no word (mup_window_attention_*) report in one that the
+ * library keeps per device, created at its first use. Their next launch on the
+ * device returns MUP_ERR_DEVICE_STATUS (and launches nothing); replays of a captured
+ * graph and a program's last call have no next launch. This reads that word and
+ * clears it, without a launch and without waiting: call it behind a synchronisation.
+ * `word` receives 0 or code << 24 | detail. `device_ptr` (may be NULL) receives the
+ * address the kernels are given, for plans and flag barriers that are to report in
+ * the same word. */
+int mup_device_status(int device, uint32_t *word, void **device_ptr);
+
 /* ---- symmetric-memory arena ---------------------------------------------- */
 
 /* Device-local physical allocation (cuMemCreate) of at least `bytes`, rounded

@@ -60,6 +60,7 @@ from .runtime import (
     DEFAULT_MAX_ROWS,
     SUPPORTED_UP_DEGREES,
     MegaUPRuntime,
+    check_status,
     initialize_emulated_group,
     initialize_runtime,
     supports_shape,
@@ -84,6 +85,7 @@ __all__ = [
     "axial_rotary_bshd",
     "axial_rotary_sbhd",
     "axial_rotary_thd",
+    "check_status",
     "emulated_peer_write",
     "emulated_pull",
     "headshard_pull_gemm_bshd",

@@ -109,6 +109,7 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "mup_set_max_active_ctas": (c_int, (c_int,)),
     "mup_status_create": (c_int, (POINTER(POINTER(c_uint32)), POINTER(c_void_p))),
     "mup_status_destroy": (c_int, (POINTER(c_uint32),)),
+    "mup_device_status": (c_int, (c_int, POINTER(c_uint32), POINTER(c_void_p))),
     "mup_arena_create": (c_int, (c_int, c_uint64, POINTER(c_void_p))),
     "mup_arena_import": (c_int, (c_int, c_int, c_uint64, POINTER(c_void_p))),
     "mup_arena_info": (c_int, (c_void_p, POINTER(c_void_p), POINTER(c_uint64), POINTER(c_int))),

@@ -167,33 +167,40 @@ int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], co
   return MUP_OK;
 }
 
-int device_status_word(int device, uint32_t** device_ptr) {
-  constexpr int kMaxDevices = 64;
+// The library's own status word of a device: its place on the host, null before its first use.
+constexpr int kMaxDevices = 64;
+struct DeviceWord {
+  uint32_t* host;
+  uint32_t* mapped;
+};
+static DeviceWord device_words[kMaxDevices];
+
+static int create_device_word(int device) {
   static std::mutex mutex;
-  static uint32_t* host[kMaxDevices];
-  static uint32_t* mapped[kMaxDevices];
+  DeviceWord& word = device_words[device];
+  if (__atomic_load_n(&word.host, __ATOMIC_ACQUIRE) != nullptr) return MUP_OK;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (word.host != nullptr) return MUP_OK;
+  // a pinned allocation is no stream operation: allowed while a stream is being captured
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  MUP_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  void *h = nullptr, *m = nullptr;
+  cudaError_t e = cudaHostAlloc(&h, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+  if (e == cudaSuccess) e = cudaHostGetDevicePointer(&m, h, 0);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return fail(MUP_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
+  memset(h, 0, 64);
+  word.mapped = static_cast<uint32_t*>(m);
+  __atomic_store_n(&word.host, static_cast<uint32_t*>(h), __ATOMIC_RELEASE);
+  return MUP_OK;
+}
+
+int device_status_word(int device, uint32_t** device_ptr) {
   if (device < 0 || device >= kMaxDevices) return fail(MUP_ERR_BAD_ARG, "device ordinal %d is out of range", device);
-  uint32_t* word = __atomic_load_n(&host[device], __ATOMIC_ACQUIRE);
-  if (word == nullptr) {
-    std::lock_guard<std::mutex> lock(mutex);
-    word = host[device];
-    if (word == nullptr) {
-      // a pinned allocation is no stream operation: allowed while a stream is being captured
-      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-      MUP_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-      void *h = nullptr, *m = nullptr;
-      cudaError_t e = cudaHostAlloc(&h, 64, cudaHostAllocMapped | cudaHostAllocPortable);
-      if (e == cudaSuccess) e = cudaHostGetDevicePointer(&m, h, 0);
-      cudaThreadExchangeStreamCaptureMode(&mode);
-      if (e != cudaSuccess) return fail(MUP_ERR_CUDA, "status word: %s", cudaGetErrorString(e));
-      memset(h, 0, 64);
-      mapped[device] = static_cast<uint32_t*>(m);
-      word = static_cast<uint32_t*>(h);
-      __atomic_store_n(&host[device], word, __ATOMIC_RELEASE);
-    }
-  }
-  *device_ptr = mapped[device];
-  const uint32_t seen = __atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL);
+  const int rc = create_device_word(device);
+  if (rc != MUP_OK) return rc;
+  *device_ptr = device_words[device].mapped;
+  const uint32_t seen = __atomic_exchange_n(device_words[device].host, 0u, __ATOMIC_ACQ_REL);
   if (seen != 0)
     return fail(MUP_ERR_DEVICE_STATUS,
                 "an earlier kernel of device %d gave up on a bounded wait (code %u, detail %u): the results of the "
@@ -1219,6 +1226,21 @@ int mup_status_create(uint32_t** host_ptr, void** device_ptr) {
 int mup_status_destroy(uint32_t* host_ptr) {
   if (host_ptr == nullptr) return MUP_OK;
   MUP_CUDA(cudaFreeHost(host_ptr));
+  return MUP_OK;
+}
+
+int mup_device_status(int device, uint32_t* word, void** device_ptr) {
+  if (word == nullptr) return fail(MUP_ERR_BAD_ARG, "null output");
+  if (device < 0 || device >= mup::kMaxDevices) return fail(MUP_ERR_BAD_ARG, "device ordinal %d is out of range", device);
+  if (device_ptr != nullptr) {
+    mup::DeviceScope scope(device);
+    MUP_CUDA(scope.error());
+    const int rc = mup::create_device_word(device);
+    if (rc != MUP_OK) return rc;
+    *device_ptr = mup::device_words[device].mapped;
+  }
+  uint32_t* host = __atomic_load_n(&mup::device_words[device].host, __ATOMIC_ACQUIRE);
+  *word = host == nullptr ? 0u : __atomic_exchange_n(host, 0u, __ATOMIC_ACQ_REL);
   return MUP_OK;
 }
 

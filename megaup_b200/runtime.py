@@ -194,6 +194,28 @@ class _StatusWord:
                 pass
 
 
+def check_status(device: torch.device | str | int | None = None) -> None:
+    """Raise if a ``window_attention_*`` kernel on ``device`` (default: the current one) gave up on a bounded wait.
+
+    A plain host load, no launch and no synchronisation: call it after the stream has been synchronised, above all
+    behind replays of a captured graph and a program's last call. The next ``window_attention_*`` call on the device
+    raises the same failure, once, whichever of the two comes first.
+    """
+
+    if not isinstance(device, int):
+        device = None if device is None else torch.device(device)
+        if device is not None and device.type != "cuda":
+            raise ValueError(f"check_status needs a CUDA device, got {device}")
+        device = torch.cuda.current_device() if device is None or device.index is None else device.index
+    word = ctypes.c_uint32()
+    _native.call("mup_device_status", device, ctypes.byref(word), None)
+    if word.value:
+        raise RuntimeError(
+            f"device-side failure on cuda:{device}: {_native.decode_status(word.value)}; the results of the "
+            "window_attention calls and graph replays enqueued since the last check are invalid"
+        )
+
+
 # --------------------------------------------------------------------------- FD exchange
 
 
@@ -401,11 +423,19 @@ class MegaUPRuntime:
         return None
 
     def check_status(self) -> None:
-        """Raise if a kernel of an earlier operation gave up on a bounded wait.
+        """Raise if a kernel of an earlier operation, or of the attention on this
+        device (``check_status`` of the package), gave up on a bounded wait.
 
-        The status word is written by the device; call after the stream has
+        The status words are written by the device; call after the stream has
         been synchronised to observe the outcome of the latest operation.
         """
+
+        self._check_operations()
+        if self.device.type == "cuda":
+            check_status(self.device)
+
+    def _check_operations(self) -> None:
+        """The arena's own operations only: a host load without a call into the library."""
 
         if self._status is None:
             return
@@ -430,7 +460,7 @@ class MegaUPRuntime:
         raises ``RuntimeError`` here, at the next operation, so that a caller who
         never calls ``check_status()`` still hears of it."""
 
-        self.check_status()
+        self._check_operations()
         stream = torch.cuda.current_stream(self.device)
         handle = stream.cuda_stream
         with self._lease_lock:
@@ -446,7 +476,7 @@ class MegaUPRuntime:
         self._leased_stream = handle
         try:
             yield self
-            self.check_status()
+            self._check_operations()
         finally:
             self._leased_stream = None
             # Two event objects take turns: a wait enqueued on the one recorded by
@@ -830,7 +860,7 @@ def initialize_runtime(
         )
         runtime.barrier()
         torch.cuda.synchronize(device)
-        runtime.check_status()
+        runtime._check_operations()
     except Exception as exc:  # noqa: BLE001
         error = f"{type(exc).__name__}: {exc}"
     _gather_phase_errors(group, up, current, "peer buffer binding", error)
