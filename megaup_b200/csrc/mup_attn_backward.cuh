@@ -180,11 +180,11 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
       for (; i < n; ++i) {
         const int ks = i % Cfg::kKStages, vs = i % Cfg::kVStages;
         const int row = seq.k0 + tiles.tile(i) * kTileRows;
-        if (i >= Cfg::kKStages && !ctl.wait(k_empty(ks), (i / Cfg::kKStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
+        if (i >= Cfg::kKStages && !ctl.wait_alone(k_empty(ks), (i / Cfg::kKStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(k_full(ks), Cfg::kTileBytes);
         load(k_map, base + Cfg::kOffK + ks * Cfg::kTileBytes, k_full(ks), row, kv_head);
         ++key_copies;
-        if (i >= Cfg::kVStages && !ctl.wait(v_empty(vs), (i / Cfg::kVStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
+        if (i >= Cfg::kVStages && !ctl.wait_alone(v_empty(vs), (i / Cfg::kVStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(v_full(vs), Cfg::kTileBytes);
         load(v_map, base + Cfg::kOffV + vs * Cfg::kTileBytes, v_full(vs), row, kv_head);
       }
@@ -479,11 +479,11 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
         const int qs = i % Cfg::kQStages, ds = i % Cfg::kDoStages;
         const int head = kv_head * group + (begin + i) / q_tiles;
         const int row = seq.q0 + (q_tile0 + (begin + i) % q_tiles) * kTileRows;
-        if (i >= Cfg::kQStages && !ctl.wait(q_empty(qs), (i / Cfg::kQStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
+        if (i >= Cfg::kQStages && !ctl.wait_alone(q_empty(qs), (i / Cfg::kQStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(q_full(qs), Cfg::kTileBytes);
         load(q_map, base + Cfg::kOffQ + qs * Cfg::kTileBytes, q_full(qs), row, head);
         ++query_copies;
-        if (i >= Cfg::kDoStages && !ctl.wait(do_empty(ds), (i / Cfg::kDoStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
+        if (i >= Cfg::kDoStages && !ctl.wait_alone(do_empty(ds), (i / Cfg::kDoStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         mbar_arrive_expect_tx(do_full(ds), Cfg::kTileBytes);
         load(do_map, base + Cfg::kOffDo + ds * Cfg::kTileBytes, do_full(ds), row, head);
       }

@@ -285,11 +285,29 @@ struct WaitControl {
   uint32_t* status;
   uint64_t timeout_ns;
 
+  // The whole warp calls this, converged, and every lane leaves with the same result: a phase that ends just as the limit
+  // is reached must not send some lanes into the aligned instructions behind the wait and others out of the loop. Where a
+  // lane saw the phase's end at the first look, the others see it at poll's first one; where none did, all are here and
+  // vote. (A vote at the first look as well costs 3 to 4 % of a backward pass: it stands between the barrier and the issue.)
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t code) const {
     if (mbar_try_wait(bar, parity)) return true;
-    if (mbar_wait_bounded(bar, parity, abort_flag, timeout_ns)) return true;
+    const uint32_t lanes = __activemask();
+    if (__all_sync(lanes, poll(bar, parity))) return true;
     give_up(code);
     return false;
+  }
+  // One thread of a warp (the copies' issuer).
+  __device__ __forceinline__ bool wait_alone(uint32_t bar, uint32_t parity, uint32_t code) const {
+    if (mbar_try_wait(bar, parity) || poll(bar, parity)) return true;
+    give_up(code);
+    return false;
+  }
+  // (a failed try_wait has suspended the thread for a while: the clock and the flag may be read each time)
+  __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) const {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity))
+      if (*abort_flag != 0u || globaltimer_ns() - t0 > timeout_ns) return false;
+    return true;
   }
   __device__ __forceinline__ void give_up(uint32_t code) const {
     if (*abort_flag == 0u) {
@@ -302,11 +320,13 @@ struct WaitControl {
   }
 };
 
-// After an abort: waits for a copy or product in flight, whatever the abort flag says; the number of polls is bounded
-// (each may suspend the thread for about a microsecond at most).
+// After an abort: waits for a copy or product in flight, whatever the abort flag says, but no longer than a fifth of a
+// second (they end within microseconds).
+constexpr uint64_t kDrainNs = 200000000;
 __device__ __forceinline__ void drain_barrier(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < (1 << 20); ++i)
-    if (mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > kDrainNs) return;
 }
 
 // The last of `loads` copies into a ring of `stages` end: a wait ran out, and their places are about to be given up.

@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(384, 1)
       bool ok = true;
       const auto load = [&](const CUtensorMap& map, int kt) {
         const int s = loads % Cfg::kStages, use = loads / Cfg::kStages;
-        if (use > 0 && !ctl.wait(empty(s), (use - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) return false;
+        if (use > 0 && !ctl.wait_alone(empty(s), (use - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) return false;
         load_tile(block, map, kt, s);
         ++loads;
         return true;

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(AttnTokensConfig<DP>::kThreads, kTokenCtas)
     if (loads_here) {
       for (int i = begin + Cfg::kStages; i < end; ++i) {
         const int n = i - begin;
-        if (!ctl.wait(empty(n % Cfg::kStages), (n / Cfg::kStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
+        if (!ctl.wait_alone(empty(n % Cfg::kStages), (n / Cfg::kStages - 1) & 1, MUP_ST_PRODUCER_SLOT_TIMEOUT)) break;
         load_tile(i);
         ++loads;
       }
