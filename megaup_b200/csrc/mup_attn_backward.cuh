@@ -230,11 +230,6 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
           if (i + 1 == n) umma_commit_1(done);
         }
       }
-      if (!ok) {
-        if (leader) umma_commit_1(drain);
-        __syncwarp();
-        drain_barrier(drain, 0);
-      }
     }
   } else {
     more_registers<216>();
@@ -332,10 +327,15 @@ __device__ __forceinline__ void attention_dq(const AttnBackward& p, const CUtens
     tc_fence_before_sync();
   }
   __syncthreads();
-  if (*abort_flag != 0u && threadIdx.x == 0 && n > 0) {  // the copies in flight end before their places are given up
-    drain_barrier(q_full, 0);
-    drain_ring(k_full(0), Cfg::kKStages, copies[0]);
-    drain_ring(v_full(0), Cfg::kVStages, copies[1]);
+  if (*abort_flag != 0u) {  // (nobody sets it any more: all threads take this branch or none)
+    // a role may have issued its last product or copy before another gave up
+    if (warp == 9) drain_products(drain);
+    if (threadIdx.x == 0 && n > 0) {
+      drain_barrier(q_full, 0);
+      drain_ring(k_full(0), Cfg::kKStages, copies[0]);
+      drain_ring(v_full(0), Cfg::kVStages, copies[1]);
+    }
+    __syncthreads();
   }
   if (warp == 9) {
     tc_fence_after_sync();
@@ -571,11 +571,6 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
         }
         if (i + 1 < n) ok = score_gradient(i + 1);
       }
-      if (!ok) {
-        if (leader) umma_commit_1(drain);
-        __syncwarp();
-        drain_barrier(drain, 0);
-      }
     }
   } else {
     more_registers<216>();
@@ -721,10 +716,15 @@ __device__ __forceinline__ void attention_dkv(const AttnBackward& p, const CUten
     tc_fence_before_sync();
   }
   __syncthreads();
-  if (*abort_flag != 0u && threadIdx.x == 0 && n > 0) {  // the copies in flight end before their places are given up
-    drain_barrier(kv_full, 0);
-    drain_ring(q_full(0), Cfg::kQStages, copies[0]);
-    drain_ring(do_full(0), Cfg::kDoStages, copies[1]);
+  if (*abort_flag != 0u) {  // (nobody sets it any more: all threads take this branch or none)
+    // a role may have issued its last product or copy before another gave up
+    if (warp == 9) drain_products(drain);
+    if (threadIdx.x == 0 && n > 0) {
+      drain_barrier(kv_full, 0);
+      drain_ring(q_full(0), Cfg::kQStages, copies[0]);
+      drain_ring(do_full(0), Cfg::kDoStages, copies[1]);
+    }
+    __syncthreads();
   }
   if (warp == 9) {
     tc_fence_after_sync();

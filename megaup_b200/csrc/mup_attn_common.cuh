@@ -277,7 +277,9 @@ __device__ __forceinline__ void umma_tmem_by_cols(uint32_t d_tmem, uint32_t a_tm
 // ---------------------------------------------------------------------------
 // Bounded waits: a wait that runs out records its cause once, raises the CTA's
 // abort flag (every other wait then gives up too) and returns false; the role
-// leaves its loop and meets the others at the CTA's last barrier.
+// leaves its loop and meets the others at the CTA's last barrier. What is in
+// flight then ends (drain_products, drain_ring) before TMEM and shared memory
+// are given up.
 // ---------------------------------------------------------------------------
 
 struct WaitControl {
@@ -327,6 +329,13 @@ __device__ __forceinline__ void drain_barrier(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity))
     if (globaltimer_ns() - t0 > kDrainNs) return;
+}
+
+// After an abort, in a warp whose elected thread issued products (elect.sync chooses the same one every time): they end.
+__device__ __forceinline__ void drain_products(uint32_t bar) {
+  if (elect_one_sync()) umma_commit_1(bar);
+  __syncwarp();
+  drain_barrier(bar, 0);
 }
 
 // The last of `loads` copies into a ring of `stages` end: a wait ran out, and their places are about to be given up.

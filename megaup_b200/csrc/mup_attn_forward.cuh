@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(384, 1)
             tc_fence_after_sync();
             if (leader) {
               umma_tmem_by_cols<DP, 4, 8>(o_tmem, s_tmem, 32, v_tile, true);
-              umma_commit_1(done(t));
               umma_commit_1(empty(vs));
+              umma_commit_1(done(t));  // the last arrival from a product: nothing reaches this CTA's barriers after it
             }
           } else if (ok && leader) {
             mbar_arrive(empty(vs));
@@ -287,11 +287,6 @@ __global__ void __launch_bounds__(384, 1)
         } else if (i < end && leader) {
           mbar_arrive(empty(ks));
         }
-      }
-      if (!ok) {
-        if (leader) umma_commit_1(drain(t));
-        __syncwarp();
-        drain_barrier(drain(t), 0);
       }
     }
   } else {
@@ -472,9 +467,14 @@ __global__ void __launch_bounds__(384, 1)
     tc_fence_before_sync();
   }
   __syncthreads();
-  if (*abort_flag != 0u && threadIdx.x == 0) {  // the copies in flight end before this CTA's shared memory is given up
-    for (int t = 0; t < static_cast<int>(copies[1]); ++t) drain_barrier(q_full(t), 0);
-    drain_ring(full(0), Cfg::kStages, copies[0]);
+  if (*abort_flag != 0u) {  // (nobody sets it any more: all threads take this branch or none)
+    // a role may have issued its last product or copy before another gave up
+    if (warp == 9 || warp == 10) drain_products(drain(warp - 9));
+    if (threadIdx.x == 0) {
+      for (int t = 0; t < static_cast<int>(copies[1]); ++t) drain_barrier(q_full(t), 0);
+      drain_ring(full(0), Cfg::kStages, copies[0]);
+    }
+    __syncthreads();
   }
   if (warp == 9) {
     tc_fence_after_sync();

@@ -24,11 +24,13 @@ def probe_library(tmp_path_factory):
     assert result.returncode == 0, result.stderr
     library = ctypes.CDLL(str(target))
     library.bounded_wait_probe.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_uint64] * 3 + [ctypes.c_int] * 2
+    library.products_probe.argtypes = [ctypes.c_void_p, ctypes.c_int]
     return library
 
 
 def test_the_probe_builds(probe_library) -> None:
     assert probe_library.bounded_wait_probe(None, None, None, 3_000_000_000, 0, 0, 0, 0) == -1
+    assert probe_library.products_probe(None, 0) == -1
 
 
 @pytest.fixture
@@ -81,3 +83,12 @@ def test_a_phase_that_ends_at_the_limit(probe) -> None:
                 seen.add(lanes[0])
             assert (status != 0) == any(lanes[0] == 0 for lanes in outcome)
     assert seen == {0, 1}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("repeats", [1, 500])
+def test_products_in_flight_end_in_the_drain(probe_library, repeats) -> None:
+    sums = torch.zeros(128, 128, device=DEVICE)
+    torch.cuda.synchronize()
+    assert probe_library.products_probe(sums.data_ptr(), repeats) == 0
+    assert bool((sums == 64.0).all())
