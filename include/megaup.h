@@ -327,7 +327,7 @@ int mup_regroup_rows_synced(void *dst, const void *src, int up, int batch, int64
  * keys; kv_lengths (device, optional) then holds the number of keys of each
  * sequence that count, the first ones. Packed form: batch = 1, seq_q and seq_k are
  * the total rows and `sequences` (device) holds, per sequence, {first query row,
- * queries, first key row, keys}; the block lists (device, 32-byte aligned) hold, for
+ * queries, first key row, keys} (16-byte aligned); the block lists (device, 32-byte aligned) hold, for
  * every block of 256 or 128 query rows or 128 key rows of a sequence, {sequence,
  * block's first row in it, the sequence's four numbers, 0, 0}. */
 typedef struct mup_window_attention {

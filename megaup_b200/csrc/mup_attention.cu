@@ -52,6 +52,30 @@ int check_tensor(const char* name, const void* base, const int64_t strides[3]) {
   return MUP_OK;
 }
 
+// What a launch reads besides the tensors. (The counts and lengths of the lists are the caller's; a list that is too short
+// for the longest sequence cannot be one of these sequences.)
+int check_tables(const mup_window_attention& a, bool backward) {
+  const auto misaligned = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+  if (misaligned(a.lse, 4) || misaligned(a.kv_lengths, 4) || misaligned(a.workspace, 16))
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: lse, kv_lengths or workspace is not aligned (4, 4, 16 bytes)");
+  if (a.sequences == nullptr) return MUP_OK;
+  if (misaligned(a.sequences, 16))
+    return host_fail(MUP_ERR_BAD_ARG, "window attention: sequences is not 16-byte aligned");
+  const struct {
+    const char* name;
+    const int32_t* list;
+    int count, needed;
+  } lists[] = {{"q_blocks_256", a.q_blocks_256, a.n_q_blocks_256, ceil_div(a.longest_q, 256)},
+               {"q_blocks_128", a.q_blocks_128, a.n_q_blocks_128, ceil_div(a.longest_q, 128)},
+               {"k_blocks_128", a.k_blocks_128, a.n_k_blocks_128, backward ? ceil_div(a.longest_k, 128) : 0}};
+  for (const auto& l : lists) {
+    if (l.count < l.needed || (l.count > 0 && (l.list == nullptr || misaligned(l.list, 32))))
+      return host_fail(MUP_ERR_BAD_ARG, "window attention: %s is null, not 32-byte aligned or has fewer than %d entries",
+                       l.name, l.needed);
+  }
+  return MUP_OK;
+}
+
 AttnShape make_shape(const mup_window_attention& a, uint32_t* status) {
   AttnShape s{};
   s.batch = a.batch, s.heads_q = a.heads_q, s.heads_kv = a.heads_kv;
@@ -381,6 +405,7 @@ int mup_window_attention_forward(const mup_window_attention* args, void* stream)
   if (rc == MUP_OK) rc = check_tensor("v", args->v, args->v_strides);
   if (rc == MUP_OK) rc = check_tensor("out", args->out, args->out_strides);
   if (rc == MUP_OK && args->out_rest != nullptr) rc = check_tensor("out_rest", args->out_rest, args->out_strides);
+  if (rc == MUP_OK) rc = check_tables(*args, false);
   if (rc == MUP_OK) rc = check_workspace(*args, forward_workspace(*args));
   if (rc != MUP_OK) return rc;
   DeviceScope scope(args->device);
@@ -407,6 +432,7 @@ int mup_window_attention_backward(const mup_window_attention* args, void* stream
   if (rc == MUP_OK) rc = check_tensor("dq", args->dq, args->dq_strides);
   if (rc == MUP_OK) rc = check_tensor("dk", args->dk, args->dk_strides);
   if (rc == MUP_OK) rc = check_tensor("dv", args->dv, args->dv_strides);
+  if (rc == MUP_OK) rc = check_tables(*args, true);
   if (rc != MUP_OK) return rc;
   DeviceScope scope(args->device);
   MUP_HOST_CUDA(scope.error());

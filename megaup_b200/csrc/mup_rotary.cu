@@ -227,6 +227,9 @@ extern "C" int mup_axial_rotary_launch(const mup_axial_rotary* args, void* strea
                      a.axes, a.heads[0], a.heads[1]);
   if (a.positions == nullptr || a.turns == nullptr || a.pair_axis == nullptr || a.position_type < 0 || a.position_type > 2)
     return host_fail(MUP_ERR_BAD_ARG, "axial rotary: positions or frequencies are missing");
+  if (reinterpret_cast<uintptr_t>(a.positions) % (a.position_type == MUP_ROTARY_INT64 ? 8 : 4) != 0 ||
+      reinterpret_cast<uintptr_t>(a.turns) % 8 != 0 || reinterpret_cast<uintptr_t>(a.pair_axis) % 4 != 0)
+    return host_fail(MUP_ERR_BAD_ARG, "axial rotary: positions or frequencies are not aligned to their type");
   RotaryParams p{};
   for (int t = 0; t < 2; ++t) {
     if (a.heads[t] == 0) continue;
