@@ -336,17 +336,19 @@ def _plan(
     sequences: PackedSequences | None, with_lengths: bool,
 ) -> _Plan:
     plans = _PLANS if sequences is None else sequences.plans
+    # (True and 1.0 are equal to 1 and would find its plan: what is no plain int is checked each time)
+    sides = window if window is None or type(window) is int else _window_sides(window, causal)
     try:
         key = (
             kind, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
-            q.device, k.device, v.device, causal, window, sinks, type(sinks), scale, with_lengths,
+            q.device, k.device, v.device, causal, sides, sinks, type(sinks), scale, with_lengths,
         )
         return plans[key]
-    except (KeyError, TypeError, AttributeError):  # new, a list as the window, not a tensor
+    except (KeyError, TypeError, AttributeError):  # new, not hashable, not a tensor
         plan = _Plan(kind, q, k, v, causal, window, sinks, scale, sequences, with_lengths)
     if len(plans) >= _MAX_PLANS:
         plans.clear()
-    plans[(*key[:14], tuple(window), *key[15:]) if isinstance(window, list) else key] = plan
+    plans[key] = plan
     return plan
 
 
