@@ -34,6 +34,7 @@ from operator import itemgetter
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _native
@@ -153,6 +154,15 @@ def _strides_are_loadable(tensor: Tensor) -> bool:
 
 def _rows_are_loadable(tensor: Tensor) -> bool:
     return tensor.data_ptr() % 16 == 0 and (tensor.is_contiguous() or _strides_are_loadable(tensor))
+
+
+def _refuse_tangents(what: str, *tensors: object) -> None:
+    """A kernel reads a dual tensor's value and would drop its tangent without a word. (Callers look at
+    ``forward_ad._current_level`` first: below 0 there are no dual tensors, and an attribute costs nothing.)"""
+
+    for x in tensors:
+        if isinstance(x, Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
 
 
 def _current_stream(device: int) -> int:
@@ -411,6 +421,8 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return None, None, None, None
+        if forward_ad._current_level >= 0:
+            _refuse_tangents("the gradient of window_attention", dout)
         plan: _Plan = ctx.plan
         a, (q, k, v, *_) = plan.saved_arguments(ctx.saved_tensors)
         if not _rows_are_loadable(dout):  # a broadcast or transposed gradient
@@ -431,6 +443,8 @@ def _attend(
     # plans are kept by these values: no object that can change (a tensor of one number) stands for them
     causal, scale = bool(causal), None if scale is None else float(scale)
     plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences, kv_lengths is not None)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(f"window_attention_{kind}", q, k, v, out)
     if kv_lengths is not None:
         _check_kv_lengths(kv_lengths, q, kind)
     if out is not None:
@@ -471,7 +485,7 @@ def window_attention_bshd(
     be passed as they are; ``D`` is a multiple of 8 up to 128. ``return_lse`` adds
     the FP32 ``[B,H,Sq]`` log-sum-exp of every row (no gradient flows through it).
     ``out`` is written instead of a new tensor; it may be ``q`` itself and overlaps
-    no other input. Differentiable in ``q``, ``k`` and ``v``.
+    no other input. Differentiable in ``q``, ``k`` and ``v``, once and in reverse mode.
     """
 
     return _attend("bshd", q, k, v, causal, window, sinks, scale, kv_lengths, None, out, return_lse)

@@ -23,11 +23,13 @@ from dataclasses import dataclass, field
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _native
 from .attention import (
-    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _row_strides, _rows_are_loadable, _strides_are_loadable,
+    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _refuse_tangents, _row_strides, _rows_are_loadable,
+    _strides_are_loadable,
 )
 from .ops import _tensor_signature
 
@@ -212,6 +214,8 @@ class _AxialRotary(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         (positions,) = ctx.saved_tensors
+        if forward_ad._current_level >= 0:
+            _refuse_tangents("the gradient of axial_rotary", *grads)
         # a broadcast or transposed gradient is laid out first
         grads = [g if _rows_are_loadable(g) else g.clone(memory_format=torch.contiguous_format) for g in grads]
         outputs = _fresh(grads)
@@ -246,6 +250,8 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
         raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
     tensors = (q,) if k is None else (q, k)
     block = _plan(kind, tensors, rotary, positions)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(f"axial_rotary_{kind}", *tensors, positions, *(out if isinstance(out, Sequence) else ()))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
@@ -274,7 +280,8 @@ def axial_rotary_bshd(
 
     ``positions`` (int32, int64 or float32 on the device) are ``[axes,S]``, shared
     by the batch, or ``[axes,B,S]``. ``out``: tensors of the same shapes to write;
-    each may be its own input and overlaps no input otherwise. Differentiable in ``q`` and ``k``.
+    each may be its own input and overlaps no input otherwise. Differentiable in ``q`` and ``k``, once and in reverse
+    mode; ``positions`` get no gradient.
     """
 
     return _rotate("bshd", q, k, rotary, positions, out)
