@@ -27,8 +27,10 @@ from __future__ import annotations
 
 import array
 import ctypes
+import math
 from collections.abc import Sequence
 from dataclasses import dataclass, field
+from functools import lru_cache
 from itertools import chain
 from operator import itemgetter
 
@@ -216,7 +218,7 @@ class _Plan:
     """The checks and the host arithmetic of a call, kept per set of shapes, strides
     and settings: the argument block without addresses, and the workspace sizes."""
 
-    __slots__ = ("kind", "block", "saved", "lse_shape", "forward_bytes", "backward_bytes", "tables")
+    __slots__ = ("kind", "block", "saved", "spans", "lse_shape", "forward_bytes", "backward_bytes", "tables")
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
@@ -292,6 +294,7 @@ class _Plan:
         # what a backward pass expects of q, k, v, out, lse and rest
         dense = (q.shape, tuple(_dense_strides(q.shape)), q.dtype, q.device)
         lse = (torch.Size(self.lse_shape), tuple(_dense_strides(self.lse_shape)), torch.float32, q.device)
+        self.spans = _span(q), _span(k), _span(v)
         self.saved = [*_layouts(q, k, v), dense, lse, dense]
         self.forward_bytes, self.backward_bytes = forward.value, backward.value
 
@@ -374,11 +377,71 @@ def _check_kv_lengths(kv_lengths: object, q: Tensor, kind: str) -> None:
         raise ValueError(f"kv_lengths must be contiguous int32 [{batch}] on {q.device}, got {_tensor_signature(kv_lengths)}")
 
 
-def _check_out(out: object, q: Tensor) -> None:
-    if not isinstance(out, Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError(f"out must be BF16 {tuple(q.shape)} on {q.device}, got {_tensor_signature(out)}")
-    if not _rows_are_loadable(out):
-        raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {out.stride()}")
+def _meet(distance: int, steps: list[tuple[int, int, int]]) -> bool:
+    """Whether ``distance`` is a sum of ``stride * t`` with ``low <= t <= high``; ``steps`` are (stride, low, high), the
+    largest stride first."""
+
+    if not steps:
+        return distance == 0
+    (stride, low, high), rest = steps[0], steps[1:]
+    # what the other steps can reach leaves a few t, for strides that nest at most two
+    least, most = sum(s * l for s, l, _ in rest), sum(s * h for s, _, h in rest)
+    first, last = max(low, -((most - distance) // stride)), min(high, (distance - least) // stride)
+    return any(_meet(distance - stride * t, rest) for t in range(first, last + 1))
+
+
+@lru_cache(256)
+def _layouts_meet(
+    a_shape: Sequence[int], a_strides: Sequence[int], b_shape: Sequence[int], b_strides: Sequence[int], distance: int
+) -> bool:
+    """Whether tensors of one buffer share an element, the second's first one ``distance`` elements behind the first's.
+    Slices with the same strides are compared exactly (interleaved ones are apart), others only where both are dense."""
+
+    if distance == 0:
+        return True
+    dims = list(zip(a_shape, b_shape, a_strides, b_strides))
+    if all(s == t or m == 1 or n == 1 for m, n, s, t in dims):
+        # an element of `a` at i and one of `b` at j are the same where the sum of (i - j) * stride is the distance
+        return _meet(distance, sorted(((t if m == 1 else s, 1 - n, m - 1) for m, n, s, t in dims), reverse=True))
+    if list(a_strides) != _dense_strides(a_shape) or list(b_strides) != _dense_strides(b_shape):
+        return False
+    return -math.prod(b_shape) < distance < math.prod(a_shape)
+
+
+def _span(x: Tensor) -> int:
+    """Bytes from the first to the last element."""
+
+    return 2 * (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1)
+
+
+def _share_elements(a: Tensor, a_span: int, b: Tensor, b_span: int) -> bool:
+    """Whether two BF16 tensors of as many dimensions are known to share an element."""
+
+    distance = b.data_ptr() - a.data_ptr()
+    return -b_span < distance < a_span and _layouts_meet(a.shape, a.stride(), b.shape, b.stride(), distance // 2)
+
+
+def _is_same(a: Tensor, b: Tensor) -> bool:
+    """Element for element the same memory."""
+
+    return a is b or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and (
+        a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+    ))
+
+
+def _check_out(plan: _Plan, out: object, q: Tensor, k: Tensor, v: Tensor) -> None:
+    q_span, k_span, v_span = plan.spans
+    span = q_span
+    if out is not q:
+        if not isinstance(out, Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError(f"out must be BF16 {tuple(q.shape)} on {q.device}, got {_tensor_signature(out)}")
+        if not _rows_are_loadable(out):
+            raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {out.stride()}")
+        span = _span(out)
+        if _share_elements(out, span, q, q_span) and not _is_same(out, q):
+            raise ValueError("out may be q itself, and must not overlap it otherwise")
+    if _share_elements(out, span, k, k_span) or _share_elements(out, span, v, v_span):
+        raise ValueError("out must not overlap k or v")
 
 
 def _forward(
@@ -448,7 +511,7 @@ def _attend(
     if kv_lengths is not None:
         _check_kv_lengths(kv_lengths, q, kind)
     if out is not None:
-        _check_out(out, q)
+        _check_out(plan, out, q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")

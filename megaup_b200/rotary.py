@@ -28,8 +28,8 @@ from torch.autograd.graph import increment_version
 
 from . import _native
 from .attention import (
-    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _refuse_tangents, _row_strides, _rows_are_loadable,
-    _strides_are_loadable,
+    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _is_same, _refuse_tangents, _row_strides,
+    _rows_are_loadable, _share_elements, _span, _strides_are_loadable,
 )
 from .ops import _tensor_signature
 
@@ -146,14 +146,28 @@ def _check(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, position
         )
 
 
-def _check_outputs(out: object, tensors: Sequence[Tensor]) -> None:
+def _check_outputs(out: object, tensors: Sequence[Tensor], spans: Sequence[int]) -> None:
     if not isinstance(out, Sequence) or len(out) != len(tensors):
         raise ValueError(f"out must hold {len(tensors)} tensors")
-    for given, x in zip(out, tensors):
+    out_spans = list(spans)
+    for i, (given, x) in enumerate(zip(out, tensors)):
+        if given is x:
+            continue
         if not isinstance(given, Tensor) or given.shape != x.shape or given.dtype != x.dtype or given.device != x.device:
             raise ValueError(f"out must be BF16 {tuple(x.shape)} on {x.device}, got {_tensor_signature(given)}")
         if not _rows_are_loadable(given):
             raise ValueError(f"out must have contiguous heads at 16-byte aligned strides, got {given.stride()}")
+        out_spans[i] = _span(given)
+        if _share_elements(given, out_spans[i], x, spans[i]) and not _is_same(given, x):
+            raise ValueError("an output may be its own input, and must not overlap it otherwise")
+    if len(out) == 2:
+        (a, b), (q, k) = out, tensors
+        if (
+            _share_elements(a, out_spans[0], b, out_spans[1])
+            or (b is not k and _share_elements(a, out_spans[0], k, spans[1]))
+            or (a is not q and _share_elements(b, out_spans[1], q, spans[0]))
+        ):
+            raise ValueError("an output must not overlap the other one or its input")
 
 
 def _block(kind: str, tensors: Sequence[Tensor], rotary: AxialRotary, positions: Tensor) -> bytes:
@@ -219,15 +233,18 @@ class _AxialRotary(torch.autograd.Function):
         # a broadcast or transposed gradient is laid out first
         grads = [g if _rows_are_loadable(g) else g.clone(memory_format=torch.contiguous_format) for g in grads]
         outputs = _fresh(grads)
-        _turn(_plan(ctx.kind, grads, ctx.rotary, positions), ctx.kind, grads, outputs, positions, True)
+        block, _ = _plan(ctx.kind, grads, ctx.rotary, positions)
+        _turn(block, ctx.kind, grads, outputs, positions, True)
         return (None, None, None, None, *outputs)
 
 
 _MAX_PLANS = 512
 
 
-def _plan(kind: str, tensors: Sequence[Tensor | None], rotary: AxialRotary, positions: Tensor) -> bytes:
-    """The checked argument block of a call, kept per set of shapes and strides."""
+def _plan(
+    kind: str, tensors: Sequence[Tensor | None], rotary: AxialRotary, positions: Tensor
+) -> tuple[bytes, list[int]]:
+    """The checked argument block of a call and its tensors' spans, kept per set of shapes and strides."""
 
     try:
         q = tensors[0]
@@ -241,15 +258,15 @@ def _plan(kind: str, tensors: Sequence[Tensor | None], rotary: AxialRotary, posi
         _check(kind, tensors[0], tensors[1] if len(tensors) > 1 else None, rotary, positions)
     if len(rotary.plans) >= _MAX_PLANS:
         rotary.plans.clear()
-    block = rotary.plans[key] = _block(kind, tensors, rotary, positions)
-    return block
+    plan = rotary.plans[key] = _block(kind, tensors, rotary, positions), [_span(x) for x in tensors]
+    return plan
 
 
 def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: Tensor, out: object):
     if not isinstance(rotary, AxialRotary):
         raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
     tensors = (q,) if k is None else (q, k)
-    block = _plan(kind, tensors, rotary, positions)
+    block, spans = _plan(kind, tensors, rotary, positions)
     if forward_ad._current_level >= 0:
         _refuse_tangents(f"axial_rotary_{kind}", *tensors, positions, *(out if isinstance(out, Sequence) else ()))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -260,7 +277,7 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
         if out is None:
             outputs = _fresh(tensors)
         else:
-            _check_outputs(out, tensors)
+            _check_outputs(out, tensors, spans)
             outputs = out
             increment_version(outputs)  # autograd refuses a graph that had saved them
         _turn(block, kind, tensors, outputs, positions, False, dense=out is None)
