@@ -512,7 +512,9 @@ def _attend(
         _check_kv_lengths(kv_lengths, q, kind)
     if out is not None:
         _check_out(plan, out, q, k, v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (
+        q.requires_grad or k.requires_grad or v.requires_grad or (out is not None and out.requires_grad)
+    ):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
         if kv_lengths is not None:

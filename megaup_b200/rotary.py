@@ -278,6 +278,8 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
             outputs = _fresh(tensors)
         else:
             _check_outputs(out, tensors, spans)
+            if torch.is_grad_enabled() and any(x.requires_grad for x in out):
+                raise ValueError("out cannot be given when a gradient is wanted")
             outputs = out
             increment_version(outputs)  # autograd refuses a graph that had saved them
         _turn(block, kind, tensors, outputs, positions, False, dense=out is None)

@@ -92,3 +92,23 @@ def test_rotary(monkeypatch) -> None:
         got = call(*tensors, rotary, positions, out=out)
         assert got[0] is out[0] and got[1] is out[1]
     assert len(launches) == len(good)
+
+
+def test_an_output_of_a_graph_of_autograd(monkeypatch) -> None:
+    """Its gradient would go to what it held before."""
+
+    launches = stub_launches(monkeypatch)
+    rotary, positions = mega_up.prepare_axial_rotary([64], device="cpu"), torch.zeros(1, 8)
+    q, k = torch.zeros(1, 8, 2, 64, dtype=BF16), torch.zeros(1, 8, 2, 64, dtype=BF16)
+    leaf = torch.zeros(1, 8, 2, 64, dtype=BF16, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="gradient"):
+            mega_up.window_attention_bshd(q, k, k, out=out)
+        for outs in ((out, k), (q, out)):
+            with pytest.raises(ValueError, match="gradient"):
+                mega_up.axial_rotary_bshd(q, k, rotary, positions, out=outs)
+        assert not launches
+        with torch.no_grad():
+            mega_up.window_attention_bshd(q, k, k, out=out)
+            mega_up.axial_rotary_bshd(q, k, rotary, positions, out=(out, k))
+        launches.clear()
