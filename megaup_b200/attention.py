@@ -167,6 +167,17 @@ def _refuse_tangents(what: str, *tensors: object) -> None:
             raise NotImplementedError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
 
 
+def _refuse_tracing(what: str, *, is_a_node: bool) -> None:
+    """A tracer sees the result's allocation and not the kernel: what it records would return memory that nobody wrote.
+    (``is_a_node``: an autograd function, which ``torch.jit.trace`` records as a whole.)"""
+
+    recorded = not is_a_node and torch._C._is_tracing()
+    if not recorded and torch._C._len_torch_dispatch_stack():
+        recorded = torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+    if recorded:
+        raise RuntimeError(f"{what} cannot be recorded by make_fx or, without gradients, by torch.jit.trace")
+
+
 def _current_stream(device: int) -> int:
     """The stream's handle. (``torch.cuda.current_stream`` makes an object of it: 1.3 us of a short call's 11.)"""
 
@@ -519,8 +530,10 @@ def _attend(
             raise ValueError("out cannot be given when a gradient is wanted")
         if kv_lengths is not None:
             raise ValueError("kv_lengths is for tokens over a cache: there is no gradient through it")
+        _refuse_tracing(f"window_attention_{kind}", is_a_node=True)
         result, lse = _WindowAttention.apply(q, k, v, plan)
     else:
+        _refuse_tracing(f"window_attention_{kind}", is_a_node=False)
         result, lse = _forward(plan, q, k, v, out, return_lse, kv_lengths)
     return (result, lse) if return_lse else result
 

@@ -28,8 +28,8 @@ from torch.autograd.graph import increment_version
 
 from . import _native
 from .attention import (
-    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _is_same, _refuse_tangents, _row_strides,
-    _rows_are_loadable, _share_elements, _span, _strides_are_loadable,
+    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _is_same, _refuse_tangents, _refuse_tracing,
+    _row_strides, _rows_are_loadable, _share_elements, _span, _strides_are_loadable,
 )
 from .ops import _tensor_signature
 
@@ -272,8 +272,10 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
+        _refuse_tracing(f"axial_rotary_{kind}", is_a_node=True)
         outputs = _AxialRotary.apply(block, kind, rotary, positions, *tensors)
     else:
+        _refuse_tracing(f"axial_rotary_{kind}", is_a_node=False)
         if out is None:
             outputs = _fresh(tensors)
         else:
