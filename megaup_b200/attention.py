@@ -514,6 +514,11 @@ def _attend(
     kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
     kv_lengths: Tensor | None, sequences: PackedSequences | None, out: Tensor | None, return_lse: bool,
 ):
+    if torch.compiler.is_dynamo_compiling():
+        # torch.compile's tracer mistakes the fields of an argument block: the call runs as it is, at a graph break
+        return torch.compiler.disable(_attend)(
+            kind, q, k, v, causal, window, sinks, scale, kv_lengths, sequences, out, return_lse
+        )
     # plans are kept by these values: no object that can change (a tensor of one number) stands for them
     causal, scale = bool(causal), None if scale is None else float(scale)
     plan = _plan(kind, q, k, v, causal, window, sinks, scale, sequences, kv_lengths is not None)

@@ -263,6 +263,8 @@ def _plan(
 
 
 def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: Tensor, out: object):
+    if torch.compiler.is_dynamo_compiling():  # see window_attention: run as it is, at a graph break
+        return torch.compiler.disable(_rotate)(kind, q, k, rotary, positions, out)
     if not isinstance(rotary, AxialRotary):
         raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
     tensors = (q,) if k is None else (q, k)
