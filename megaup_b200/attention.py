@@ -167,21 +167,24 @@ def _refuse_tangents(what: str, *tensors: object) -> None:
             raise NotImplementedError(f"{what} has no forward-mode derivative, and an argument carries a tangent")
 
 
-def _refuse_tracing(what: str, *, is_a_node: bool) -> None:
-    """A tracer sees the result's allocation and not the kernel: what it records would return memory that nobody wrote.
-    (``is_a_node``: an autograd function, which ``torch.jit.trace`` records as a whole.)"""
+# (bound once: a chain of attributes costs a tenth of a microsecond of a short call's ten)
+_is_compiled = torch.compiler.is_dynamo_compiling
+_is_traced = torch._C._is_tracing
+_dispatch_modes = torch._C._len_torch_dispatch_stack
 
-    recorded = not is_a_node and torch._C._is_tracing()
-    if not recorded and torch._C._len_torch_dispatch_stack():
-        recorded = torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
-    if recorded:
+
+def _refuse_tracing(what: str, *, is_a_node: bool) -> None:
+    """For calls where ``_is_traced() or _dispatch_modes()``: a tracer sees the result's allocation and not the kernel,
+    and what it records would return memory that nobody wrote. (``is_a_node``: an autograd function, which
+    ``torch.jit.trace`` records as a whole.)"""
+
+    proxies = _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+    if proxies or (_is_traced() and not is_a_node):
         raise RuntimeError(f"{what} cannot be recorded by make_fx or, without gradients, by torch.jit.trace")
 
 
-def _current_stream(device: int) -> int:
-    """The stream's handle. (``torch.cuda.current_stream`` makes an object of it: 1.3 us of a short call's 11.)"""
-
-    return torch._C._cuda_getCurrentRawStream(device)
+# The handle of a device's current stream. (``torch.cuda.current_stream`` makes an object of it: 1.3 us of a short call's 11.)
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dense_strides(shape: Sequence[int]) -> list[int]:
@@ -221,15 +224,23 @@ def _window_sides(window: object, causal: bool) -> tuple[int, int]:
     )
 
 
-def _layouts(*tensors: Tensor) -> list[tuple]:
-    return [(x.shape, x.stride(), x.dtype, x.device) for x in tensors]
+def _saved_layouts(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, rest: Tensor) -> tuple:
+    """What decides whether a backward pass may go by the forward pass's block. (Sizes as bytes: four microseconds of a
+    short call's 120 with all shapes and types, two without.)"""
+
+    return (
+        q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype,
+        out.is_contiguous(), lse.is_contiguous(), rest.is_contiguous(),
+        q.nbytes, k.nbytes, v.nbytes, out.nbytes, lse.nbytes, rest.nbytes,
+        q.device, k.device, v.device, out.device, lse.device, rest.device,
+    )
 
 
 class _Plan:
     """The checks and the host arithmetic of a call, kept per set of shapes, strides
     and settings: the argument block without addresses, and the workspace sizes."""
 
-    __slots__ = ("kind", "block", "saved", "spans", "lse_shape", "forward_bytes", "backward_bytes", "tables")
+    __slots__ = ("kind", "block", "device", "index", "shapes", "saved", "spans", "lse_shape", "forward_bytes", "backward_bytes", "tables")
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
@@ -303,10 +314,12 @@ class _Plan:
         )
         self.lse_shape = (heads, rows) if batch_axis is None else (batch, heads, rows)
         # what a backward pass expects of q, k, v, out, lse and rest
-        dense = (q.shape, tuple(_dense_strides(q.shape)), q.dtype, q.device)
-        lse = (torch.Size(self.lse_shape), tuple(_dense_strides(self.lse_shape)), torch.float32, q.device)
         self.spans = _span(q), _span(k), _span(v)
-        self.saved = [*_layouts(q, k, v), dense, lse, dense]
+        lse = q.new_empty(self.lse_shape, dtype=torch.float32, device="meta")
+        dense = q.new_empty(q.shape, device="meta")
+        self.shapes = q.shape, k.shape, v.shape, q.shape, lse.shape, q.shape
+        self.saved = (*_saved_layouts(q, k, v, dense, lse, dense)[:-6], *[q.device] * 6)
+        self.device, self.index = q.device, q.device.index
         self.forward_bytes, self.backward_bytes = forward.value, backward.value
 
     def arguments(self, q: Tensor, k: Tensor, v: Tensor) -> _native.MupWindowAttention:
@@ -320,23 +333,25 @@ class _Plan:
         """The block of a backward pass, and ``q, k, v, out, lse, rest`` as its copies may read them. A hook of saved
         tensors (offloading, checkpointing) may return them with other strides or addresses than the forward pass had."""
 
-        tensors, restrided = list(saved), []
-        for i, (want, got) in enumerate(zip(self.saved, _layouts(*saved))):
-            x = tensors[i]
-            if want == got and x.data_ptr() % 16 == 0:
-                continue
-            name = ("q", "k", "v", "out", "lse", "rest")[i]
-            if (want[0], *want[2:]) != (got[0], *got[2:]):
+        q, k, v, out, lse, rest = saved
+        if _saved_layouts(q, k, v, out, lse, rest) == self.saved:
+            a = _native.MupWindowAttention.from_buffer_copy(self.block)
+            a.q, a.k, a.v = aq, ak, av = q.data_ptr(), k.data_ptr(), v.data_ptr()
+            a.out, a.lse, a.out_rest = ao, al, ar = out.data_ptr(), lse.data_ptr(), rest.data_ptr()
+            if not (aq | ak | av | ao | al | ar) % 16:
+                return a, saved
+        tensors = list(saved)
+        for i, name in enumerate(("q", "k", "v", "out", "lse", "rest")):
+            x, shape, dtype = saved[i], self.shapes[i], torch.float32 if name == "lse" else torch.bfloat16
+            if x.shape != shape or x.dtype != dtype or x.device != self.device:
                 raise RuntimeError(
-                    f"the saved {name} was {want[2]} {tuple(want[0])} on {want[3]}, a hook of saved tensors returned "
-                    f"{got[2]} {tuple(got[0])} on {got[3]}"
+                    f"a hook of saved tensors returned {x.dtype} {tuple(x.shape)} on {x.device} for {name}, which was "
+                    f"{dtype} {tuple(shape)} on {self.device}"
                 )
             if not (_rows_are_loadable(x) if i < 3 else x.is_contiguous() and x.data_ptr() % 16 == 0):
-                x = tensors[i] = x.clone(memory_format=torch.contiguous_format)
-            if i < 3:
-                restrided.append((name, x))
+                tensors[i] = x.clone(memory_format=torch.contiguous_format)
         a = self.arguments(*tensors[:3])
-        for name, x in restrided:
+        for name, x in zip("qkv", tensors):
             setattr(a, name + "_strides", _stride_array(x.shape, x.stride(), self.kind))
         a.out, a.lse, a.out_rest = (x.data_ptr() for x in tensors[3:])
         return a, tensors
@@ -348,7 +363,7 @@ class _Plan:
             # freed with this frame: the allocator hands it out again in stream order
             workspace = q.new_empty(workspace_bytes, dtype=torch.uint8)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace_bytes
-        _native.call(function, ctypes.byref(a), _current_stream(a.device))
+        _native.call(function, ctypes.byref(a), _current_stream(self.index))
 
 
 _PLANS: dict[object, _Plan] = {}
@@ -514,7 +529,7 @@ def _attend(
     kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int, scale: float | None,
     kv_lengths: Tensor | None, sequences: PackedSequences | None, out: Tensor | None, return_lse: bool,
 ):
-    if torch.compiler.is_dynamo_compiling():
+    if _is_compiled():
         # torch.compile's tracer mistakes the fields of an argument block: the call runs as it is, at a graph break
         return torch.compiler.disable(_attend)(
             kind, q, k, v, causal, window, sinks, scale, kv_lengths, sequences, out, return_lse
@@ -535,10 +550,12 @@ def _attend(
             raise ValueError("out cannot be given when a gradient is wanted")
         if kv_lengths is not None:
             raise ValueError("kv_lengths is for tokens over a cache: there is no gradient through it")
-        _refuse_tracing(f"window_attention_{kind}", is_a_node=True)
+        if _dispatch_modes():
+            _refuse_tracing(f"window_attention_{kind}", is_a_node=True)
         result, lse = _WindowAttention.apply(q, k, v, plan)
     else:
-        _refuse_tracing(f"window_attention_{kind}", is_a_node=False)
+        if _dispatch_modes() or _is_traced():
+            _refuse_tracing(f"window_attention_{kind}", is_a_node=False)
         result, lse = _forward(plan, q, k, v, out, return_lse, kv_lengths)
     return (result, lse) if return_lse else result
 

@@ -28,8 +28,8 @@ from torch.autograd.graph import increment_version
 
 from . import _native
 from .attention import (
-    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _is_same, _refuse_tangents, _refuse_tracing,
-    _row_strides, _rows_are_loadable, _share_elements, _span, _strides_are_loadable,
+    _AXES, _check_heads_tensor, _current_stream, _dense_strides, _dispatch_modes, _is_compiled, _is_same, _is_traced,
+    _refuse_tangents, _refuse_tracing, _row_strides, _rows_are_loadable, _share_elements, _span, _strides_are_loadable,
 )
 from .ops import _tensor_signature
 
@@ -263,7 +263,7 @@ def _plan(
 
 
 def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positions: Tensor, out: object):
-    if torch.compiler.is_dynamo_compiling():  # see window_attention: run as it is, at a graph break
+    if _is_compiled():  # see window_attention: run as it is, at a graph break
         return torch.compiler.disable(_rotate)(kind, q, k, rotary, positions, out)
     if not isinstance(rotary, AxialRotary):
         raise TypeError("rotary must be an AxialRotary from prepare_axial_rotary")
@@ -274,10 +274,12 @@ def _rotate(kind: str, q: Tensor, k: Tensor | None, rotary: AxialRotary, positio
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise ValueError("out cannot be given when a gradient is wanted")
-        _refuse_tracing(f"axial_rotary_{kind}", is_a_node=True)
+        if _dispatch_modes():
+            _refuse_tracing(f"axial_rotary_{kind}", is_a_node=True)
         outputs = _AxialRotary.apply(block, kind, rotary, positions, *tensors)
     else:
-        _refuse_tracing(f"axial_rotary_{kind}", is_a_node=False)
+        if _dispatch_modes() or _is_traced():
+            _refuse_tracing(f"axial_rotary_{kind}", is_a_node=False)
         if out is None:
             outputs = _fresh(tensors)
         else:

@@ -115,6 +115,17 @@ def test_the_gradients_do_not_change(kind, unpack) -> None:
 
 
 @pytest.mark.gpu
+def test_a_tensor_that_was_left_on_the_host_is_refused() -> None:
+    q, k, v = _fused(40, DEVICE)
+    for place in range(6):
+        count = iter(range(6))
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x.cpu() if next(count) == place else x):
+            out = mega_up.window_attention_bshd(q, k, v)
+        with pytest.raises(RuntimeError, match="hook of saved tensors"):
+            out.sum().backward()
+
+
+@pytest.mark.gpu
 def test_offloading_and_checkpointing() -> None:
     q, k, v = _fused(300, DEVICE)
     out = mega_up.window_attention_bshd(q, k, v, window=90)
