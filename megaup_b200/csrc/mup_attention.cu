@@ -155,8 +155,9 @@ TokenPlan plan_tokens(const mup_window_attention& a) {
   const int64_t most = std::max<int64_t>(1, ceil_div(visible, kTokenKeys));
   const int64_t fill = std::max<int64_t>(1, kTokenCtas * kSms / places);
   TokenPlan t{};
-  // Short: joined within a cluster, without a workspace and a second launch. Measured with 8 heads over 256 / 1024 / 2000
-  // keys: 5.7 / 7.2 / 8.3 us on the GPU (two launches about 6.2 / 6.5 / 7.0), but 11 us of host time a call instead of 15.
+  // Short: joined within a cluster, without a workspace and a second launch. Measured with 8 heads over 256 / 512 / 1024 /
+  // 2000 keys: a call takes 9 us of host time instead of 13, and replays of a graph 5.6 / 6.5 / 7.1 / 8.2 us instead of
+  // 6.0 / 6.1 / 6.2 / 7.0. The rule is that of calls; a graph of tokens over 512 keys and more would be better off without.
   if (most <= 4 * kTokenCluster) {
     t.splits = static_cast<int>(std::min<int64_t>({most, fill, kTokenCluster}));
     t.cluster = t.splits > 1;

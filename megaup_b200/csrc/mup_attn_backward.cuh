@@ -4,7 +4,11 @@
 // One launch of two kinds of CTAs, which both recompute S and dP: one walks the key tiles of a block of query rows and sums
 // dQ, one walks the query tiles of a block of key rows (over all heads of the group) and sums dK and dV. That is seven
 // products per pair of tiles where CTAs that share dQ would need five, but every sum stays in one CTA's TMEM: no atomics,
-// no FP32 gradient in memory, the same bits every time.
+// no FP32 gradient in memory, the same bits every time. (A shared dQ to which key tiles add in a fixed order would have
+// the same bits too; it was neither built nor measured.)
+//
+// Rounded to 16 bits: P for dV's product and dS for dK's and dQ's, whose other operands are BF16 and whose type is both
+// operands'. Each is off by at most 2^-8 of itself, as the gradients' own rounding; the FP32 values of P make dS.
 //
 // Bound by the board's power on long sequences: 65536 rows, window 4096, 4 heads of one group, 128 wide take 1632 us in
 // one launch (two launches 1770: the first one's last wave left SMs idle), seven products at 1.14 PFLOP/s.

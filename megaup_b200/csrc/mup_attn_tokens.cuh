@@ -6,6 +6,7 @@
 // take 16 keys of every tile each: S = Q K^T (m16n8k16, K by ldmatrix), softmax in registers, O += P V (V by
 // ldmatrix.trans). The warps of a CTA join their (maximum, sum, O) in shared memory; CTAs that share a sequence join
 // through the shared memory of their cluster where there are few, else through the workspace and the combining kernel.
+// Roundings are those of the 128-row kernel: P to BF16 for the second product, then the result.
 //
 // Measured on B200: one token of 4 heads over a window of 1024 keys 7.1 us; 16 tokens of 8 heads over caches of 8192 to
 // 65536 keys (308 MB) 57 us, 5.4 TB/s, 82 % of the copy rate. Two CTAs of three 32 KB tiles per SM; one of six 60 us, two of
