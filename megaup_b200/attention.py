@@ -240,7 +240,9 @@ class _Plan:
     """The checks and the host arithmetic of a call, kept per set of shapes, strides
     and settings: the argument block without addresses, and the workspace sizes."""
 
-    __slots__ = ("kind", "block", "device", "index", "shapes", "saved", "spans", "lse_shape", "forward_bytes", "backward_bytes", "tables")
+    __slots__ = (
+        "kind", "block", "device", "index", "shapes", "saved", "spans", "lse_shape", "forward_bytes", "backward_bytes", "tables",
+    )
 
     def __init__(
         self, kind: str, q: Tensor, k: Tensor, v: Tensor, causal: bool, window: object, sinks: int,
